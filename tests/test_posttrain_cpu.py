@@ -1,0 +1,146 @@
+"""Log-probabilities out of logits, policy and preference losses, gradient clipping: refusals, and the PyTorch forms that run where
+the kernels do not, against definitions written apart from them in fp64."""
+import math
+
+import pytest
+import torch
+
+from posttrain_oracle import policy_oracle, preference_oracle, token_oracle
+from trainscale_b200.optim import clip_grad_norm_
+from trainscale_b200.rl import clipped_policy_loss, preference_loss, token_log_probs
+
+
+def _gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+@pytest.mark.parametrize("cap", [0.0, 5.0])
+@pytest.mark.parametrize("shape", [(), (4,), (2, 3), (2, 3, 2)])
+def test_token_log_probs(shape, cap):
+    g = _gen(1)
+    z = torch.randn(*shape, 11, generator=g, dtype=torch.float64).mul_(3)
+    z.view(-1)[3] = -math.inf
+    y = torch.randint(0, 11, shape, generator=g)
+    if shape:
+        y.view(-1)[-1] = -100
+    z.requires_grad_()
+    a = dict(temperature=0.7, logit_softcapping=cap, logit_scale=1.5, return_entropy=True)
+    got, want = token_log_probs(z, y, **a), token_oracle(z, y, 0.7, cap, 1.5)
+    for x, w in zip(got, want):
+        torch.testing.assert_close(x, w, rtol=1e-12, atol=1e-12)
+    up = [torch.randn(shape, generator=g, dtype=torch.float64) for _ in range(2)]
+    ga, = torch.autograd.grad(got, z, up)
+    gb, = torch.autograd.grad(want, z, up)
+    torch.testing.assert_close(ga, gb, rtol=1e-10, atol=1e-12)
+
+
+def test_a_label_outside_the_vocabulary_gives_nan():
+    lp = token_log_probs(torch.zeros(3, 4), torch.tensor([4, -1, 3]))
+    assert lp.isnan().tolist() == [True, True, False]
+    assert float(token_log_probs(torch.zeros(1, 4), torch.tensor([-100]))) == 0
+    assert float(token_log_probs(torch.zeros(1, 4), torch.tensor([-100]), ignore_index=None)) != 0
+
+
+@pytest.mark.parametrize("per_token", [False, True])
+@pytest.mark.parametrize("reduction", ["sequence", "token", "constant"])
+def test_policy_loss(reduction, per_token):
+    g = _gen(2)
+    B, T = 4, 9
+    logp = torch.randn(B, T, generator=g, dtype=torch.float64)
+    old, ref = logp + 0.3 * torch.randn(B, T, generator=g), logp + torch.randn(B, T, generator=g)
+    adv = torch.randn(B, T, generator=g) if per_token else torch.randn(B, generator=g)
+    mask = (torch.rand(B, T, generator=g) < 0.6).long()
+    mask[2] = 0
+    logp[mask == 0], ref[mask == 0], old[mask == 0] = math.nan, math.inf, -math.inf       # what masked places hold is of no interest
+    x = logp.clone().requires_grad_()
+    loss, stats = clipped_policy_loss(x, old, adv, mask, ref, clip=0.2, clip_high=0.28, beta=0.1, reduction=reduction, max_len=12,
+                                      return_stats=True)
+    want, grad, want_stats = policy_oracle(logp, old, adv, mask, ref, 0.2, 0.28, 0.1, reduction, 12)
+    torch.testing.assert_close(loss, want, rtol=1e-10, atol=1e-12)
+    for a, b in zip(stats, want_stats):
+        torch.testing.assert_close(a, b, rtol=1e-10, atol=1e-12)
+    loss.backward()
+    torch.testing.assert_close(x.grad, grad, rtol=1e-10, atol=1e-12)
+    assert (x.grad[mask == 0] == 0).all()
+
+
+@pytest.mark.parametrize("normalized", [False, True])
+@pytest.mark.parametrize("kind", ["sigmoid", "robust", "hinge", "ipo"])
+def test_preference_loss(kind, normalized):
+    g = _gen(3)
+    P, T = 5, 8
+    lp = torch.randn(2 * P, T, generator=g, dtype=torch.float64)
+    ref = lp + torch.randn(2 * P, T, generator=g)
+    mask = torch.rand(2 * P, T, generator=g) < 0.7
+    mask[P + 1] = False
+    lp[~mask], ref[~mask] = math.nan, math.inf
+    a = (0.8, kind, 0.1, 0.0 if kind == "ipo" else 0.3, normalized, 0.2)
+    x = lp.clone().requires_grad_()
+    got = preference_loss(x, ref, mask, beta=a[0], loss_type=kind, label_smoothing=a[2], gamma=a[3], length_normalized=normalized,
+                          nll_weight=a[5])
+    want = preference_oracle(lp, ref, mask, *a)
+    for u, v in zip(got, want[:3]):
+        torch.testing.assert_close(u, v, rtol=1e-10, atol=1e-12)
+    got[0].backward()
+    torch.testing.assert_close(x.grad, want[3], rtol=1e-10, atol=1e-12)
+
+
+def test_gradients_against_differences():
+    g = _gen(4)
+    z, y = torch.randn(3, 5, generator=g, dtype=torch.float64, requires_grad=True), torch.tensor([0, 4, -100])
+    f = lambda z: token_log_probs(z, y, temperature=0.5, logit_softcapping=3.0, return_entropy=True)       # noqa: E731
+    assert torch.autograd.gradcheck(f, (z,)) and torch.autograd.gradgradcheck(f, (z,))
+    lp = torch.randn(4, 5, generator=g, dtype=torch.float64, requires_grad=True)
+    old, adv, mask = lp.detach() + 0.05, torch.randn(4, generator=g), torch.ones(4, 5)
+    assert torch.autograd.gradcheck(lambda p: clipped_policy_loss(p, old, adv, mask, old - 0.3, beta=0.3), (lp,))
+    assert torch.autograd.gradcheck(lambda p: preference_loss(p, old, mask, loss_type="ipo")[0], (lp,))
+
+
+def test_nothing_to_learn_from():
+    empty = torch.zeros(0, 4, requires_grad=True)
+    loss = clipped_policy_loss(empty, empty.detach(), torch.zeros(0), empty.detach())
+    loss.backward()
+    assert float(loss) == 0 and empty.grad.shape == (0, 4)
+    assert float(clipped_policy_loss(torch.zeros(3, 0), torch.zeros(3, 0), torch.zeros(3), torch.zeros(3, 0))) == 0
+    assert float(preference_loss(torch.zeros(0, 4), None, torch.zeros(0, 4))[0]) == 0
+    assert float(preference_loss(torch.zeros(2, 0), None, torch.zeros(2, 0))[0]) == pytest.approx(math.log(2))
+    assert token_log_probs(torch.zeros(0, 4), torch.zeros(0, dtype=torch.long)).shape == (0,)
+
+
+def test_refusals():
+    z, y = torch.zeros(2, 3, 5), torch.zeros(2, 3, dtype=torch.long)
+    for kw in (dict(temperature=0.0), dict(temperature=math.inf), dict(temperature=-1.0), dict(logit_softcapping=-1.0),
+               dict(logit_scale=-2.0), dict(logit_softcapping=math.nan)):
+        with pytest.raises(ValueError):
+            token_log_probs(z, y, **kw)
+    with pytest.raises(ValueError):
+        token_log_probs(z, y[:, :2])
+    with pytest.raises(ValueError):
+        token_log_probs(torch.zeros(2, 0), torch.zeros(2, dtype=torch.long))
+    with pytest.raises(TypeError):
+        token_log_probs(z, y.float())
+    with pytest.raises(TypeError):
+        token_log_probs(z.long(), y)
+    p, a, m = torch.zeros(2, 3), torch.zeros(2), torch.ones(2, 3)
+    for args, kw in (((p, p, a, m), dict(reduction="mean")), ((p, p, a, m), dict(beta=0.1)), ((p, p, a, m), dict(clip=-0.1)),
+                     ((p, p, a, m), dict(clip_high=math.nan)), ((p, p, a, m), dict(max_len=0)), ((p, p, a, m), dict(beta=math.inf)),
+                     ((p[0], p[0], a, m[0]), {}), ((p, p[:, :2], a, m), {}), ((p, p, torch.zeros(3), m), {}), ((p, p, a, m[:1]), {}),
+                     ((p, p, a, m, p[:1]), {})):
+        with pytest.raises(ValueError):
+            clipped_policy_loss(*args, **kw)
+    for args, kw in (((p, None, m), dict(loss_type="dpo")), ((p, None, m), dict(beta=0.0)), ((p, None, m), dict(beta=math.nan)),
+                     ((p, None, m), dict(label_smoothing=1.5)), ((p, None, m), dict(loss_type="robust", label_smoothing=0.5)),
+                     ((p, None, m), dict(loss_type="ipo", gamma=0.1)), ((p, None, m), dict(nll_weight=math.inf)),
+                     ((torch.zeros(3, 2), None, torch.zeros(3, 2)), {}), ((p, p[:1], m), {}), ((p, None, m[:, :1]), {}),
+                     ((p[0], None, m[0]), {})):
+        with pytest.raises(ValueError):
+            preference_loss(*args, **kw)
+
+
+def test_clipping_on_the_cpu_is_as_before():
+    ps = [torch.nn.Parameter(torch.zeros(3)), torch.nn.Parameter(torch.zeros(2, 2))]
+    for p in ps:
+        p.grad = torch.full_like(p, 2.0)
+    assert float(clip_grad_norm_(ps, 1.0)) == pytest.approx(math.sqrt(28))
+    assert float(ps[0].grad[0]) == pytest.approx(2 / math.sqrt(28), rel=1e-5)
+    assert float(clip_grad_norm_([torch.nn.Parameter(torch.zeros(1))], 1.0)) == 0

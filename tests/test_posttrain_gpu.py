@@ -1,0 +1,655 @@
+"""Kernels between a model's logits and its update (csrc/logprob.cu, csrc/posttrain.cu, csrc/gradnorm.cu) against definitions in
+fp64.  Tolerances count roundings: half a step of the result's type, and what fp32 exponentials and sums may be off by."""
+import math
+
+import pytest
+import torch
+
+from posttrain_oracle import policy_oracle, preference_oracle
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+HALF = {t: torch.finfo(t).eps / 2 for t in (torch.float32, torch.bfloat16, torch.float16)}
+F32 = HALF[torch.float32]
+
+
+def _gen(seed):
+    return torch.Generator(DEV).manual_seed(seed)
+
+
+def _near(got, want, tol):
+    """|got - want| <= tol elementwise; equal where not finite."""
+    got, want = got.double(), want.double()
+    finite = want.isfinite()
+    assert torch.equal(finite, got.isfinite()), "finite in other places"
+    off = (got - want).abs() - tol
+    worst = off.where(finite, -1.0).max() if off.numel() else torch.tensor(-1.0)
+    assert float(worst) <= 0, f"off by {float(worst):.3e} more than allowed"
+    assert torch.equal(got[~finite].nan_to_num(7.0), want[~finite].nan_to_num(7.0))
+
+
+# ------------------------------------------------------------------------------------------------ log-probabilities
+def _token64(z, y, temperature, cap, g, h):
+    """Log-probabilities, entropies, gradient, and what fp32 may be off by in each: rows' largest |logit| counts in the exponent's
+    rounding, the number of terms of a thread in a sum's, two units in the last place in an exponential's."""
+    V = z.shape[-1]
+    x = z.double()
+    t = torch.tanh(x / cap) if cap else None
+    v = (cap * t if cap else x) / temperature
+    slope = (1 - t * t if cap else torch.ones_like(x)) / temperature
+    used = y != -100
+    lse = torch.logsumexp(v, -1, keepdim=True)
+    lp = v - lse
+    p = lp.exp()
+    safe = lp.where(p > 0, 0.0)
+    at = y.where(used, 0).unsqueeze(-1)
+    logp = lp.gather(-1, at).squeeze(-1).where(used, 0.0)
+    H = -(p * safe).sum(-1)
+    big = v.where(v.isfinite(), 0.0).abs().amax(-1) + (cap / temperature if cap else 0.0)
+    tol = F32 * (8 * big + V / 256 + 64)
+    g, h = (torch.zeros_like(H) if d is None else d.double().where(used, 0.0) for d in (g, h))
+    one = torch.zeros_like(x).scatter_(-1, at, 1.0)
+    grad = slope * (one * g.unsqueeze(-1) - p * (g.unsqueeze(-1) + h.unsqueeze(-1) * (safe + H.unsqueeze(-1))))
+    size = slope.abs().amax(-1) * (g.abs() + h.abs() * (H + 1 + safe.abs().amax(-1)))
+    return logp, H.where(used, 0.0), grad, tol, tol * 4 * (1 + H), (size * tol * 4).unsqueeze(-1)
+
+
+def _check_tokens(z, y, temperature=1.0, cap=0.0, entropy=True, seed=0):
+    from trainscale_b200.rl import token_log_probs
+    g, h = (torch.randn(y.shape, device=DEV, generator=_gen(seed + i)) for i in (1, 2))
+    h = h if entropy else None
+    logp, H, grad, tol, tol_H, tol_grad = _token64(z, y, temperature, cap, g, h)
+    a = dict(temperature=temperature, logit_softcapping=cap, return_entropy=entropy)
+    out = token_log_probs(z, y, **a)
+    out = out if entropy else (out,)
+    _near(out[0], logp, tol + F32 * logp.abs().where(logp.isfinite(), 0.0))
+    if entropy:
+        _near(out[1], H, tol_H)
+    x = z.detach().requires_grad_()
+    again = token_log_probs(x, y, **a)
+    again = again if entropy else (again,)
+    assert all(torch.equal(u, v) for u, v in zip(out, again))
+    (d,) = torch.autograd.grad(again, x, (g, h) if entropy else (g,))
+    assert d.dtype == z.dtype and d.shape == z.shape
+    _near(d, grad, tol_grad + HALF[z.dtype] * grad.abs() * 1.01 + (2.0 ** -25 if z.dtype == torch.float16 else 0.0))
+    assert (d[y == -100] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", list(HALF))
+@pytest.mark.parametrize("V", [1, 2, 7, 8, 33, 1000, 1001, 4099, 32001])
+def test_token_log_probs(V, dtype):
+    z = (torch.randn(2, 9, V, device=DEV, generator=_gen(V)) * 3).to(dtype)
+    y = torch.randint(0, V, (2, 9), device=DEV, generator=_gen(V + 1))
+    y[0, :3] = -100
+    _check_tokens(z, y)
+
+
+@pytest.mark.parametrize("entropy", [False, True])
+@pytest.mark.parametrize("cap", [0.0, 20.0])
+@pytest.mark.parametrize("rows,V,dtype", [(1, 128256, torch.bfloat16), (9, 128256, torch.float32), (150, 50001, torch.float16),
+                                          (700, 32000, torch.bfloat16)])
+def test_token_log_probs_of_few_and_many_rows(rows, V, dtype, cap, entropy):
+    z = (torch.randn(rows, V, device=DEV, generator=_gen(rows)) * 6).to(dtype)
+    y = torch.randint(0, V, (rows,), device=DEV, generator=_gen(rows + 1))
+    _check_tokens(z, y, 0.6, cap, entropy)
+
+
+@pytest.mark.parametrize("V", [515, 520])
+def test_rows_that_lie_elsewhere(V):
+    """Slices, pitched rows, unaligned starts, transposed storage, one row, four dimensions."""
+    for dtype in HALF:
+        full = (torch.randn(3, 8, V + 5, device=DEV, generator=_gen(5)) * 2).to(dtype)
+        for z in (full[:, :-1, :V], full[:, 1:, 3:3 + V], full[::2, ::3, 5:], full[1, :, :V], full[0, 2, 1:1 + V],
+                  full[:, :, :V].transpose(1, 2).contiguous().transpose(1, 2), full[:, :, :V].unsqueeze(1).expand(3, 2, 8, V)):
+            y = torch.randint(0, z.shape[-1], z.shape[:-1], device=DEV, generator=_gen(6))
+            _check_tokens(z, y)
+
+
+@pytest.mark.parametrize("dtype", list(HALF))
+def test_logits_that_are_not_finite_or_far_apart(dtype):
+    from trainscale_b200.rl import token_log_probs
+    V = 777
+    z = torch.randn(8, V, device=DEV, generator=_gen(1)).to(dtype)
+    z[0, 1:] = -math.inf                                    # one token left
+    z[1, ::2] = -math.inf
+    z[2, :] = torch.finfo(dtype).min                        # a mask of the lowest value over everything
+    z[3, :-1] = torch.finfo(dtype).min
+    z[4, 5] = 3e4                                           # one that drowns the others
+    z[5] = 60000.0
+    z[6] *= 1e-4
+    y = torch.tensor([0, 2, 3, 776, 6, 1, 1, 0], device=DEV)
+    want = torch.log_softmax(z.double(), -1).gather(1, y.unsqueeze(1)).squeeze(1)
+    got, H = token_log_probs(z, y, return_entropy=True)
+    _near(got, want, F32 * (8 * z.double().where(z.isfinite() & (z > -1e4), 0.0).abs().amax(1) + 128) + F32 * want.abs().where(want.isfinite(), 0.0) * 2)
+    assert float(H[0]) == 0 and float(H[3]) == 0 and abs(float(H[2]) - math.log(V)) < 1e-5 and abs(float(H[5]) - math.log(V)) < 1e-5
+    x = z.clone().requires_grad_()
+    logp, H = token_log_probs(x, y, return_entropy=True)
+    (logp.where(logp.isfinite(), 0.0).sum() + H.sum()).backward()
+    assert x.grad.isfinite().all() and float(x.grad[0].abs().max()) == 0 and (x.grad[1, ::2] == 0)[1:].all()
+    bad = torch.zeros(5, V, device=DEV, dtype=dtype)
+    bad[0], bad[1, 700], bad[2, 3], bad[3, 3], bad[3, 4] = -math.inf, math.nan, math.inf, math.inf, math.nan
+    lp, H = token_log_probs(bad, torch.tensor([0, 0, 0, 3, 0], device=DEV), return_entropy=True)
+    assert lp[:2].isnan().all() and float(lp[2]) == -math.inf and lp[3].isnan() and lp[4].isfinite() and H[:4].isnan().all()
+    lp = token_log_probs(bad, torch.tensor([-100, -100, V, -1, 5], device=DEV))
+    assert (lp[:2] == 0).all() and lp[2:4].isnan().all()
+
+
+def test_rows_without_an_upstream_gradient_and_unused_results():
+    from trainscale_b200.rl import token_log_probs
+    z = torch.randn(6, 300, device=DEV, requires_grad=True)
+    y = torch.arange(6, device=DEV)
+    logp, H = token_log_probs(z, y, return_entropy=True)
+    w = torch.tensor([0.0, 1, 0, 2, 0, 3], device=DEV)
+    (a,) = torch.autograd.grad((logp * w).sum(), z, retain_graph=True)
+    assert (a[::2] == 0).all()
+    torch.testing.assert_close(a, torch.autograd.grad((torch.log_softmax(z, -1)[y, y] * w).sum(), z)[0], rtol=1e-5, atol=1e-6)
+    (b,) = torch.autograd.grad(H.sum(), z)
+    lp = torch.log_softmax(z, -1)
+    torch.testing.assert_close(b, torch.autograd.grad(-(lp.exp() * lp).sum(), z)[0], rtol=1e-4, atol=1e-6)
+    logp, H = token_log_probs(z, y, return_entropy=True)
+    logp *= 2                                               # results may be changed in place
+    H += 1
+    (logp.sum() + H.sum()).backward()
+
+
+def test_selective_log_softmax_keeps_its_results():
+    from trainscale_b200.rl import selective_log_softmax
+    y = torch.randint(0, 999, (4, 5), device=DEV)
+    for dtype, kw in ((torch.float32, dict(temperature=0.7, logit_softcapping=9.0, logit_scale=1.2)), (torch.float32, {}),
+                      (torch.bfloat16, {}), (torch.bfloat16, dict(temperature=0.7, logit_softcapping=9.0))):
+        z = (torch.randn(4, 5, 999, device=DEV, generator=_gen(3)) * 4).to(dtype)
+        v = z
+        if kw:
+            v = kw["logit_softcapping"] * torch.tanh(z / kw["logit_softcapping"])
+            v = v * kw.get("logit_scale", 1.0) / kw["temperature"] if "logit_scale" in kw else v / kw["temperature"]
+        want = v.gather(-1, y.unsqueeze(-1)).squeeze(-1).float() - torch.logsumexp(v.float(), -1)
+        torch.testing.assert_close(selective_log_softmax(z, y, **kw), want, rtol=2e-6, atol=2e-5)
+    z = torch.randn(3, 7, device=DEV, requires_grad=True)   # a gradient that is differentiated itself
+    (d,) = torch.autograd.grad(selective_log_softmax(z, torch.tensor([0, 3, 6], device=DEV)).sum(), z, create_graph=True)
+    (dd,) = torch.autograd.grad(d.pow(2).sum(), z)
+    x = z.detach().double().requires_grad_()
+    (e,) = torch.autograd.grad(torch.log_softmax(x, -1)[[0, 1, 2], [0, 3, 6]].sum(), x, create_graph=True)
+    (ee,) = torch.autograd.grad(e.pow(2).sum(), x)
+    torch.testing.assert_close(dd.double(), ee, rtol=1e-4, atol=1e-5)
+
+
+# ------------------------------------------------------------------------------------------------ policy loss
+MASKS = [torch.bool, torch.uint8, torch.int32, torch.int64, torch.float32, torch.bfloat16, torch.float16, torch.float64]
+
+
+def _policy_case(B, T, dtype, mask_type, seed, per_token=False, spoil=True):
+    g = _gen(seed)
+    logp = -torch.rand(B, T, device=DEV, generator=g) * 3
+    old = (logp + 0.15 * torch.randn(B, T, device=DEV, generator=g)).to(dtype)
+    ref = (logp + 0.4 * torch.randn(B, T, device=DEV, generator=g)).to(dtype)
+    logp = logp.to(dtype)
+    mask = torch.rand(B, T, device=DEV, generator=g) < 0.7
+    if B > 1:
+        mask[B // 2] = False
+    if spoil:
+        logp[~mask], old[~mask], ref[~mask] = math.nan, math.inf, -math.inf
+    adv = torch.randn(B, T, device=DEV, generator=g) if per_token else torch.randn(B, device=DEV, generator=g)
+    if not per_token and B > 2:
+        adv[0] = 0
+    mask = mask.to(mask_type)
+    if mask.is_floating_point():
+        mask = mask * 0.5                                   # weights count
+    return logp, old, adv, mask, ref
+
+
+def _check_policy(logp, old, adv, mask, ref, low=0.2, high=0.28, beta=0.1, reduction="sequence", length=None):
+    from trainscale_b200.rl import clipped_policy_loss
+    want, grad, stats = policy_oracle(logp, old, adv, mask, ref, low, high, beta, reduction, length or logp.shape[1])
+    # an exponential is off by 2^-22, its argument (a rounded difference of a few units) by as much: 2^-21 of every term
+    size = policy_oracle(logp, old, adv.abs(), mask, ref, -1e30, 1e30, 0.0, reduction, length or logp.shape[1])
+    kl_size = beta * 2 * float(policy_oracle(logp, old, adv * 0, mask, ref, low, high, 1.0, reduction, length or logp.shape[1])[0]) if ref is not None else 0
+    x = logp.clone().requires_grad_() if logp.is_contiguous() else logp.detach().requires_grad_()
+    loss, got = clipped_policy_loss(x, old, adv, mask, ref, clip=low, clip_high=high, beta=beta, reduction=reduction, max_len=length,
+                                    return_stats=True)
+    assert loss.dtype == torch.float32 and loss.dim() == 0
+    _near(loss, want, 2.0 ** -21 * (size[0].abs() + kl_size + want.abs()) + 1e-12)
+    for u, v in zip(got, stats):
+        _near(u, v, 2.0 ** -20 * v.abs() + 1e-9)
+    (d,) = torch.autograd.grad(loss, x, retain_graph=True)
+    assert d.dtype == logp.dtype and d.shape == logp.shape
+    m = mask.double()
+    d_ref = torch.where(m != 0, (ref.double() - logp.double()), 0.0).expm1().abs() if ref is not None else 0.0
+    w = (size[1].abs() + beta * d_ref * m)
+    tol = 2.0 ** -20 * w * 2 + HALF[logp.dtype] * grad.abs() * 1.01 + (2.0 ** -25 if logp.dtype == torch.float16 else 1e-30)
+    _near(d, grad, tol)
+    assert (d[mask == 0] == 0).all()
+    (again,) = torch.autograd.grad(loss, x, retain_graph=True)
+    assert torch.equal(d, again) and d.data_ptr() != again.data_ptr()
+    # another upstream gradient: one rounding of the scaled gradient, not two
+    s = torch.tensor(0.3, device=DEV)
+    (scaled,) = torch.autograd.grad(loss, x, s)
+    f = float(s)
+    _near(scaled, grad * f, tol * f + F32 * 2 * grad.abs() * f + (2.0 ** -25 if logp.dtype == torch.float16 else 0.0))
+    assert torch.equal(loss.detach(), clipped_policy_loss(x.detach(), old, adv, mask, ref, clip=low, clip_high=high, beta=beta,
+                                                          reduction=reduction, max_len=length))
+
+
+@pytest.mark.parametrize("reduction", ["sequence", "token", "constant"])
+@pytest.mark.parametrize("B,T", [(1, 1), (2, 1), (1, 7), (3, 33), (8, 61), (1025, 5), (257, 130), (5, 4099), (2, 70001), (3000, 17)])
+def test_policy_loss(B, T, reduction):
+    _check_policy(*_policy_case(B, T, torch.float32, torch.bool, B + T), reduction=reduction, length=None if T % 2 else T + 3)
+
+
+@pytest.mark.parametrize("mask_type", MASKS)
+@pytest.mark.parametrize("dtype", list(HALF))
+def test_policy_loss_types(dtype, mask_type):
+    for reduction, per_token in (("sequence", True), ("token", False)):
+        _check_policy(*_policy_case(9, 203, dtype, mask_type, 3, per_token), reduction=reduction)
+        logp, old, adv, mask, _ = _policy_case(130, 202, dtype, mask_type, 4, per_token)
+        _check_policy(logp, old, adv, mask, None, beta=0.0, reduction=reduction)
+
+
+def test_policy_loss_of_inputs_that_lie_elsewhere():
+    logp, old, adv, mask, ref = _policy_case(40, 70, torch.float32, torch.int64, 9, True)
+    _check_policy(logp[:, 1:], old[:, :-1].clone(), adv[:, 1:], mask[:, 1:], ref[:, 1:])
+    _check_policy(logp[::3, 5:50], old[::3, 5:50], adv[::3, 5:50], mask[::3, 5:50], ref[::3, 5:50])
+    one = mask[1:2].expand(40, 70)
+    logp, old, _, _, ref = _policy_case(40, 70, torch.float32, torch.bool, 9, spoil=False)
+    _check_policy(logp, old[:1].expand(40, 70), adv[:, 0], one, ref.t().contiguous().t())
+    _check_policy(logp.t(), old.t(), torch.randn(70, device=DEV, generator=_gen(1)), one.t(), ref.t(), reduction="token")
+    _check_policy(logp.bfloat16(), old, adv[:, 0], one, ref.half())                # three types: computed in fp32
+
+
+def test_policy_bounds_and_extremes():
+    from trainscale_b200.rl import clipped_policy_loss
+    up, down = math.log(1.2), math.log(0.8)
+    old = torch.zeros(1, 8, device=DEV)
+    f = lambda v, to: torch.nextafter(torch.tensor(v, dtype=torch.float32), torch.tensor(to, dtype=torch.float32)).item()      # noqa: E731
+    logp = torch.tensor([[f(up, 9.0), f(up, -9.0), f(down, 9.0), f(down, -9.0), 100.0, 100.0, -200.0, 0.0]], device=DEV)
+    for sign in (1.0, -1.0):
+        adv = torch.full((1,), sign, device=DEV)
+        x = logp.clone().requires_grad_()
+        clipped_policy_loss(x, old, adv, torch.tensor([[1, 1, 1, 1, 0, 0, 1, 1]], device=DEV)).backward()
+        _, want, _ = policy_oracle(logp, old, adv, torch.tensor([[1, 1, 1, 1, 0, 0, 1, 1]], device=DEV), None, 0.2, 0.2, 0.0, "sequence", 8)
+        _near(x.grad, want, 2.0 ** -20 * want.abs() + 2.0 ** -126)      # (e^-200 is below fp32)
+    zero = clipped_policy_loss(logp, old, torch.zeros(1, device=DEV), torch.ones(1, 8, device=DEV))
+    assert float(zero) == 0                                 # ratios that overflow have no say without an advantage
+    assert float(clipped_policy_loss(logp, old, torch.ones(1, device=DEV), torch.zeros(1, 8, device=DEV))) == 0
+    bad = logp.clone()
+    bad[0, 2] = math.nan
+    assert clipped_policy_loss(bad, old, torch.zeros(1, device=DEV), torch.ones(1, 8, device=DEV)).isnan()
+
+
+def test_group_relative_losses_keep_their_results():
+    from trainscale_b200 import rl
+    logp, old, adv, mask, ref = _policy_case(16, 300, torch.float32, torch.float32, 5, spoil=False)
+
+    def pytorch(kind, x, clip_high=0.2):
+        ratio = torch.exp(x - old)
+        obj = torch.minimum(ratio * adv[:, None], ratio.clamp(0.8, 1 + clip_high) * adv[:, None])
+        if kind == "dapo":
+            return -(obj * mask).sum() / mask.sum().clamp(min=1)
+        if kind == "drgrpo":
+            return -((obj * mask).sum(-1) / 512).mean()
+        d = ref - x
+        return ((-obj + 0.01 * (torch.exp(d) - d - 1)) * mask).sum(-1).div(mask.sum(-1).clamp(min=1)).mean()
+
+    calls = {"grpo": lambda x: rl.grpo_loss(x, old, ref, adv, mask), "drgrpo": lambda x: rl.drgrpo_loss(x, old, adv, mask, max_len=512),
+             "dapo": lambda x: rl.dapo_loss(x, old, adv, mask)}
+    for kind, call in calls.items():
+        x, y = logp.clone().requires_grad_(), logp.clone().requires_grad_()
+        a, b = call(x), pytorch(kind, y, 0.28 if kind == "dapo" else 0.2)
+        assert type(a.grad_fn).__name__ == "_LossBackward"
+        torch.testing.assert_close(a, b, rtol=1e-4, atol=1e-6)
+        a.backward()
+        b.backward()
+        torch.testing.assert_close(x.grad, y.grad, rtol=1e-4, atol=1e-8)
+    # gradients of other inputs, and of a gradient, as before
+    o = old.clone().requires_grad_()
+    rl.grpo_loss(logp.clone().requires_grad_(), o, ref, adv, mask).backward()
+    assert o.grad.abs().sum() > 0
+    x = logp.clone().requires_grad_()
+    (d,) = torch.autograd.grad(rl.grpo_loss(x, old, ref, adv, mask), x, create_graph=True)
+    (dd,) = torch.autograd.grad(d.sum(), x)
+    y = logp.clone().requires_grad_()
+    (e,) = torch.autograd.grad(pytorch("grpo", y), y, create_graph=True)
+    torch.testing.assert_close(dd, torch.autograd.grad(e.sum(), y)[0], rtol=1e-4, atol=1e-8)
+    g = rl.GRPOCompute(group_size=4, beta=0.01)
+    loss, stats = g.compute_grpo_loss(logp.clone().requires_grad_(), ref, torch.randn(16, device=DEV), mask, old)
+    assert set(stats) == {"reward_mean", "reward_std", "advantage_abs_mean", "kl"} and type(loss.grad_fn).__name__ == "_LossBackward"
+
+
+# ------------------------------------------------------------------------------------------------ pairs
+def _pair_case(P, T, dtype, mask_type, seed, spoil=True):
+    g = _gen(seed)
+    lp = -torch.rand(2 * P, T, device=DEV, generator=g) * 3
+    ref = (lp + torch.randn(2 * P, T, device=DEV, generator=g) * (2 / math.sqrt(T))).to(dtype)
+    lp = lp.to(dtype)
+    mask = torch.rand(2 * P, T, device=DEV, generator=g) < 0.8
+    if P > 1:
+        mask[1] = False
+        mask[2 * P - 1] = False
+    if spoil:
+        lp[~mask], ref[~mask] = -math.inf, math.nan
+    mask = mask.to(mask_type)
+    return lp, ref, mask * 0.5 if mask.is_floating_point() else mask
+
+
+def _check_pairs(lp, ref, mask, kind="sigmoid", beta=0.1, eps=0.0, gamma=0.0, normalized=False, nll=0.0):
+    from trainscale_b200.rl import preference_loss
+    want = preference_oracle(lp, ref, mask, beta, kind, eps, gamma, normalized, nll)
+    # fp64 throughout: one rounding to fp32, and what a difference of long fp64 sums leaves
+    scale = 1e-13 * float((lp.double().where(mask != 0, 0.0).abs().sum(1).max() + 1) * (1 + beta)) * (1 + float(want[0].abs().sqrt()))
+    x = lp.clone().requires_grad_() if lp.is_contiguous() else lp.detach().requires_grad_()
+    kw = dict(beta=beta, loss_type=kind, label_smoothing=eps, gamma=gamma, length_normalized=normalized, nll_weight=nll)
+    got = preference_loss(x, ref, mask, **kw)
+    for u, v in zip(got, want[:3]):
+        assert u.dtype == torch.float32
+        _near(u.cpu(), v, F32 * 1.01 * v.abs() + scale)
+    (d,) = torch.autograd.grad(got[0], x, retain_graph=True)
+    grad = want[3].to(DEV)
+    tiny = scale + (2.0 ** -25 if lp.dtype == torch.float16 else 1e-30)
+    _near(d, grad, HALF[lp.dtype] * 1.01 * grad.abs() + tiny)
+    (again,) = torch.autograd.grad(got[0], x, torch.tensor(0.7, device=DEV))
+    f = float(torch.tensor(0.7))
+    _near(again, grad * f, (HALF[lp.dtype] * 1.01 + F32 * 2) * grad.abs() * f + tiny)
+    assert all(torch.equal(u.detach(), v) for u, v in zip(got, preference_loss(x.detach(), ref, mask, **kw)))
+
+
+@pytest.mark.parametrize("kind", ["sigmoid", "robust", "hinge", "ipo"])
+@pytest.mark.parametrize("P,T", [(1, 1), (1, 2), (3, 31), (8, 2047), (300, 5), (2, 40001), (70, 1000), (1, 100003)])
+def test_preference_loss(P, T, kind):
+    lp, ref, mask = _pair_case(P, T, torch.float32, torch.bool, P + T)
+    _check_pairs(lp, ref, mask, kind, eps=0.1)
+    _check_pairs(lp, None, mask, kind, 2.0, 0.1, 0.0 if kind == "ipo" else 0.5, True, 0.3)
+
+
+@pytest.mark.parametrize("mask_type", MASKS)
+@pytest.mark.parametrize("dtype", list(HALF))
+def test_preference_loss_types(dtype, mask_type):
+    for P, T in ((5, 77), (40, 3001)):
+        _check_pairs(*_pair_case(P, T, dtype, mask_type, 1), eps=0.1, nll=0.2)
+
+
+def test_preference_loss_of_inputs_that_lie_elsewhere():
+    lp, ref, mask = _pair_case(6, 90, torch.float32, torch.int64, 2)
+    _check_pairs(lp[:, 1:], ref[:, 1:], mask[:, 1:])
+    _check_pairs(lp[::2, 3:80:2], ref[::2, 3:80:2], mask[::2, 3:80:2])
+    lp, ref, _ = _pair_case(6, 90, torch.float32, torch.bool, 2, spoil=False)
+    _check_pairs(lp.t().contiguous().t(), ref[:1].expand(12, 90), mask[:1].expand(12, 90))
+    _check_pairs(lp.half(), ref, mask)
+
+
+def test_far_pairs_do_not_overflow():
+    from trainscale_b200.rl import preference_loss
+    lp = torch.tensor([[-3e4, -3e4], [0.0, 0.0]], device=DEV, requires_grad=True)
+    for kind in ("sigmoid", "robust", "hinge", "ipo"):
+        for order in (lp, lp.flip(0)):
+            loss, _, _ = preference_loss(order, None, torch.ones(2, 2, device=DEV), beta=1.0, loss_type=kind)
+            (d,) = torch.autograd.grad(loss, lp)
+            assert loss.isfinite() and d.isfinite().all()
+
+
+@pytest.mark.parametrize("kind,kw", [("dpo", {}), ("dpo", dict(loss_type="ipo")), ("dpo", dict(loss_type="robust", label_smoothing=0.1)),
+                                     ("dpo", dict(loss_type="hinge")), ("dpo", dict(reference_free=True)), ("simpo", dict(gamma=0.4)),
+                                     ("cpo", dict(alpha=0.5)), ("dpo", dict(loss_type="kto_pair")), ("orpo", {}), ("kto", {})])
+def test_preference_trainer_goes_through_the_kernel(kind, kw, monkeypatch):
+    """The trainer's loss, metrics and weight gradients, with the pair kernel and without it."""
+    from trainscale_b200.data.synthetic import synthetic_preference_dataloader
+    from trainscale_b200.models.llama import build_model
+    from trainscale_b200.ops import policy
+    from trainscale_b200.rl import PreferenceTrainer
+    torch.manual_seed(0)
+    model = build_model("tiny", dtype=torch.bfloat16, device=DEV)
+    ref = PreferenceTrainer.make_reference(model)
+    with torch.no_grad():
+        for p in model.parameters():
+            p.add_(torch.randn_like(p) * 0.01)
+    batch = next(iter(synthetic_preference_dataloader(32000, 20, 40, 4)))
+    batch = {k: v.to(DEV) for k, v in batch.items()}
+
+    def run():
+        t = PreferenceTrainer(model, None, ref, kind, **({} if kind == "orpo" else dict(beta=0.3)), **kw)
+        model.zero_grad()
+        loss, metrics = t.compute_loss(batch)
+        loss.backward()
+        return loss.detach(), metrics, [p.grad.float() for p in model.parameters()]
+
+    seen = []
+    one = policy.preference_loss
+    monkeypatch.setattr(policy, "preference_loss", lambda *a, **k: seen.append(1) or one(*a, **k))
+    a = run()
+    assert bool(seen) == (kind in ("dpo", "simpo", "cpo") and kw.get("loss_type") != "kto_pair")
+    monkeypatch.setattr(PreferenceTrainer, "_pair_kernel", lambda self: None)
+    b = run()
+    torch.testing.assert_close(a[0], b[0], rtol=1e-4, atol=1e-4)
+    assert set(a[1]) == set(b[1])
+    for k in a[1]:
+        torch.testing.assert_close(a[1][k], b[1][k], rtol=1e-3, atol=1e-4)
+    for u, v in zip(a[2], b[2]):
+        assert float((u - v).norm()) <= 2e-2 * float(v.norm()) + 1e-6       # bf16 weight gradients of two fp32 roundings apart
+
+
+# ------------------------------------------------------------------------------------------------ gradient clipping
+def _clip(grads, limit, kind=2.0, **kw):
+    from trainscale_b200.optim import clip_grad_norm_
+    ps = []
+    for g in grads:
+        p = torch.nn.Parameter(torch.empty(0, device=g.device, dtype=g.dtype).expand(0).new_zeros(g.shape))
+        p.grad = g
+        ps.append(p)
+    return clip_grad_norm_(ps, limit, kind, **kw)
+
+
+def _norm64(grads, kind):
+    v = torch.cat([g.double().reshape(-1) for g in grads])
+    return torch.linalg.vector_norm(v, kind)
+
+
+@pytest.mark.parametrize("kind", [2.0, 1.0, math.inf])
+@pytest.mark.parametrize("sizes,types", [([(1,)], 0), ([(3,), (5, 7), (1000, 33), (1 << 20,), (0,), (70000, 3)], 1),
+                                         ([(17,)] * 1500, 1), ([(9, 11)] * 40 + [(2048, 2049)], 2)])
+def test_clip_grad_norm(sizes, types, kind):
+    each = {0: [torch.float32], 1: [torch.float32, torch.bfloat16, torch.float16], 2: [torch.bfloat16]}[types]
+    for factor in (0.3, 2.0):
+        grads = [(torch.randn(s, device=DEV, generator=_gen(i)) * 0.1).to(each[i % len(each)]) for i, s in enumerate(sizes)]
+        before = [g.clone() for g in grads]
+        norm = _norm64(grads, kind)
+        limit = float(norm) * factor
+        got = _clip(grads, limit, kind)
+        _near(got, norm, F32 * 2 * norm)
+        c = min(1.0, limit / (float(norm) + 1e-6))
+        for g, b in zip(grads, before):
+            if factor > 1:
+                assert torch.equal(g, b)
+            else:
+                want = b.double() * c
+                _near(g, want, (HALF[g.dtype] * 1.01 + 6 * F32) * want.abs() + (2.0 ** -25 if g.dtype == torch.float16 else 1e-38))
+
+
+def test_clip_of_views_and_neighbours():
+    """Views of one buffer at odd offsets: what lies between them stays as it is."""
+    for dtype in HALF:
+        flat = torch.randn(5000, device=DEV, generator=_gen(1)).to(dtype)
+        before = flat.clone()
+        grads = [flat[1:18], flat[19:19 + 33 * 7].view(33, 7), flat[300:300], flat[401:4000], flat[4003:4003 + 35 * 7].view(35, 7).t()]
+        norm = _norm64(grads, 2.0)
+        got = _clip(grads, float(norm) / 4)
+        _near(got, norm, F32 * 2 * norm)
+        mine = torch.zeros(5000, dtype=torch.bool, device=DEV)
+        for a, b in ((1, 18), (19, 19 + 33 * 7), (401, 4000), (4003, 4003 + 35 * 7)):
+            mine[a:b] = True
+        assert torch.equal(flat[~mine], before[~mine])
+        want = before.double()[mine] * (float(norm) / 4) / (float(norm) + 1e-6)
+        _near(flat[mine], want, (HALF[dtype] * 1.01 + 6 * F32) * want.abs() + (2.0 ** -25 if dtype == torch.float16 else 0.0))
+
+
+def test_clip_lists_that_go_tensor_by_tensor():
+    """The same gradient twice, gradients that overlap, strided and fp64 ones, another norm: as before."""
+    from trainscale_b200.optim import clip_grad_norm_
+    p = torch.nn.Parameter(torch.zeros(100, device=DEV))
+    p.grad = torch.ones(100, device=DEV)
+    assert float(clip_grad_norm_([p, p], 1.0)) == pytest.approx(math.sqrt(200))
+    assert float(p.grad[0]) == pytest.approx(1 / 200, rel=1e-4)             # scaled twice, one after the other
+    flat = torch.ones(64, device=DEV)
+    assert float(_clip([flat[:40], flat[24:]], 1.0)) == pytest.approx(math.sqrt(80))
+    assert float(flat[30]) == pytest.approx(1 / 80, rel=1e-4) and float(flat[0]) == pytest.approx(1 / math.sqrt(80), rel=1e-4)
+    g = torch.ones(10, 10, device=DEV)
+    assert float(_clip([g[:, ::2]], 1.0)) == pytest.approx(math.sqrt(50)) and float(g[0, 1]) == 1
+    assert float(_clip([torch.ones(4, device=DEV, dtype=torch.float64)], 1.0)) == pytest.approx(2.0)
+    assert float(_clip([torch.ones(8, device=DEV)], 1.0, 3.0)) == pytest.approx(2.0, rel=1e-6)
+    assert _clip([torch.ones(8, device=DEV, dtype=torch.bfloat16)], 1.0, math.inf).dtype == torch.bfloat16
+
+
+def test_clip_of_extreme_gradients():
+    one = lambda v, dtype=torch.float32: [torch.full((3000,), v, device=DEV, dtype=dtype)]          # noqa: E731
+    for v in (1e30, 1e-30, 3e-42, 1e-20, 0.0):              # squares that leave the range of fp32
+        g = one(v)
+        norm = _norm64(g, 2.0)
+        _near(_clip(g, math.inf), norm, F32 * 2 * norm + 2.0 ** -150)
+    g = one(1e30)
+    _clip(g, 1.0)
+    assert float(g[0][0]) == pytest.approx(1 / math.sqrt(3000), rel=1e-5)
+    mixed = one(1e-25) + one(1.0)
+    norm = _norm64(mixed, 2.0)
+    _near(_clip(mixed, math.inf), norm, F32 * 2 * norm)
+    for bad in (math.nan, math.inf, -math.inf):
+        for kind in (2.0, 1.0, math.inf):
+            g = one(1.0)
+            g[0][1234] = bad
+            got = _clip(g, 1.0, kind)
+            assert got.isnan() if math.isnan(bad) else float(got) == math.inf
+            if math.isnan(bad):
+                assert g[0].isnan().all()
+            with pytest.raises(RuntimeError):
+                _clip(one(1.0) + g, 1.0, kind, error_if_nonfinite=True)
+
+
+def test_fused_clip_grad_norm():
+    from trainscale_b200.parallel.dist_utils import fused_clip_grad_norm_
+    m = torch.nn.Sequential(torch.nn.Linear(64, 65), torch.nn.Linear(65, 3)).to(DEV)
+    for kind in (2.0, 1.0, math.inf):
+        for p in m.parameters():
+            p.grad = torch.randn(p.shape, device=DEV, generator=_gen(2))
+        norm = _norm64([p.grad for p in m.parameters()], kind)
+        got = fused_clip_grad_norm_(m, float(norm) / 3, norm_type=kind)
+        _near(got, norm, F32 * 2 * norm)
+        after = _norm64([p.grad for p in m.parameters()], kind)
+        assert float(after) == pytest.approx(float(norm) / 3, rel=1e-5)
+
+
+def test_clip_marks_gradients_as_changed():
+    x = torch.randn(50, device=DEV, requires_grad=True)
+    p = torch.nn.Parameter(torch.zeros(50, device=DEV))
+    g = (x * x).detach()
+    p.grad = g
+    y = x * g                                               # keeps g for its backward pass
+    from trainscale_b200.optim import clip_grad_norm_
+    clip_grad_norm_([p], 1e-3)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+
+
+# ------------------------------------------------------------------------------------------------ together
+def _step(logits, labels, old, ref, adv, mask, weight, native=True):
+    """Logits -> log-probabilities and entropies -> policy loss -> gradient of the head's weight -> clipping."""
+    from trainscale_b200.optim import clip_grad_norm_
+    from trainscale_b200.rl import clipped_policy_loss, token_log_probs
+    head = torch.nn.Parameter(weight.clone())
+    z = (logits @ head)[:, :-1]
+    if native:
+        logp, H = token_log_probs(z, labels, temperature=0.8, return_entropy=True)
+        loss = clipped_policy_loss(logp, old, adv, mask, ref, beta=0.05) - 0.01 * (H * mask).sum() / mask.sum()
+        loss.backward()
+        norm = clip_grad_norm_([head], 0.01)
+    else:
+        lp = torch.log_softmax(z / 0.8, -1)
+        logp, H = lp.gather(-1, labels.unsqueeze(-1)).squeeze(-1), -(lp.exp() * lp).sum(-1)
+        r, d = (logp - old).exp(), ref - logp
+        token = -torch.minimum(r * adv[:, None], r.clamp(0.8, 1.2) * adv[:, None]) + 0.05 * (d.exp() - 1 - d)
+        loss = ((token * mask).sum(1) / mask.sum(1).clamp(min=1)).mean() - 0.01 * (H * mask).sum() / mask.sum()
+        loss.backward()
+        norm = head.grad.norm()
+        head.grad.mul_((0.01 / (norm + 1e-6)).clamp(max=1.0))
+    return loss.detach(), norm, head.grad
+
+
+def _step_inputs(dtype=torch.float32):
+    g = _gen(0)
+    B, T, H, V = 6, 17, 32, 1003
+    x = torch.randn(B, T + 1, H, device=DEV, generator=g)
+    weight = torch.randn(H, V, device=DEV, generator=g) * 0.2
+    labels = torch.randint(0, V, (B, T), device=DEV, generator=g)
+    lp = torch.log_softmax((x @ weight)[:, :-1] / 0.8, -1).gather(-1, labels.unsqueeze(-1)).squeeze(-1)
+    old = lp + 0.1 * torch.randn(B, T, device=DEV, generator=g)
+    ref = lp + 0.3 * torch.randn(B, T, device=DEV, generator=g)
+    mask = (torch.rand(B, T, device=DEV, generator=g) < 0.8).float()
+    mask[2] = 0
+    return [t.to(dtype) if t.is_floating_point() else t for t in (x, labels, old, ref, torch.randn(B, device=DEV, generator=g), mask, weight)]
+
+
+def test_a_policy_step():
+    a = _step_inputs()
+    got = _step(*a)
+    want = _step(*[t.double() if t.is_floating_point() else t for t in a], native=False)
+    torch.testing.assert_close(got[0].double(), want[0], rtol=1e-5, atol=1e-6)
+    torch.testing.assert_close(got[1].double(), want[1], rtol=1e-5, atol=1e-7)
+    torch.testing.assert_close(got[2].double(), want[2], rtol=1e-4, atol=1e-7)
+
+
+def test_a_captured_policy_step_and_another_stream():
+    from trainscale_b200.ops.optim import GradList
+    from trainscale_b200.rl import clipped_policy_loss, preference_loss, token_log_probs
+    x, labels, old, ref, adv, mask, weight = _step_inputs()
+    logits = (x @ weight)[:, :-1].contiguous()
+    pairs = old.clone()
+
+    def step(z, p):
+        z, p = z.detach().requires_grad_(), p.detach().requires_grad_()
+        logp, H = token_log_probs(z, labels, return_entropy=True)
+        loss = clipped_policy_loss(logp, old, adv, mask, ref, beta=0.05, reduction="token") + 0.01 * H.mean()
+        second, chosen, rejected = preference_loss(p, ref, mask)
+        dz, dp = torch.autograd.grad((loss, second), (z, p), (torch.full((), 0.5, device=DEV), torch.ones((), device=DEV)))
+        listed = GradList.of([dz, dp], 2.0)
+        norm = listed.norm(2.0)
+        listed.clip_(norm, 0.05)
+        return loss.detach(), second.detach(), chosen, rejected, dz, dp, norm
+
+    want = [t.clone() for t in step(logits, pairs)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            other = step(logits, pairs)
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(u, v) for u, v in zip(want, other))
+    z, p = torch.zeros_like(logits), torch.zeros_like(pairs)
+    graphs = []
+    for _ in range(2):                                      # two graphs, each with its own workspaces
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = step(z, p)
+        graphs.append((g, out))
+    z.copy_(logits)
+    p.copy_(pairs)
+    for _ in range(3):
+        for g, _ in graphs:
+            g.replay()
+    torch.cuda.synchronize()
+    for _, out in graphs:
+        assert all(torch.equal(u, v) for u, v in zip(want, out))
+
+
+def test_runs_are_the_same_bits():
+    from trainscale_b200.rl import clipped_policy_loss, preference_loss, token_log_probs
+    z = torch.randn(33, 50257, device=DEV, generator=_gen(1)).bfloat16()
+    y = torch.randint(0, 50257, (33,), device=DEV, generator=_gen(2))
+    logp, old, adv, mask, ref = _policy_case(300, 900, torch.float32, torch.bool, 5)
+    lp, rf, m = _pair_case(20, 9001, torch.float32, torch.bool, 6)
+    grads = [torch.randn(100000 + i, device=DEV, generator=_gen(i)) for i in range(20)]
+
+    def run():
+        x, p, q = z.clone().requires_grad_(), logp.clone().requires_grad_(), lp.clone().requires_grad_()
+        a, H = token_log_probs(x, y, return_entropy=True)
+        b, s = clipped_policy_loss(p, old, adv, mask, ref, beta=0.1, return_stats=True)
+        c = preference_loss(q, rf, m)
+        return [a, H, b, *s, *c, *torch.autograd.grad((a.sum(), H.sum(), b, c[0]), (x, p, q)), _clip([g.clone() for g in grads], 1.0)]
+
+    first = run()
+    for _ in range(3):
+        assert all(torch.equal(u, v) for u, v in zip(first, run()))

@@ -93,6 +93,54 @@ def scale_cast_(dst: torch.Tensor, src: torch.Tensor, mul: float = 1.0, accumula
 
 
 # ---------------------------------------------------------------------------------------------------------------
+# The global norm of a list of gradients, and their clipping (library "gradnorm")
+# ---------------------------------------------------------------------------------------------------------------
+_GRAD_TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+_NORMS = {2.0: 0, 1.0: 1, float("inf"): 2}
+
+
+class GradList:
+    """Gradients as the kernels take them.  `GradList.of` gives None where they do not: other types or devices, gradients that are
+    not dense in memory, norms other than 1, 2 and inf."""
+
+    def __init__(self, grads, total):
+        n = len(grads)
+        self.grads, self.total = grads, total
+        self.args = ((ctypes.c_void_p * n)(*[g.data_ptr() for g in grads]), (_ll * n)(*[g.numel() for g in grads]),
+                     (ctypes.c_ubyte * n)(*[_GRAD_TYPES[g.dtype] for g in grads]), n)
+
+    @staticmethod
+    def of(grads: list, norm_type) -> "GradList | None":
+        if not torch.cuda.is_available() or norm_type not in _NORMS:
+            return None
+        here, total = torch._C._cuda_getDevice(), 0
+        for g in grads:
+            if (type(g) is not torch.Tensor or g.dtype not in _GRAD_TYPES or not g.is_cuda or g.get_device() != here
+                    or not (g.is_contiguous() or (g.dim() == 2 and g.t().is_contiguous()))):
+                return None
+            total += g.numel()
+        return GradList(grads, total) if total else None
+
+    def norm(self, norm_type) -> torch.Tensor | None:
+        """Their norm, an fp32 scalar on the device; None where some of them share memory."""
+        lib, dev = _lib.load("gradnorm"), self.grads[0].device
+        lib.ts_grad_norm_workspace.restype = _ll
+        work = torch.empty(lib.ts_grad_norm_workspace(self.args[3], _ll(self.total)), dtype=torch.float64, device=dev)
+        out = torch.empty((), dtype=torch.float32, device=dev)
+        rc = lib.ts_grad_norm(*self.args, _NORMS[norm_type], _lib.ptr(work), _lib.ptr(out), _lib.stream_ptr())
+        if rc == -2:
+            return None
+        _lib.check(rc, "ts_grad_norm")
+        return out
+
+    def clip_(self, norm: torch.Tensor, max_norm: float) -> None:
+        """Every gradient times min(1, max_norm / (norm + 1e-6)); the coefficient stays fp32 and on the device."""
+        rc = _lib.load("gradnorm").ts_grad_scale(*self.args, _lib.ptr(norm), _f(max_norm), _lib.stream_ptr())
+        _lib.check(rc, "ts_grad_scale")
+        torch.autograd.graph.increment_version(self.grads)
+
+
+# ---------------------------------------------------------------------------------------------------------------
 # Per-tensor optimizer kernels (library "optim"): 8-bit AdamW, LAMB, Sophia-G, schedule-free AdamW, ADOPT, AdaFactor.
 # Parameters / gradients may be bf16 or fp32; every data-dependent scalar stays on the device.
 # ---------------------------------------------------------------------------------------------------------------

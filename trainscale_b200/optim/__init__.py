@@ -26,9 +26,23 @@ _IMPL_OPTIONS = {"use_triton": ANY, "fused_foreach": ANY, "enable_metrics": ANY}
 @torch.no_grad()
 def clip_grad_norm_(parameters: Iterable[torch.Tensor], max_norm: float, norm_type: float = 2.0,
                     error_if_nonfinite: bool = False) -> torch.Tensor:
+    """Scale the gradients of `parameters` in place so that their global norm is at most `max_norm`; returns the norm before.
+    Nothing is read back to the host unless `error_if_nonfinite` asks for it.
+
+    bf16, fp16 and fp32 gradients of the current GPU and norms 1, 2 and inf take two launches over the whole list: the
+    sums are fp64, the coefficient min(1, max_norm / (norm + 1e-6)) is fp32 and each product is rounded once.  Other gradients,
+    and lists in which some share memory, go tensor by tensor."""
     grads = [p.grad for p in parameters if p.grad is not None]
     if not grads:
         return torch.zeros(())
+    listed = K.GradList.of(grads, norm_type) if isinstance(max_norm, (int, float)) else None
+    total = listed.norm(norm_type) if listed is not None else None
+    if total is not None:
+        if error_if_nonfinite and not bool(torch.isfinite(total)):
+            raise RuntimeError(f"the total gradient norm is {float(total)}: gradients are not clipped")
+        listed.clip_(total, max_norm)
+        # (the largest value of gradients of one type is returned in it, as it always was)
+        return total if norm_type != float("inf") or any(g.dtype != grads[0].dtype for g in grads) else total.to(grads[0].dtype)
     if norm_type == float("inf"):
         total = torch.stack([g.abs().max() for g in grads]).max()
     else:

@@ -22,6 +22,7 @@ import numpy as np
 import torch
 import torch.distributed as dist
 
+from ..ops.optim import GradList
 from ..utils.refargs import ANY, reference_kwargs
 
 logger = logging.getLogger("trainscale_b200")
@@ -334,6 +335,20 @@ def fused_clip_grad_norm_(parameters, max_norm: float, group=None, norm_type: fl
     if not grads:
         return torch.zeros(())
     sharded = group is not None and dist.is_initialized() and dist.get_world_size(group) > 1
+    listed = GradList.of(grads, norm_type) if isinstance(max_norm, (int, float)) else None
+    norm = listed.norm(norm_type) if listed is not None else None
+    if norm is not None:
+        if sharded:
+            if norm_type == float("inf"):
+                dist.all_reduce(norm, op=dist.ReduceOp.MAX, group=group)
+            else:
+                norm = norm.pow(norm_type)
+                dist.all_reduce(norm, group=group)
+                norm = norm.pow(1.0 / norm_type)
+        if error_if_nonfinite and not bool(torch.isfinite(norm)):
+            raise RuntimeError(f"the total gradient norm is {float(norm)}")
+        listed.clip_(norm, max_norm)
+        return norm
     if norm_type == float("inf"):
         norm = torch.stack([g.float().abs().max() for g in grads]).max()
         if sharded:

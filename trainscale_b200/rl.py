@@ -6,10 +6,15 @@ Utilities after data_pipeline/trainer/rl_training.py:95-671 (`selective_log_soft
 (data_pipeline/trainer/loss/sota_losses.py:1151, preprocessing/prompt_engine.py:1929); `PreferenceTrainer` is that
 loop: policy (and a frozen reference copy) under the flat engine, chosen and rejected sequences concatenated into
 one forward, per-token log-probs from the fused lm_head + log-prob kernel (logits never materialised).
+
+`token_log_probs`, `clipped_policy_loss` and `preference_loss` are the kernels under them (csrc/logprob.cu, csrc/posttrain.cu):
+logits to log-probabilities and entropies, log-probabilities to a policy loss, and to the loss of (chosen, rejected) pairs.  On the
+CPU, and for what the kernels do not take, they are PyTorch operations with the same meaning.
 """
 from __future__ import annotations
 
 import copy
+import math
 from typing import Any, Dict
 
 import torch
@@ -18,14 +23,39 @@ import torch.nn.functional as F
 
 from .losses import CPOLoss, DPOLoss, KTOLoss, ORPOLoss, SimPOLoss
 from .ops import cross_entropy as ce_ops
+from .ops import logprob as lp_ops
+from .ops import policy as policy_ops
+from .ops.policy import PolicyStats
 from .utils.refargs import ANY, reference_kwargs
+
+
+def token_log_probs(logits: torch.Tensor, labels: torch.Tensor, *, temperature: float = 1.0, logit_softcapping: float = 0.0,
+                    logit_scale: float = 0.0, ignore_index: int | None = -100, return_entropy: bool = False):
+    """log p(labels) under `logits` [..., V] in fp32, shape of `labels` [...]; differentiable in the logits.
+
+    Transforms of the logits, in this order: soft-cap c tanh(z / c), scale, divide by the temperature (0 switches the first two off).
+    Rows whose label is `ignore_index` give 0 and no gradient, and are not read; a label outside the vocabulary gives NaN.
+    `return_entropy`: (log-probabilities, entropy of each row's distribution), both differentiable; logits of -inf are tokens of no
+    probability.  bf16, fp16 and fp32 logits with rows that are dense within themselves (also of a slice such as `logits[:, :-1]`) are
+    read in place, once in each direction."""
+    for name, value, least in (("temperature", temperature, None), ("logit_softcapping", logit_softcapping, 0), ("logit_scale", logit_scale, 0)):
+        if not math.isfinite(value) or (value <= 0 if least is None else value < least):
+            raise ValueError(f"{name} is {value}: it must be finite and {'positive' if least is None else 'not negative'}")
+    return lp_ops.token_log_probs(logits, labels, (logit_scale or 1.0) / temperature, float(logit_softcapping), ignore_index,
+                                  return_entropy)
 
 
 @reference_kwargs(input_ids="index")
 def selective_log_softmax(logits: torch.Tensor, index: torch.Tensor, temperature: float = 1.0,
                           logit_softcapping: float = 0.0, logit_scale: float = 0.0) -> torch.Tensor:
     """log_softmax(logits)[..., index] without keeping the full log-softmax.  Optional transforms of the logits, in
-    this order: soft-cap c tanh(z / c), scale, divide by the temperature."""
+    this order: soft-cap c tanh(z / c), scale, divide by the temperature.  The transforms happen in the type of the logits;
+    `token_log_probs` makes them in fp32 whatever that is, and is what computes this on the GPU where the two agree."""
+    plain = not (logit_softcapping or logit_scale) and temperature == 1.0
+    if ((plain or logits.dtype == torch.float32) and index.dtype == torch.int64 and index.shape == logits.shape[:-1] and temperature > 0
+            and logit_softcapping >= 0 and logit_scale >= 0 and lp_ops.native(logits, index)):
+        return token_log_probs(logits, index, temperature=temperature, logit_softcapping=logit_softcapping, logit_scale=logit_scale,
+                               ignore_index=None)
     if logit_softcapping:
         logits = logit_softcapping * torch.tanh(logits / logit_softcapping)
     if logit_scale:
@@ -119,6 +149,83 @@ def _reference_rl_loss(kind: str, policy_log_probs, ref_log_probs, third, mask, 
     return loss, metrics
 
 
+def clipped_policy_loss(logp: torch.Tensor, old_logp: torch.Tensor, advantages: torch.Tensor, mask: torch.Tensor,
+                        ref_logp: torch.Tensor | None = None, *, clip: float = 0.2, clip_high: float | None = None, beta: float = 0.0,
+                        reduction: str = "sequence", max_len: int | None = None, return_stats: bool = False):
+    """Clipped policy loss with a KL term over token log-probabilities [B, T]:
+
+        r = e^(logp - old_logp);  token = -min(r A, clamp(r, 1 - clip, 1 + clip_high) A) + beta (e^d - 1 - d),  d = ref_logp - logp
+
+    `advantages`: [B], or [B, T].  `mask` [B, T]: tokens count with its value; where it is zero nothing is read into the loss, not even
+    inf or NaN.  `reduction`: "sequence" (mean over the rows of the mean over their tokens), "token" (mean over all tokens) or
+    "constant" (sum over B * max_len; max_len is T by default); a mask that leaves nothing counts as one token.
+    `old_logp`, `advantages` and `ref_logp` are constants.  `return_stats`: (loss, `PolicyStats`), on the device.
+    On the GPU the loss and the gradient of fp32, bf16 or fp16 log-probabilities come out of one pass, summed in fp64."""
+    if logp.dim() != 2:
+        raise ValueError(f"log-probabilities are [sequences, tokens], not {tuple(logp.shape)}")
+    if reduction not in policy_ops.REDUCTIONS:
+        raise ValueError(f"unknown reduction {reduction!r}; one of {sorted(policy_ops.REDUCTIONS)}")
+    for name, t in (("old_logp", old_logp), ("mask", mask), ("ref_logp", ref_logp)):
+        if t is not None and t.shape != logp.shape:
+            raise ValueError(f"{name} of shape {tuple(t.shape)} for log-probabilities of shape {tuple(logp.shape)}")
+    if advantages.shape not in (logp.shape, logp.shape[:1]):
+        raise ValueError(f"advantages of shape {tuple(advantages.shape)} for log-probabilities of shape {tuple(logp.shape)}")
+    high = clip if clip_high is None else clip_high
+    if not (math.isfinite(clip) and math.isfinite(high) and clip >= 0 and high >= 0):
+        raise ValueError(f"clip ranges are finite and not negative, not {clip} and {high}")
+    if not math.isfinite(beta):
+        raise ValueError(f"beta is {beta}")
+    if beta and ref_logp is None:
+        raise ValueError("a KL term needs ref_logp")
+    if max_len is not None and max_len <= 0:
+        raise ValueError(f"max_len is {max_len}")
+    loss, stats = policy_ops.policy_loss(logp, old_logp, advantages, mask, ref_logp, float(clip), float(high), float(beta), reduction,
+                                         max_len)
+    return (loss, PolicyStats(*stats.unbind())) if return_stats else loss
+
+
+def _takes_policy_kernel(logp, old_logp, ref_logp, advantages, mask) -> bool:
+    """Whether `clipped_policy_loss` stands for the PyTorch form of a group-relative loss: fp32 on the GPU, a gradient for the
+    policy's log-probabilities alone."""
+    others = [t for t in (old_logp, ref_logp, advantages, mask) if t is not None]
+    return (all(torch.is_tensor(t) for t in (logp, *others)) and policy_ops.native(logp, *others)
+            and all(t.dtype == torch.float32 for t in (logp, old_logp, advantages) if t is not None)
+            and (ref_logp is None or ref_logp.dtype == torch.float32) and advantages.shape == logp.shape[:1]
+            and old_logp.shape == mask.shape == logp.shape and (ref_logp is None or ref_logp.shape == logp.shape)
+            and not (torch.is_grad_enabled() and any(t.requires_grad for t in others)))
+
+
+def preference_loss(policy_logps: torch.Tensor, ref_logps: torch.Tensor | None, mask: torch.Tensor, *, beta: float = 0.1,
+                    loss_type: str = "sigmoid", label_smoothing: float = 0.0, gamma: float = 0.0, length_normalized: bool = False,
+                    nll_weight: float = 0.0):
+    """Loss of preference pairs straight from token log-probabilities [2 P, T], the chosen sequences first: returns
+    (loss, rewards of the chosen [P], rewards of the rejected [P]).
+
+    A sequence's score is the sum of mask * (policy - reference), divided by its tokens with `length_normalized`; the rewards are beta
+    times the scores, and the loss is the mean over the pairs of a function of x, the difference of the two scores:
+    "sigmoid" -log sigma(beta x - gamma) with `label_smoothing`, "robust" (its unbiased form under flipped labels), "hinge"
+    max(0, 1 - beta x + gamma) or "ipo" (x - 1 / (2 beta))^2.  `nll_weight` adds the chosen sequences' mean negative log-likelihood.
+    Without `ref_logps` the loss is reference-free; reference log-probabilities are constants.  Tokens of mask zero are not read into
+    the loss, not even inf or NaN.  Scores and what follows from them are fp64."""
+    if policy_logps.dim() != 2 or policy_logps.shape[0] % 2:
+        raise ValueError(f"log-probabilities are [2 * pairs, tokens], not {tuple(policy_logps.shape)}")
+    for name, t in (("ref_logps", ref_logps), ("mask", mask)):
+        if t is not None and t.shape != policy_logps.shape:
+            raise ValueError(f"{name} of shape {tuple(t.shape)} for log-probabilities of shape {tuple(policy_logps.shape)}")
+    if loss_type not in policy_ops.KINDS:
+        raise ValueError(f"unknown preference loss {loss_type!r}; one of {sorted(policy_ops.KINDS)}")
+    if not (math.isfinite(beta) and beta > 0 and math.isfinite(gamma) and math.isfinite(nll_weight)):
+        raise ValueError(f"beta is finite and positive, gamma and nll_weight are finite, not {beta}, {gamma} and {nll_weight}")
+    if not 0 <= label_smoothing <= 1 or (loss_type == "robust" and label_smoothing >= 0.5):
+        raise ValueError(f"label_smoothing is {label_smoothing}: it lies in [0, 1], below 0.5 for the robust loss")
+    if gamma and loss_type == "ipo":
+        raise ValueError("ipo has no margin gamma")
+    P = policy_logps.shape[0] // 2
+    loss, rewards = policy_ops.preference_loss(policy_logps, ref_logps, mask, float(beta), loss_type, float(label_smoothing), float(gamma),
+                                               bool(length_normalized), float(nll_weight))
+    return loss, rewards[:P], rewards[P:]
+
+
 def grpo_loss(logp: torch.Tensor = None, old_logp: torch.Tensor = None, ref_logp: torch.Tensor | None = None,
               advantages: torch.Tensor = None, mask: torch.Tensor = None, clip: float = 0.2, beta: float = 0.01, *,
               policy_log_probs=None, ref_log_probs=None):
@@ -127,6 +234,8 @@ def grpo_loss(logp: torch.Tensor = None, old_logp: torch.Tensor = None, ref_logp
     the reference's sequence-level loss instead and returns (loss, metrics): see `_reference_rl_loss`."""
     if policy_log_probs is not None:
         return _reference_rl_loss("grpo", policy_log_probs, ref_log_probs, advantages, mask, beta)
+    if _takes_policy_kernel(logp, old_logp, ref_logp, advantages, mask) and 0 <= clip and 0 <= beta:
+        return clipped_policy_loss(logp, old_logp, advantages, mask, ref_logp if beta else None, clip=clip, beta=beta if ref_logp is not None else 0.0)
     ratio = torch.exp(logp - old_logp)
     a = advantages.unsqueeze(-1)
     obj = torch.minimum(ratio * a, ratio.clamp(1 - clip, 1 + clip) * a)
@@ -144,6 +253,8 @@ def drgrpo_loss(logp=None, old_logp=None, advantages=None, mask=None, clip: floa
     returning (loss, metrics)."""
     if policy_log_probs is not None:
         return _reference_rl_loss("drgrpo", policy_log_probs, ref_log_probs, advantages, mask, beta, epsilon)
+    if _takes_policy_kernel(logp, old_logp, None, advantages, mask) and 0 <= clip and (max_len is None or max_len > 0):
+        return clipped_policy_loss(logp, old_logp, advantages, mask, clip=clip, reduction="constant", max_len=max_len)
     ratio = torch.exp(logp - old_logp)
     a = advantages.unsqueeze(-1)
     obj = torch.minimum(ratio * a, ratio.clamp(1 - clip, 1 + clip) * a)
@@ -158,6 +269,8 @@ def dapo_loss(logp=None, old_logp=None, advantages=None, mask=None, clip_low: fl
     returning (loss, metrics)."""
     if policy_log_probs is not None:
         return _reference_rl_loss("dapo", policy_log_probs, ref_log_probs, rewards, mask, beta, temperature=temperature)
+    if _takes_policy_kernel(logp, old_logp, None, advantages, mask) and 0 <= clip_low and 0 <= clip_high:
+        return clipped_policy_loss(logp, old_logp, advantages, mask, clip=clip_low, clip_high=clip_high, reduction="token")
     ratio = torch.exp(logp - old_logp)
     a = advantages.unsqueeze(-1)
     obj = torch.minimum(ratio * a, ratio.clamp(1 - clip_low, 1 + clip_high) * a)
@@ -297,7 +410,8 @@ class PreferenceTrainer:
             p.requires_grad_(False)
         return ref.eval()
 
-    def _seq_logps(self, model, ids, mask, labels, grad: bool):
+    def _token_logps(self, model, ids, mask, labels, grad: bool):
+        """Log-probabilities of the next tokens, and where there is one."""
         ctx = torch.enable_grad() if grad else torch.no_grad()
         with ctx:
             h = model.model(ids)
@@ -305,17 +419,45 @@ class PreferenceTrainer:
             lab = labels.masked_fill(mask == 0, -100)
             tgt = torch.full_like(lab, -100)
             tgt[:, :-1] = lab[:, 1:]
-            lp = ce_ops.fused_linear_token_logprobs(h, w if grad else w.detach(), tgt)
-            return lp.sum(-1), (tgt != -100).sum(-1)
+            return ce_ops.fused_linear_token_logprobs(h, w if grad else w.detach(), tgt), tgt != -100
+
+    def _seq_logps(self, model, ids, mask, labels, grad: bool):
+        lp, valid = self._token_logps(model, ids, mask, labels, grad)
+        return lp.sum(-1), valid.sum(-1)
+
+    def _pair_kernel(self) -> dict | None:
+        """The loss as arguments of `preference_loss`; None for those that are not a function of one pair's scores."""
+        f, kind = self.loss_fn, self.kind
+        if kind == "dpo" and f.loss_type in policy_ops.KINDS and (f.loss_type != "robust" or f.label_smoothing < 0.5):
+            kw = dict(loss_type=f.loss_type, label_smoothing=f.label_smoothing if f.loss_type in ("sigmoid", "robust") else 0.0)
+        elif kind == "simpo":
+            kw = dict(label_smoothing=f.eps, gamma=f.gamma, length_normalized=True)
+        elif kind == "cpo":
+            kw = dict(label_smoothing=f.eps, nll_weight=f.alpha)
+        else:
+            return None
+        return dict(kw, beta=f.beta) if f.beta > 0 and 0 <= kw["label_smoothing"] <= 1 else None
 
     def compute_loss(self, batch: Dict[str, torch.Tensor]):
         B = batch["chosen_input_ids"].shape[0]
         ids = torch.cat((batch["chosen_input_ids"], batch["rejected_input_ids"]))
         mask = torch.cat((batch["chosen_attention_mask"], batch["rejected_attention_mask"]))
         labels = torch.cat((batch["chosen_labels"], batch["rejected_labels"]))
-        lp, n = self._seq_logps(self.policy, ids, mask, labels, True)
-        pc, pr, nc, nr = lp[:B], lp[B:], n[:B], n[B:]
+        tokens, valid = self._token_logps(self.policy, ids, mask, labels, True)
         metrics = {}
+        kernel = self._pair_kernel()
+        if kernel is not None and policy_ops.native(tokens, valid):
+            ref = None
+            if self.kind == "dpo" and self.ref is not None and not self.loss_fn.reference_free:
+                ref, _ = self._token_logps(self.ref, ids, mask, labels, False)
+            loss, cr, rjr = preference_loss(tokens, ref, valid, **kernel)
+            if self.kind != "cpo":
+                metrics["reward_accuracy"] = (cr > rjr).float().mean()
+            if self.kind == "dpo":
+                metrics["reward_margin"] = (cr - rjr).mean()
+            return loss, metrics
+        lp, n = tokens.sum(-1), valid.sum(-1)
+        pc, pr, nc, nr = lp[:B], lp[B:], n[:B], n[B:]
         if self.kind == "dpo":
             rc = rr = None
             if self.ref is not None and not self.loss_fn.reference_free:
