@@ -8,7 +8,10 @@ Clip coefficient min(1, max_norm / (norm + 1e-6)) as in data_pipeline/trainer/di
 """
 from __future__ import annotations
 
+import array
 import ctypes
+import functools
+import operator
 
 import torch
 
@@ -96,38 +99,51 @@ def scale_cast_(dst: torch.Tensor, src: torch.Tensor, mul: float = 1.0, accumula
 # The global norm of a list of gradients, and their clipping (library "gradnorm")
 # ---------------------------------------------------------------------------------------------------------------
 _GRAD_TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+_DTYPE = operator.attrgetter("dtype")
 _NORMS = {2.0: 0, 1.0: 1, float("inf"): 2}
+
+
+@functools.lru_cache(maxsize=None)
+def _gradnorm():
+    lib, p = _lib.load("gradnorm"), ctypes.c_void_p
+    lib.ts_grad_norm_workspace.argtypes, lib.ts_grad_norm_workspace.restype = [ctypes.c_int, _ll], _ll
+    lib.ts_grad_norm.argtypes = [p, p, ctypes.c_char_p, ctypes.c_int, ctypes.c_int, p, p, p]
+    lib.ts_grad_scale.argtypes = [p, p, ctypes.c_char_p, ctypes.c_int, p, _f, p]
+    return lib
 
 
 class GradList:
     """Gradients as the kernels take them.  `GradList.of` gives None where they do not: other types or devices, gradients that are
     not dense in memory, norms other than 1, 2 and inf."""
 
-    def __init__(self, grads, total):
-        n = len(grads)
-        self.grads, self.total = grads, total
-        self.args = ((ctypes.c_void_p * n)(*[g.data_ptr() for g in grads]), (_ll * n)(*[g.numel() for g in grads]),
-                     (ctypes.c_ubyte * n)(*[_GRAD_TYPES[g.dtype] for g in grads]), n)
+    def __init__(self, grads: list, codes: bytes):
+        self.grads, self.codes = grads, codes
+        self.data = array.array("Q", map(torch.Tensor.data_ptr, grads))
+        self.size = array.array("q", map(torch.Tensor.numel, grads))
+        self.args = (self.data.buffer_info()[0], self.size.buffer_info()[0], codes, len(grads))
 
     @staticmethod
     def of(grads: list, norm_type) -> "GradList | None":
-        if not torch.cuda.is_available() or norm_type not in _NORMS:
+        # (each check is one C-level pass over the list: a loop in Python costs more than the kernels of a short list)
+        if norm_type not in _NORMS or set(map(type, grads)) != {torch.Tensor}:
             return None
-        here, total = torch._C._cuda_getDevice(), 0
-        for g in grads:
-            if (type(g) is not torch.Tensor or g.dtype not in _GRAD_TYPES or not g.is_cuda or g.get_device() != here
-                    or not (g.is_contiguous() or (g.dim() == 2 and g.t().is_contiguous()))):
+        if not grads[0].is_cuda or set(map(torch.Tensor.get_device, grads)) != {torch._C._cuda_getDevice()}:
+            return None
+        codes = list(map(_GRAD_TYPES.get, map(_DTYPE, grads)))
+        if None in codes or any(g.layout != torch.strided for g in grads):
+            return None
+        if not all(map(torch.Tensor.is_contiguous, grads)):
+            if not all(g.is_contiguous() or (g.dim() == 2 and g.t().is_contiguous()) for g in grads):
                 return None
-            total += g.numel()
-        return GradList(grads, total) if total else None
+        listed = GradList(grads, bytes(codes))
+        return listed if any(listed.size) else None
 
     def norm(self, norm_type) -> torch.Tensor | None:
         """Their norm, an fp32 scalar on the device; None where some of them share memory."""
-        lib, dev = _lib.load("gradnorm"), self.grads[0].device
-        lib.ts_grad_norm_workspace.restype = _ll
-        work = torch.empty(lib.ts_grad_norm_workspace(self.args[3], _ll(self.total)), dtype=torch.float64, device=dev)
+        lib, dev, n = _gradnorm(), self.grads[0].device, len(self.grads)
+        work = torch.empty(lib.ts_grad_norm_workspace(n, sum(self.size)), dtype=torch.float64, device=dev)
         out = torch.empty((), dtype=torch.float32, device=dev)
-        rc = lib.ts_grad_norm(*self.args, _NORMS[norm_type], _lib.ptr(work), _lib.ptr(out), _lib.stream_ptr())
+        rc = lib.ts_grad_norm(*self.args, _NORMS[norm_type], work.data_ptr(), out.data_ptr(), _lib.stream_ptr())
         if rc == -2:
             return None
         _lib.check(rc, "ts_grad_norm")
@@ -135,8 +151,7 @@ class GradList:
 
     def clip_(self, norm: torch.Tensor, max_norm: float) -> None:
         """Every gradient times min(1, max_norm / (norm + 1e-6)); the coefficient stays fp32 and on the device."""
-        rc = _lib.load("gradnorm").ts_grad_scale(*self.args, _lib.ptr(norm), _f(max_norm), _lib.stream_ptr())
-        _lib.check(rc, "ts_grad_scale")
+        _lib.check(_gradnorm().ts_grad_scale(*self.args, norm.data_ptr(), max_norm, _lib.stream_ptr()), "ts_grad_scale")
         torch.autograd.graph.increment_version(self.grads)
 
 

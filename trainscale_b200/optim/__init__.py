@@ -32,7 +32,7 @@ def clip_grad_norm_(parameters: Iterable[torch.Tensor], max_norm: float, norm_ty
     bf16, fp16 and fp32 gradients of the current GPU and norms 1, 2 and inf take two launches over the whole list: the
     sums are fp64, the coefficient min(1, max_norm / (norm + 1e-6)) is fp32 and each product is rounded once.  Other gradients,
     and lists in which some share memory, go tensor by tensor."""
-    grads = [p.grad for p in parameters if p.grad is not None]
+    grads = [g for p in parameters if (g := p.grad) is not None]
     if not grads:
         return torch.zeros(())
     listed = K.GradList.of(grads, norm_type) if isinstance(max_norm, (int, float)) else None
