@@ -5,8 +5,9 @@
 //   r = e^(logp - old),  clipped = a > 0 ? r > 1 + high : a < 0 and r < 1 - low,  d = ref - logp
 //   token = -a (clipped ? bound : r) + beta (e^d - 1 - d),  d token / d logp = (clipped ? 0 : -a r) - beta (e^d - 1)
 //   loss  = sum m w token,  w = 1 / (rows sum_row m), 1 / sum m or 1 / (rows length); the sums of m are at least 1
-// Which side of a bound a token is on is decided in 64 bits (the difference of two fp32 numbers is exact there): its gradient
-// jumps at the bound.  e^d - 1 - d is a power series near zero, where the difference would cancel.  Sums are fp64.
+// A token's gradient jumps at a bound, so the side that it is on is decided by logp - old without rounding (two fp32 numbers whose
+// sum is the difference).  e^d - 1 - d is a power series near zero, where the difference would cancel.  Sums of four or eight
+// tokens are fp32, sums of those fp64, in an order that depends on the sizes alone.
 //
 // Pairs, rows p (chosen) and P + p (rejected), of scores s = sum m (logp - ref), divided by max(sum m, 1) where asked:
 //   x = s_p - s_(P + p),  q = beta x - gamma
@@ -16,17 +17,27 @@
 //
 // Gradients leave with the loss, for an upstream gradient of one.  Where it turns out to be another, fp32 gradients are multiplied
 // by it; 16-bit ones, which that would round twice, are computed again (`Upstream`).
+#include <cooperative_groups.h>
+
 #include "common.cuh"
 #include "host_common.h"
 
 namespace ts {
 
-constexpr int PT_THREADS = 256;
-constexpr int PT_TILE = 2048;            // tokens of a block
+namespace cg = cooperative_groups;
 
+constexpr int PT_THREADS = 256;
+
+template <typename T, int N>
+struct alignas(sizeof(T) * N) Few {
+  T v[N];
+};
 __device__ __forceinline__ float pt_f32(float v) { return v; }
 __device__ __forceinline__ float pt_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
 __device__ __forceinline__ float pt_f32(__half v) { return __half2float(v); }
+__device__ __forceinline__ float pt_f32(unsigned char v) { return static_cast<float>(v); }
+__device__ __forceinline__ float pt_f32(int v) { return static_cast<float>(v); }
+__device__ __forceinline__ float pt_f32(long long v) { return static_cast<float>(v); }
 template <typename T>
 __device__ __forceinline__ T pt_from(float v);
 template <>
@@ -36,6 +47,44 @@ __device__ __forceinline__ __nv_bfloat16 pt_from<__nv_bfloat16>(float v) { retur
 template <>
 __device__ __forceinline__ __half pt_from<__half>(float v) { return __float2half(v); }
 
+// N consecutive values, aligned to N of them where N > 1.
+template <int N, typename T>
+__device__ __forceinline__ void fetch(const T* p, float* f) {
+  using V = Few<T, N>;
+  if constexpr (sizeof(V) <= 16) {
+    const V v = *reinterpret_cast<const V*>(p);
+#pragma unroll
+    for (int i = 0; i < N; ++i) f[i] = pt_f32(v.v[i]);
+  } else {
+    fetch<N / 2>(p, f);
+    fetch<N / 2>(p + N / 2, f + N / 2);
+  }
+}
+template <int N, typename T>
+__device__ __forceinline__ void put(T* p, const float* f) {
+  Few<T, N> v;
+#pragma unroll
+  for (int i = 0; i < N; ++i) v.v[i] = pt_from<T>(f[i]);
+  *reinterpret_cast<Few<T, N>*>(p) = v;
+}
+
+struct Mask {
+  const void* p;
+  long long stride;                      // elements between rows
+  int kind;                              // 0 bool / uint8, 1 int32, 2 int64, 3 fp32, 4 bf16, 5 fp16
+  template <int N>
+  __device__ __forceinline__ void get(long long i, float* f) const {
+    switch (kind) {
+      case 0: return fetch<N>(static_cast<const unsigned char*>(p) + i, f);
+      case 1: return fetch<N>(static_cast<const int*>(p) + i, f);
+      case 2: return fetch<N>(static_cast<const long long*>(p) + i, f);
+      case 3: return fetch<N>(static_cast<const float*>(p) + i, f);
+      case 4: return fetch<N>(static_cast<const __nv_bfloat16*>(p) + i, f);
+      default: return fetch<N>(static_cast<const __half*>(p) + i, f);
+    }
+  }
+};
+
 // What flows into the loss: nothing known yet (null), or a factor of the gradient; `redo`: also where it is one.
 struct Upstream {
   const float* factor;
@@ -44,139 +93,300 @@ struct Upstream {
   __device__ __forceinline__ float get() const { return factor ? *factor : 1.f; }
 };
 
-struct Mask {
-  const void* p;
-  long long stride;                      // elements between rows
-  int kind;                              // 0 bool / uint8, 1 int32, 2 int64, 3 fp32, 4 bf16, 5 fp16
-  __device__ __forceinline__ float at(long long row, long long t) const {
-    const long long i = row * stride + t;
-    switch (kind) {
-      case 0: return static_cast<float>(static_cast<const unsigned char*>(p)[i]);
-      case 1: return static_cast<float>(static_cast<const int*>(p)[i]);
-      case 2: return static_cast<float>(static_cast<const long long*>(p)[i]);
-      case 3: return static_cast<const float*>(p)[i];
-      case 4: return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
-      default: return __half2float(static_cast<const __half*>(p)[i]);
-    }
-  }
-};
-
-// Sum over the block in a fixed order; every thread gets it.
-__device__ __forceinline__ double block_sum64(double v, double* scratch) {
+// Sums over the block in a fixed order; every thread gets them.
+template <int N>
+__device__ __forceinline__ void block_sums(double* v, double (*scratch)[N]) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nwarp = blockDim.x >> 5;
 #pragma unroll
-  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  __syncthreads();
-  if (lane == 0) scratch[warp] = v;
-  __syncthreads();
-  v = lane < nwarp ? scratch[lane] : 0.0;
+  for (int k = 0; k < N; ++k)
 #pragma unroll
-  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
+    for (int o = 16; o; o >>= 1) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
+  __syncthreads();
+  if (lane == 0)
+#pragma unroll
+    for (int k = 0; k < N; ++k) scratch[warp][k] = v[k];
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    v[k] = lane < nwarp ? scratch[lane][k] : 0.0;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
+  }
 }
 
 // ---------------------------------------------------------------------------------------------------
-// Clipped policy loss
+// Clipped policy loss.  Tokens are numbered row after row; a block takes a run of them, a thread VEC at a time.
 // ---------------------------------------------------------------------------------------------------
+constexpr int POLICY_PER_SM = 4;         // blocks of an SM
 constexpr int POLICY_SUMS = 5;           // loss, kl m, clipped m, ratio m, m
+constexpr int POLICY_SPLIT = 8;          // most blocks that count a row
+constexpr int POLICY_ALONE = 8192;       // tokens that one block takes by itself, in one launch
+constexpr int POLICY_ALONE_THREADS = 1024, POLICY_ALONE_ROWS = 4096;
 
 struct Policy {
   const void *logp, *old, *ref;
   long long s_logp, s_old, s_ref;        // elements between rows
   const float* advantages;               // [rows] or [rows][T]
-  int per_token;
   Mask mask;
-  long long rows, T;
-  double log_low, log_high;              // ln(1 - low), ln(1 + high)
+  long long rows, T, tokens, run;        // tokens = rows T; run: tokens of a block
+  double constant;                       // 1 / (rows length) of reduction 2
+  float bound_low[2], bound_high[2];     // ln(1 - low) and ln(1 + high), each as a sum of two
   float low, high, beta;                 // 1 - low, 1 + high
-  int reduction;                         // 0 rows' means, 1 all tokens, 2 a constant
-  double constant;                       // 1 / (rows * length) of reduction 2
+  int per_token, reduction;              // 0 rows' means, 1 all tokens, 2 a constant
+  int flat;                              // rows follow one another without gaps in every tensor
 };
 
-__global__ void __launch_bounds__(PT_THREADS) policy_count_kernel(Mask mask, long long T, double* __restrict__ counts, Upstream up) {
-  __shared__ double scratch[32];
-  if (up.done()) return;
-  double n = 0.0;
-  for (long long t = threadIdx.x; t < T; t += PT_THREADS) n += mask.at(blockIdx.x, t);
-  n = block_sum64(n, scratch);
-  if (threadIdx.x == 0) counts[blockIdx.x] = n;
-}
-
-// e^d - 1 - d, where e = e^d - 1
-__device__ __forceinline__ float exp_rest(float d, float e) {
+// e^d - 1 - d and e^d - 1
+__device__ __forceinline__ float exp_rest(float d, float* less) {
   const float series = 0.5f + d * (1.f / 6.f + d * (1.f / 24.f + d * (1.f / 120.f + d * (1.f / 720.f + d * (1.f / 5040.f +
                        d * (1.f / 40320.f + d * (1.f / 362880.f)))))));
-  return fabsf(d) < 0.5f ? d * d * series : e - d;
+  const bool near = fabsf(d) < 0.5f;
+  const float rest = d * d * series, e = expf(d) - 1.f;
+  *less = near ? d + rest : e;
+  return near ? rest : e - d;
 }
 
-template <typename T>
-__global__ void __launch_bounds__(PT_THREADS) policy_kernel(Policy a, const double* __restrict__ counts, T* __restrict__ grad,
-                                                            double* __restrict__ partial, Upstream up) {
-  __shared__ double scratch[32];
+// Where a thread's next tokens are: stepping by a block's width costs no division.
+struct Place {
+  int row, t, T, rows, rest;
+  __device__ __forceinline__ Place(long long token, int width, long long length)
+      : row(static_cast<int>(token / length)), t(static_cast<int>(token - row * length)), T(static_cast<int>(length)),
+        rows(width / static_cast<int>(length)), rest(width - rows * static_cast<int>(length)) {}
+  __device__ __forceinline__ void step() {
+    row += rows;
+    t += rest;
+    if (t >= T) t -= T, ++row;
+  }
+  __device__ __forceinline__ long long in(long long stride) const { return row * stride + t; }
+};
+
+// Sum of the mask over tokens [begin, end), which lie in one row or are `flat`.
+template <int VEC>
+__device__ __forceinline__ double mask_run(const Policy& a, long long begin, long long end) {
+  const long long at = a.flat ? 0 : begin / a.T * (a.mask.stride - a.T), width = static_cast<long long>(blockDim.x) * VEC;
+  double n = 0.0;
+  for (long long i = begin + static_cast<long long>(threadIdx.x) * VEC; i < end; i += 4 * width) {
+    float m[4][VEC], s = 0.f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) m[j][e] = 0.f;
+      if (i + j * width < end) a.mask.get<VEC>(at + i + j * width, m[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) s += m[j][e];
+    n += s;
+  }
+  return n;
+}
+
+// The same of any tokens.
+template <int VEC>
+__device__ __forceinline__ double mask_sum(const Policy& a, long long begin, long long end) {
+  if (a.flat) return mask_run<VEC>(a, begin, end);
+  const int width = static_cast<int>(blockDim.x) * VEC;
+  long long i = begin + static_cast<long long>(threadIdx.x) * VEC;
+  double n = 0.0;
+  for (Place at(i, width, a.T); i < end; i += width, at.step()) {
+    float m[VEC], s = 0.f;
+    a.mask.get<VEC>(at.in(a.mask.stride), m);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) s += m[e];
+    n += s;
+  }
+  return n;
+}
+
+// Gradient and sums of tokens [begin, end).  Weights: of the row (`weights`), or the same for all.
+template <typename T, int VEC, bool FLAT>
+__device__ __forceinline__ void policy_tokens(const Policy& a, long long begin, long long end, const float* weights, float uniform,
+                                              float factor, T* __restrict__ grad, double* sums) {
+  const int width = static_cast<int>(blockDim.x) * VEC;
+  const bool whole = a.T % VEC == 0;     // a thread's tokens are in one row
+  long long next = begin + static_cast<long long>(threadIdx.x) * VEC;
+  Place ahead(next, width, a.T);
+  float coming[VEC];                     // the mask is read a step ahead: tokens that it leaves out are not read at all
+  if (next < end) a.mask.get<VEC>(FLAT ? next : ahead.in(a.mask.stride), coming);
+  while (next < end) {
+    const long long i = next;
+    const Place at = ahead;
+    float logp[VEC], old[VEC], ref[VEC], m[VEC], adv[VEC], w[VEC], slope[VEC], part[POLICY_SUMS] = {};
+    bool any = false;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) m[e] = coming[e], any |= m[e] != 0.f, slope[e] = 0.f;
+    next += width;
+    ahead.step();
+    if (next < end) a.mask.get<VEC>(FLAT ? next : ahead.in(a.mask.stride), coming);
+    if (!any) {
+      if (grad) put<VEC>(grad + i, slope);
+      continue;
+    }
+    fetch<VEC>(static_cast<const T*>(a.logp) + (FLAT ? i : at.in(a.s_logp)), logp);
+    fetch<VEC>(static_cast<const T*>(a.old) + (FLAT ? i : at.in(a.s_old)), old);
+    if (a.ref) fetch<VEC>(static_cast<const T*>(a.ref) + (FLAT ? i : at.in(a.s_ref)), ref);
+    if (whole) {
+      const float row_w = weights ? weights[at.row] : uniform, row_adv = a.per_token ? 0.f : a.advantages[at.row];
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) w[e] = row_w, adv[e] = row_adv;
+    } else {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        const int row = at.row + (at.t + e) / at.T;
+        w[e] = weights ? weights[row] : uniform;
+        adv[e] = a.per_token ? 0.f : a.advantages[row];
+      }
+    }
+    if (a.per_token) fetch<VEC>(a.advantages + i, adv);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      // whatever a masked token holds reaches nothing
+      const bool used = m[e] != 0.f;
+      const float g = used ? adv[e] : 0.f, x = used ? logp[e] : 0.f, y = used ? old[e] : 0.f;
+      const float moved = x - y;
+      bool above = moved > a.bound_high[0], below = moved < a.bound_low[0];
+      if (moved == a.bound_high[0] || moved == a.bound_low[0]) {
+        // x - y = moved + lost exactly
+        const float back = moved - x, lost = (x - (moved - back)) - (y + back);
+        above = moved == a.bound_high[0] && lost > a.bound_high[1];
+        below = moved == a.bound_low[0] && lost < a.bound_low[1];
+      }
+      const bool clipped = g > 0.f ? above : g < 0.f && below;
+      const float ratio = expf(moved);
+      // (0 * inf: a ratio that overflows has no say where the advantage is zero)
+      const float gain = g == 0.f && ratio == INFINITY ? 0.f : g * (clipped ? (g > 0.f ? a.high : a.low) : ratio);
+      float token = -gain;
+      slope[e] = clipped ? 0.f : -gain;
+      if (a.ref) {
+        float less;
+        const float kl = exp_rest(used ? ref[e] - x : 0.f, &less);
+        token += a.beta * kl;
+        slope[e] -= a.beta * less;
+        part[1] += m[e] * kl;
+      }
+      const float mw = m[e] * w[e];
+      part[0] += mw * token;
+      part[2] += clipped ? m[e] : 0.f;
+      part[3] += m[e] * ratio;
+      part[4] += m[e];
+      slope[e] *= mw * factor;
+    }
+#pragma unroll
+    for (int k = 0; k < POLICY_SUMS; ++k) sums[k] += part[k];
+    if (grad) put<VEC>(grad + i, slope);
+  }
+}
+
+__device__ __forceinline__ void policy_results(const double* sums, float* loss, float* stats) {
+  *loss = static_cast<float>(sums[0]);
+  if (stats)
+    for (int k = 1; k < 4; ++k) stats[k - 1] = static_cast<float>(sums[k] / fmax(sums[4], 1.0));
+}
+
+// What the tokens weigh: weights [rows] (reduction 0, a block or a cluster per row), sums of the mask by block (reduction 1); and the
+// counter that tells the next kernel's last block.
+template <int VEC>
+__global__ void __launch_bounds__(PT_THREADS) policy_count_kernel(Policy a, float* __restrict__ weights, double* __restrict__ counts,
+                                                                  unsigned* __restrict__ ticket, Upstream up) {
+  __shared__ double scratch[32][1];
+  __shared__ double by_block[POLICY_SPLIT];
+  cg::cluster_group cluster = cg::this_cluster();
   if (up.done()) return;
-  const float factor = up.get();
-  const long long n = a.rows * a.T;
-  double all = 0.0;
+  if (blockIdx.x == 0 && threadIdx.x == 0) *ticket = 0;
+  if (a.reduction == 2) return;
+  const int parts = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
   if (a.reduction == 1) {
-    for (long long r = threadIdx.x; r < a.rows; r += PT_THREADS) all += counts[r];
-    all = block_sum64(all, scratch);
+    double n[1] = {mask_sum<VEC>(a, blockIdx.x * a.run, min(a.tokens, (blockIdx.x + 1ll) * a.run))};
+    block_sums<1>(n, scratch);
+    if (threadIdx.x == 0) counts[blockIdx.x] = n[0];
+    return;
+  }
+  const long long row = blockIdx.x / parts, part = (a.T / VEC + parts - 1) / parts * VEC;
+  const long long begin = row * a.T + rank * part, end = rank == parts - 1 ? (row + 1) * a.T : min((row + 1) * a.T, begin + part);
+  // (a row that starts between vectors is counted token by token)
+  double n[1] = {(row * a.T | a.T) % VEC == 0 ? mask_run<VEC>(a, begin, end) : mask_run<1>(a, begin, end)};
+  block_sums<1>(n, scratch);
+  if (parts > 1) {
+    if (threadIdx.x == 0) *cluster.map_shared_rank(by_block + rank, 0) = n[0];
+    cluster.sync();
+    if (rank != 0) return;
+    n[0] = 0.0;
+    for (int i = 0; i < parts; ++i) n[0] += by_block[i];
+  }
+  if (threadIdx.x == 0) weights[row] = static_cast<float>(1.0 / (fmax(n[0], 1.0) * static_cast<double>(a.rows)));
+}
+
+template <typename T, int VEC, bool FLAT>
+__global__ void __launch_bounds__(PT_THREADS, POLICY_PER_SM) policy_kernel(Policy a, const float* __restrict__ weights, const double* __restrict__ counts,
+                                                            double* __restrict__ partial, unsigned* __restrict__ ticket,
+                                                            T* __restrict__ grad, float* __restrict__ loss, float* __restrict__ stats,
+                                                            Upstream up) {
+  __shared__ double scratch[32][POLICY_SUMS];
+  __shared__ bool last;
+  if (up.done()) return;
+  float uniform = static_cast<float>(a.constant);
+  if (a.reduction == 1) {
+    double n[POLICY_SUMS] = {};
+    for (unsigned i = threadIdx.x; i < gridDim.x; i += PT_THREADS) n[0] += counts[i];
+    block_sums<POLICY_SUMS>(n, scratch);
+    uniform = static_cast<float>(1.0 / fmax(n[0], 1.0));
   }
   double sums[POLICY_SUMS] = {};
-  const long long end = min(n, (blockIdx.x + 1ll) * PT_TILE);
-  for (long long i = blockIdx.x * static_cast<long long>(PT_TILE) + threadIdx.x; i < end; i += PT_THREADS) {
-    const long long row = i / a.T, t = i - row * a.T;
-    const float m = a.mask.at(row, t);
-    float slope = 0.f;
-    if (m != 0.f) {
-      const double w = a.reduction == 0 ? 1.0 / (fmax(counts[row], 1.0) * static_cast<double>(a.rows))
-                       : a.reduction == 1 ? 1.0 / fmax(all, 1.0) : a.constant;
-      const float logp = pt_f32(static_cast<const T*>(a.logp)[row * a.s_logp + t]);
-      const float old = pt_f32(static_cast<const T*>(a.old)[row * a.s_old + t]);
-      const float adv = a.advantages[a.per_token ? i : row];
-      const double moved = static_cast<double>(logp) - static_cast<double>(old);
-      const float ratio = expf(static_cast<float>(moved));
-      const bool clipped = (adv > 0.f && moved > a.log_high) || (adv < 0.f && moved < a.log_low);
-      // (0 * inf: a ratio that overflows has no say where the advantage is zero)
-      const float gain = adv == 0.f && ratio == INFINITY ? 0.f : adv * (clipped ? (adv > 0.f ? a.high : a.low) : ratio);
-      float token = -gain, kl = 0.f;
-      slope = clipped ? 0.f : -gain;
-      if (a.ref) {
-        const float d = static_cast<float>(static_cast<double>(pt_f32(static_cast<const T*>(a.ref)[row * a.s_ref + t])) - logp);
-        const float e = expm1f(d);
-        kl = exp_rest(d, e);
-        token += a.beta * kl;
-        slope -= a.beta * e;
-      }
-      sums[0] += m * w * token;
-      sums[1] += static_cast<double>(m) * kl;
-      sums[2] += clipped ? m : 0.f;
-      sums[3] += static_cast<double>(m) * ratio;
-      sums[4] += m;
-      slope = static_cast<float>(slope * m * w * factor);
-    }
-    if (grad) grad[i] = pt_from<T>(slope);
+  const long long begin = blockIdx.x * a.run;
+  policy_tokens<T, VEC, FLAT>(a, begin, min(a.tokens, begin + a.run), a.reduction == 0 ? weights : nullptr, uniform, up.get(), grad, sums);
+  if (!loss) return;
+  block_sums<POLICY_SUMS>(sums, scratch);
+  if (threadIdx.x == 0) {
+#pragma unroll
+    for (int k = 0; k < POLICY_SUMS; ++k) __stcg(partial + k * static_cast<long long>(gridDim.x) + blockIdx.x, sums[k]);
+    __threadfence();
+    last = atomicAdd(ticket, 1) == gridDim.x - 1;
   }
+  __syncthreads();
+  if (!last) return;
+  __threadfence();
 #pragma unroll
   for (int k = 0; k < POLICY_SUMS; ++k) {
-    const double v = block_sum64(sums[k], scratch);
-    if (threadIdx.x == 0) partial[blockIdx.x * static_cast<long long>(POLICY_SUMS) + k] = v;
+    sums[k] = 0.0;
+    for (unsigned i = threadIdx.x; i < gridDim.x; i += PT_THREADS) sums[k] += __ldcg(partial + k * static_cast<long long>(gridDim.x) + i);
   }
+  block_sums<POLICY_SUMS>(sums, scratch);
+  if (threadIdx.x == 0) policy_results(sums, loss, stats);
 }
 
-// stats: mean kl, share of clipped tokens, mean ratio
-__global__ void __launch_bounds__(1024) policy_finish_kernel(const double* __restrict__ partial, int blocks, float* __restrict__ loss,
-                                                             float* __restrict__ stats) {
-  __shared__ double scratch[32];
-  double v[POLICY_SUMS];
-  for (int k = 0; k < POLICY_SUMS; ++k) {
-    v[k] = 0.0;
-    for (int i = threadIdx.x; i < blocks; i += blockDim.x) v[k] += partial[i * static_cast<long long>(POLICY_SUMS) + k];
-    v[k] = block_sum64(v[k], scratch);
+// All of it in one block.
+template <typename T, int VEC, bool FLAT>
+__global__ void __launch_bounds__(POLICY_ALONE_THREADS) policy_alone_kernel(Policy a, T* __restrict__ grad, float* __restrict__ loss,
+                                                                            float* __restrict__ stats, Upstream up) {
+  __shared__ double scratch[32][POLICY_SUMS];
+  __shared__ float weights[POLICY_ALONE_ROWS];
+  if (up.done()) return;
+  float uniform = static_cast<float>(a.constant);
+  if (a.reduction == 0) {
+    const int lane = threadIdx.x & 31;
+    for (int r = threadIdx.x >> 5; r < a.rows; r += POLICY_ALONE_THREADS / 32) {
+      double n = 0.0;
+      for (long long t = lane; t < a.T; t += 32) {
+        float m;
+        a.mask.get<1>(r * a.mask.stride + t, &m);
+        n += m;
+      }
+#pragma unroll
+      for (int o = 16; o; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
+      if (lane == 0) weights[r] = static_cast<float>(1.0 / (fmax(n, 1.0) * static_cast<double>(a.rows)));
+    }
+    __syncthreads();
+  } else if (a.reduction == 1) {
+    double n[POLICY_SUMS] = {mask_sum<VEC>(a, 0, a.tokens)};
+    block_sums<POLICY_SUMS>(n, scratch);
+    uniform = static_cast<float>(1.0 / fmax(n[0], 1.0));
   }
-  if (threadIdx.x == 0) {
-    *loss = static_cast<float>(v[0]);
-    for (int k = 1; k < 4; ++k) stats[k - 1] = static_cast<float>(v[k] / fmax(v[4], 1.0));
-  }
+  double sums[POLICY_SUMS] = {};
+  policy_tokens<T, VEC, FLAT>(a, 0, a.tokens, a.reduction == 0 ? weights : nullptr, uniform, up.get(), grad, sums);
+  if (!loss) return;
+  block_sums<POLICY_SUMS>(sums, scratch);
+  if (threadIdx.x == 0) policy_results(sums, loss, stats);
 }
 
 // grad *= *factor; a factor of one leaves it as it is
@@ -190,6 +400,9 @@ __global__ void __launch_bounds__(PT_THREADS) scale_kernel(float* __restrict__ g
 // ---------------------------------------------------------------------------------------------------
 // Pairs
 // ---------------------------------------------------------------------------------------------------
+constexpr int PAIR_SPLIT = 8;            // most blocks of a pair
+constexpr int PAIR_TOKENS = 2048;        // tokens of a row that are worth a block
+
 struct Pairs {
   const void *logp, *ref;
   long long s_logp, s_ref;
@@ -220,69 +433,118 @@ __device__ __forceinline__ double pair_loss(const Pairs& a, double x, double* sl
   return d * d;
 }
 
-// One block per pair: scores, loss, rewards, and the gradient of both rows.
-template <typename T>
+// Calls f(t, N) over [begin, end) of a row whose token 0 is `phase` tokens behind a vector's boundary: single tokens up to the first
+// boundary and behind the last, VEC at a time between them.
+template <int VEC, typename F>
+__device__ __forceinline__ void over_row(long long begin, long long end, int phase, F&& f) {
+  if (VEC == 1) {
+    for (long long t = begin + threadIdx.x; t < end; t += PT_THREADS) f(t, std::integral_constant<int, 1>());
+    return;
+  }
+  const long long first = min(end, begin + (VEC - (begin + phase) % VEC) % VEC), past = first + (end - first) / VEC * VEC;
+  for (long long t = first + static_cast<long long>(threadIdx.x) * VEC; t < past; t += PT_THREADS * VEC) f(t, std::integral_constant<int, VEC>());
+  const long long lone = threadIdx.x < first - begin ? begin + threadIdx.x : past + (threadIdx.x - (first - begin));
+  if (lone < end && threadIdx.x < (first - begin) + (end - past)) f(lone, std::integral_constant<int, 1>());
+}
+
+// A block, or a cluster of them, per pair: scores, loss, rewards, and the gradient of both rows.
+template <typename T, int VEC>
 __global__ void __launch_bounds__(PT_THREADS) pair_kernel(Pairs a, T* __restrict__ grad, double* __restrict__ loss,
                                                           float* __restrict__ rewards, Upstream up) {
-  __shared__ double scratch[32];
+  __shared__ double scratch[32][5];
+  __shared__ double by_block[PAIR_SPLIT][5];
+  cg::cluster_group cluster = cg::this_cluster();
   if (up.done()) return;
-  const long long p = blockIdx.x;
-  double score[2], count[2], own = 0.0;
+  const int parts = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
+  const long long p = blockIdx.x / parts;
+  const long long begin = a.T * rank / parts, end = a.T * (rank + 1) / parts;
+  double sums[5] = {};                   // score and tokens of the chosen, of the rejected row; the chosen's own log-probability
+#pragma unroll
   for (int side = 0; side < 2; ++side) {
     const long long row = p + side * a.pairs;
-    double s = 0.0, c = 0.0, l = 0.0;
-    for (long long t = threadIdx.x; t < a.T; t += PT_THREADS) {
-      const float m = a.mask.at(row, t);
-      if (m == 0.f) continue;
-      const double v = pt_f32(static_cast<const T*>(a.logp)[row * a.s_logp + t]);
-      const double r = a.ref ? pt_f32(static_cast<const T*>(a.ref)[row * a.s_ref + t]) : 0.f;
-      s += m * (v - r);
-      l += m * v;
-      c += m;
-    }
-    score[side] = block_sum64(s, scratch);
-    count[side] = fmax(block_sum64(c, scratch), 1.0);
-    if (side == 0) own = block_sum64(l, scratch) / count[0];
-    if (a.normalized) score[side] /= count[side];
+    over_row<VEC>(begin, end, static_cast<int>(row * a.T % VEC), [&](long long t, auto n) {
+      constexpr int N = decltype(n)::value;
+      float m[N], v[N], r[N];
+      a.mask.get<N>(row * a.mask.stride + t, m);
+      fetch<N>(static_cast<const T*>(a.logp) + row * a.s_logp + t, v);
+      if (a.ref) fetch<N>(static_cast<const T*>(a.ref) + row * a.s_ref + t, r);
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        if (m[e] == 0.f) continue;       // whatever a masked token holds reaches nothing
+        const double w = m[e], x = v[e];
+        sums[2 * side] += w * (a.ref ? x - r[e] : x);
+        sums[2 * side + 1] += w;
+        if (side == 0) sums[4] += w * x;
+      }
+    });
   }
+  block_sums<5>(sums, scratch);
+  if (parts > 1) {
+    if (static_cast<int>(threadIdx.x) < parts) {
+      double* to = cluster.map_shared_rank(&by_block[rank][0], threadIdx.x);
+#pragma unroll
+      for (int k = 0; k < 5; ++k) to[k] = sums[k];
+    }
+    cluster.sync();
+#pragma unroll
+    for (int k = 0; k < 5; ++k) {
+      sums[k] = 0.0;
+      for (int i = 0; i < parts; ++i) sums[k] += by_block[i][k];
+    }
+  }
+  const double count[2] = {fmax(sums[1], 1.0), fmax(sums[3], 1.0)};
+  const double score[2] = {a.normalized ? sums[0] / count[0] : sums[0], a.normalized ? sums[2] / count[1] : sums[2]};
   double slope;
-  const double value = pair_loss(a, score[0] - score[1], &slope) - (a.nll != 0.0 ? a.nll * own : 0.0);
-  if (threadIdx.x == 0 && rewards) {
+  const double value = pair_loss(a, score[0] - score[1], &slope) - (a.nll != 0.0 ? a.nll * sums[4] / count[0] : 0.0);
+  if (threadIdx.x == 0 && rank == 0 && rewards) {
     loss[p] = value;
     rewards[p] = static_cast<float>(a.beta * score[0]);
     rewards[p + a.pairs] = static_cast<float>(a.beta * score[1]);
   }
   if (!grad) return;
+#pragma unroll
   for (int side = 0; side < 2; ++side) {
     const long long row = p + side * a.pairs;
     double w = (side ? -slope : slope) / (a.normalized ? count[side] : 1.0);
     if (side == 0) w -= a.nll / count[0];
-    w *= up.get() / static_cast<double>(a.pairs);
-    for (long long t = threadIdx.x; t < a.T; t += PT_THREADS) {
-      const float m = a.mask.at(row, t);
-      grad[row * a.T + t] = pt_from<T>(m == 0.f ? 0.f : static_cast<float>(w * m));
-    }
+    const float weight = static_cast<float>(w * up.get() / static_cast<double>(a.pairs));
+    over_row<VEC>(begin, end, static_cast<int>(row * a.T % VEC), [&](long long t, auto n) {
+      constexpr int N = decltype(n)::value;
+      float m[N];
+      a.mask.get<N>(row * a.mask.stride + t, m);
+#pragma unroll
+      for (int e = 0; e < N; ++e) m[e] = m[e] == 0.f ? 0.f : weight * m[e];
+      put<N>(grad + row * a.T + t, m);
+    });
   }
 }
 
 __global__ void __launch_bounds__(1024) pair_finish_kernel(const double* __restrict__ loss, long long pairs, float* __restrict__ out) {
-  __shared__ double scratch[32];
-  double v = 0.0;
-  for (long long i = threadIdx.x; i < pairs; i += blockDim.x) v += loss[i];
-  v = block_sum64(v, scratch);
-  if (threadIdx.x == 0) *out = static_cast<float>(v / static_cast<double>(pairs));
+  __shared__ double scratch[32][1];
+  double v[1] = {0.0};
+  for (long long i = threadIdx.x; i < pairs; i += blockDim.x) v[0] += loss[i];
+  block_sums<1>(v, scratch);
+  if (threadIdx.x == 0) *out = static_cast<float>(v[0] / static_cast<double>(pairs));
 }
 
+// ---------------------------------------------------------------------------------------------------
 template <typename F>
 static int pt_by_type(int dtype, F&& launch) {
   switch (dtype) {
-    case 0: launch(static_cast<__nv_bfloat16*>(nullptr)); break;
-    case 1: launch(static_cast<__half*>(nullptr)); break;
-    case 2: launch(static_cast<float*>(nullptr)); break;
+    case 0: return launch(static_cast<__nv_bfloat16*>(nullptr));
+    case 1: return launch(static_cast<__half*>(nullptr));
+    case 2: return launch(static_cast<float*>(nullptr));
     default: return -1;
   }
-  return static_cast<int>(cudaGetLastError());
 }
+
+static bool on_boundary(const void* p, int bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
+static int mask_bytes(int kind) {
+  static const int bytes[6] = {1, 4, 8, 4, 2, 2};
+  return bytes[kind];
+}
+static int type_bytes(int dtype) { return dtype == 2 ? 4 : 2; }
+static double high_part(double v) { return static_cast<double>(static_cast<float>(v)); }
 
 }  // namespace ts
 
@@ -290,54 +552,144 @@ using namespace ts;
 
 TS_DEFINE_ERROR_API(ts_posttrain)
 
-// Number of doubles that ts_policy_loss needs as workspace.
+// The arguments of a call, eight bytes each (ops/policy.py packs them).  dtype (of logp, old, ref and grad): 0 bf16, 1 fp16, 2 fp32.
+// ref, grad and stats may be null; loss too where only the gradient is wanted, times *factor (and where that is one, with `redo`
+// alone).  stats: mean kl, share of clipped tokens, mean ratio.
+struct PolicyCall {
+  long long dtype;
+  const void* logp;
+  long long s_logp;
+  const void* old;
+  long long s_old;
+  const void* ref;
+  long long s_ref;
+  const float* advantages;
+  long long per_token;
+  const void* mask;
+  long long s_mask, mask_kind, rows, T;
+  double log_low, log_high, low, high, beta;
+  long long reduction;
+  double constant;
+  void* grad;
+  float *loss, *stats;
+  const float* factor;
+  long long redo;
+  double* workspace;
+};
+
+static bool policy_alone(long long rows, long long T) { return rows <= POLICY_ALONE_ROWS && rows * T <= POLICY_ALONE; }
+
+// Number of doubles that ts_policy_loss needs as workspace: weights, counts, sums, a counter.  None where one block does it.
 extern "C" long long ts_policy_workspace(long long rows, long long T) {
-  return rows + POLICY_SUMS * ((rows * T + PT_TILE - 1) / PT_TILE);
+  return policy_alone(rows, T) ? 0 : rows + (POLICY_SUMS + 1) * static_cast<long long>(sm_count()) * POLICY_PER_SM + 1;
 }
 
-// dtype (of logp, old, ref and grad): 0 bf16, 1 fp16, 2 fp32.  ref and grad may be null.  loss: one float;
-// stats: three; both null where only the gradient is wanted, times *factor (and where that is one, with `redo` alone).
-extern "C" int ts_policy_loss(int dtype, const void* logp, long long s_logp, const void* old, long long s_old, const void* ref,
-                              long long s_ref, const float* advantages, int per_token, const void* mask, long long s_mask,
-                              int mask_kind, long long rows, long long T, double log_low, double log_high, double low, double high,
-                              double beta, int reduction, double constant, void* grad, float* loss, float* stats, const float* factor,
-                              int redo, double* workspace, void* stream) {
-  const long long blocks = (rows * T + PT_TILE - 1) / PT_TILE;
-  if (rows <= 0 || T <= 0 || rows > 0x7fffffffll || blocks > 0x7fffffffll || reduction < 0 || reduction > 2) return -1;
+extern "C" int ts_policy_loss(const PolicyCall* c, void* stream) {
+  const long long n = c->rows * c->T;
+  if (c->rows <= 0 || c->T <= 0 || c->rows > 0x7fffffffll / POLICY_SPLIT || c->T > 0x7fffffffll || c->reduction < 0 || c->reduction > 2 ||
+      c->mask_kind < 0 || c->mask_kind > 5 || c->dtype < 0 || c->dtype > 2)
+    return -1;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const Mask m{mask, s_mask, mask_kind};
-  const Policy a{logp, old, ref, s_logp, s_old, s_ref, advantages, per_token, m, rows, T, log_low, log_high,
-                 static_cast<float>(low), static_cast<float>(high), static_cast<float>(beta), reduction, constant};
-  const Upstream up{factor, redo};
-  double *counts = workspace, *partial = workspace + rows;
-  if (reduction != 2) policy_count_kernel<<<static_cast<unsigned>(rows), PT_THREADS, 0, st>>>(m, T, counts, up);
-  return pt_by_type(dtype, [&](auto* t) {
+  Policy a;
+  a.logp = c->logp, a.old = c->old, a.ref = c->ref;
+  a.s_logp = c->s_logp, a.s_old = c->s_old, a.s_ref = c->s_ref;
+  a.advantages = c->advantages, a.per_token = static_cast<int>(c->per_token);
+  a.mask = {c->mask, c->s_mask, static_cast<int>(c->mask_kind)};
+  a.rows = c->rows, a.T = c->T, a.tokens = n;
+  a.constant = c->constant, a.reduction = static_cast<int>(c->reduction);
+  a.bound_low[0] = static_cast<float>(c->log_low), a.bound_low[1] = c->log_low < -1e30 ? 0.f : static_cast<float>(c->log_low - high_part(c->log_low));
+  a.bound_high[0] = static_cast<float>(c->log_high), a.bound_high[1] = static_cast<float>(c->log_high - high_part(c->log_high));
+  a.low = static_cast<float>(c->low), a.high = static_cast<float>(c->high), a.beta = static_cast<float>(c->beta);
+  // four tokens at a time where they lie together and on a boundary in every tensor: rows without gaps, or rows of whole fours
+  const int e = type_bytes(static_cast<int>(c->dtype)), m = mask_bytes(a.mask.kind);
+  a.flat = a.s_logp == a.T && a.s_old == a.T && (!a.ref || a.s_ref == a.T) && a.mask.stride == a.T;
+  const bool fours = (a.flat || ((a.T | a.s_logp | a.s_old | (a.ref ? a.s_ref : 0) | a.mask.stride) & 3) == 0) && on_boundary(a.logp, 4 * e) &&
+                     on_boundary(a.old, 4 * e) && on_boundary(a.ref, 4 * e) && on_boundary(a.mask.p, m == 8 ? 16 : 4 * m) &&
+                     on_boundary(c->grad, 4 * e) && (!a.per_token || on_boundary(a.advantages, 16)) && n % 4 == 0;
+  const int vec = fours ? 4 : 1;
+  const Upstream up{c->factor, static_cast<int>(c->redo)};
+  const long long tile = static_cast<long long>(PT_THREADS) * vec, most = static_cast<long long>(sm_count()) * POLICY_PER_SM;
+  const long long tiles = (n + tile - 1) / tile, blocks = tiles < most ? tiles : most;
+  a.run = (tiles + blocks - 1) / blocks * tile;
+  const unsigned used = static_cast<unsigned>((n + a.run - 1) / a.run);
+  float* weights = reinterpret_cast<float*>(c->workspace);
+  double *counts = c->workspace + a.rows, *partial = counts + most;
+  unsigned* ticket = reinterpret_cast<unsigned*>(partial + POLICY_SUMS * most);
+  return pt_by_type(static_cast<int>(c->dtype), [&](auto* t) {
     using E = std::remove_pointer_t<decltype(t)>;
-    policy_kernel<E><<<static_cast<unsigned>(blocks), PT_THREADS, 0, st>>>(a, counts, static_cast<E*>(grad), partial, up);
-    if (loss) policy_finish_kernel<<<1, 1024, 0, st>>>(partial, static_cast<int>(blocks), loss, stats);
+    auto run = [&](auto v, auto f) {
+      constexpr int VEC = decltype(v)::value;
+      constexpr bool FLAT = decltype(f)::value;
+      if (policy_alone(a.rows, a.T)) {
+        policy_alone_kernel<E, VEC, FLAT><<<1, POLICY_ALONE_THREADS, 0, st>>>(a, static_cast<E*>(c->grad), c->loss, c->stats, up);
+        return static_cast<int>(cudaGetLastError());
+      }
+      // a row is split while blocks are fewer than two to an SM and a part is worth one
+      int parts = 1;
+      if (a.reduction == 0)
+        while (parts < POLICY_SPLIT && a.rows * parts < 2 * sm_count() && a.T / parts >= 8 * PT_THREADS * VEC) parts *= 2;
+      const unsigned counters = a.reduction == 0 ? static_cast<unsigned>(a.rows * parts) : a.reduction == 1 ? used : 1;
+      const int rc = launch_chained(policy_count_kernel<VEC>, dim3(counters), dim3(PT_THREADS), 0, st, parts, false, a, weights, counts, ticket, up);
+      if (rc) return rc;
+      policy_kernel<E, VEC, FLAT><<<used, PT_THREADS, 0, st>>>(a, weights, counts, partial, ticket, static_cast<E*>(c->grad), c->loss, c->stats, up);
+      return static_cast<int>(cudaGetLastError());
+    };
+    using four = std::integral_constant<int, 4>;
+    using one = std::integral_constant<int, 1>;
+    return fours ? (a.flat ? run(four(), std::true_type()) : run(four(), std::false_type()))
+                 : (a.flat ? run(one(), std::true_type()) : run(one(), std::false_type()));
   });
 }
 
 // grad [n] *= *factor.
 extern "C" int ts_scale_by(float* grad, const float* factor, long long n, void* stream) {
   if (n <= 0) return -1;
-  const long long blocks = (n + PT_THREADS * 4 - 1) / (PT_THREADS * 4);
-  scale_kernel<<<static_cast<unsigned>(blocks < 2368 ? blocks : 2368), PT_THREADS, 0, static_cast<cudaStream_t>(stream)>>>(grad, factor, n);
+  const long long blocks = (n + PT_THREADS * 4 - 1) / (PT_THREADS * 4), most = sm_count() * 8ll;
+  scale_kernel<<<static_cast<unsigned>(blocks < most ? blocks : most), PT_THREADS, 0, static_cast<cudaStream_t>(stream)>>>(grad, factor, n);
   return static_cast<int>(cudaGetLastError());
 }
 
 // Rows 0 .. pairs - 1 are the chosen, the next the rejected sequences.  loss: one float; rewards: 2 * pairs floats; workspace:
 // `pairs` doubles.  ref and grad may be null; loss, rewards, factor and redo as above.
-extern "C" int ts_preference_loss(int dtype, const void* logp, long long s_logp, const void* ref, long long s_ref, const void* mask,
-                                  long long s_mask, int mask_kind, long long pairs, long long T, double beta, double gamma,
-                                  double smoothing, double nll, int kind, int normalized, void* grad, float* loss, float* rewards,
-                                  const float* factor, int redo, double* workspace, void* stream) {
-  if (pairs <= 0 || T <= 0 || pairs > 0x3fffffffll || kind < 0 || kind > 3) return -1;
+struct PairsCall {
+  long long dtype;
+  const void* logp;
+  long long s_logp;
+  const void* ref;
+  long long s_ref;
+  const void* mask;
+  long long s_mask, mask_kind, pairs, T;
+  double beta, gamma, smoothing, nll;
+  long long kind, normalized;
+  void* grad;
+  float *loss, *rewards;
+  const float* factor;
+  long long redo;
+  double* workspace;
+};
+
+extern "C" int ts_preference_loss(const PairsCall* c, void* stream) {
+  if (c->pairs <= 0 || c->T <= 0 || c->pairs > 0x7fffffffll / PAIR_SPLIT || c->kind < 0 || c->kind > 3 || c->mask_kind < 0 ||
+      c->mask_kind > 5 || c->dtype < 0 || c->dtype > 2)
+    return -1;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const Pairs a{logp, ref, s_logp, s_ref, {mask, s_mask, mask_kind}, pairs, T, beta, gamma, smoothing, nll, kind, normalized};
-  return pt_by_type(dtype, [&](auto* t) {
+  const Pairs a{c->logp, c->ref, c->s_logp, c->s_ref, {c->mask, c->s_mask, static_cast<int>(c->mask_kind)}, c->pairs, c->T,
+                c->beta, c->gamma, c->smoothing, c->nll, static_cast<int>(c->kind), static_cast<int>(c->normalized)};
+  // four tokens at a time where all tensors start on a boundary and their rows are as far behind one (the gradient's rows are T long)
+  const int e = type_bytes(static_cast<int>(c->dtype)), m = mask_bytes(a.mask.kind);
+  const bool fours = ((a.s_logp ^ a.T) & 3) == 0 && (!a.ref || ((a.s_ref ^ a.T) & 3) == 0) && ((a.mask.stride ^ a.T) & 3) == 0 &&
+                     on_boundary(a.logp, 4 * e) && on_boundary(a.ref, 4 * e) && on_boundary(a.mask.p, m == 8 ? 16 : 4 * m) &&
+                     on_boundary(c->grad, 4 * e);
+  // a pair is split while blocks are fewer than four to an SM and its parts are worth one
+  int parts = 1;
+  while (parts < PAIR_SPLIT && a.pairs * parts < 4 * sm_count() && a.T / parts >= 2 * PAIR_TOKENS) parts *= 2;
+  return pt_by_type(static_cast<int>(c->dtype), [&](auto* t) {
     using E = std::remove_pointer_t<decltype(t)>;
-    pair_kernel<E><<<static_cast<unsigned>(pairs), PT_THREADS, 0, st>>>(a, static_cast<E*>(grad), workspace, rewards, {factor, redo});
-    if (loss) pair_finish_kernel<<<1, 1024, 0, st>>>(workspace, pairs, loss);
+    auto kernel = fours ? pair_kernel<E, 4> : pair_kernel<E, 1>;
+    const int rc = launch_chained(kernel, dim3(static_cast<unsigned>(a.pairs * parts)), dim3(PT_THREADS), 0, st, parts, false, a,
+                                  static_cast<E*>(c->grad), c->workspace, c->rewards, Upstream{c->factor, static_cast<int>(c->redo)});
+    if (rc) return rc;
+    if (c->loss) pair_finish_kernel<<<1, 1024, 0, st>>>(c->workspace, a.pairs, c->loss);
+    return static_cast<int>(cudaGetLastError());
   });
 }

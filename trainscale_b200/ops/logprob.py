@@ -12,13 +12,15 @@ import torch
 from . import _lib
 
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+_PLAIN = (torch.Tensor, torch.nn.Parameter)
 
 
 def on_this_gpu(*tensors) -> bool:
-    """Plain CUDA tensors of the current device, outside functorch transforms and forward-mode differentiation."""
-    return (all(type(t) in (torch.Tensor, torch.nn.Parameter) and t.is_cuda and t.get_device() == torch._C._cuda_getDevice()
-                for t in tensors)
-            and not torch._C._are_functorch_transforms_active() and torch.autograd.forward_ad._current_level < 0)
+    """Plain CUDA tensors of the current device (or None), outside functorch transforms and forward-mode differentiation."""
+    for t in tensors:
+        if t is not None and (type(t) not in _PLAIN or not t.is_cuda or t.get_device() != torch._C._cuda_getDevice()):
+            return False
+    return not torch._C._are_functorch_transforms_active() and torch.autograd.forward_ad._current_level < 0
 
 
 def native(logits: torch.Tensor, labels: torch.Tensor) -> bool:

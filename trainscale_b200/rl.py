@@ -180,7 +180,7 @@ def clipped_policy_loss(logp: torch.Tensor, old_logp: torch.Tensor, advantages: 
     if max_len is not None and max_len <= 0:
         raise ValueError(f"max_len is {max_len}")
     loss, stats = policy_ops.policy_loss(logp, old_logp, advantages, mask, ref_logp, float(clip), float(high), float(beta), reduction,
-                                         max_len)
+                                         max_len, return_stats)
     return (loss, PolicyStats(*stats.unbind())) if return_stats else loss
 
 
