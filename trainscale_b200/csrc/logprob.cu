@@ -8,8 +8,9 @@
 // logits cost no bits and rows of a type's lowest value do not overflow.  S = sum 2^u and U = sum u 2^u give
 // logp = k ln2 (v_label - m) - ln S and H = ln S - ln2 U / S, both terms of which are positive: nothing cancels.
 //
-// Forward reads the logits once: every thread keeps a running (m, S, U) over 16-byte vectors and raises m once for the vectors that
-// it has in flight; the triples meet in the block and, where a row is split, in the cluster's shared memory.
+// Forward reads the logits once: a thread keeps a running (m, S, U) over 16-byte vectors and raises m once for the vectors that it
+// has in flight.  Few rows: a block or a cluster per row, one launch.  Many: a warp per part of a row, all of them alike, so that
+// blocks end evenly and nothing waits inside a block; a second launch joins a row's parts.
 #include <cooperative_groups.h>
 
 #include "common.cuh"
@@ -20,6 +21,8 @@ namespace ts {
 constexpr int LP_THREADS = 512;
 constexpr int LP_FLIGHT = 4;             // vectors of a thread in flight
 constexpr int LP_SPLIT = 8;              // most blocks of a row
+constexpr int LP_BACK_THREADS = 64, LP_BACK_FLIGHT = 8;
+constexpr int LP_PART_THREADS = 128, LP_PART_FLIGHT = 4, LP_PART = 1024;     // vectors of a warp's part
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 constexpr float LP_LOWEST = -1e30f;      // 2^u = 0, and u 2^u = 0 as well
 
@@ -35,12 +38,24 @@ __device__ __forceinline__ float fast_rcp(float x) {
   return y;
 }
 
+// Pairs of fp32 in one instruction.
+struct Pair {
+  uint64_t v;
+  __device__ __forceinline__ Pair(uint64_t x) : v(x) {}
+  __device__ __forceinline__ Pair(float a, float b) : v(pack_f32x2(a, b)) {}
+  __device__ __forceinline__ Pair operator+(Pair o) const { return add_f32x2(v, o.v); }
+  __device__ __forceinline__ Pair operator*(Pair o) const { return mul_f32x2(v, o.v); }
+  __device__ __forceinline__ float2 get() const { return unpack_f32x2(v); }
+};
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) { return fma_f32x2(a.v, b.v, c.v); }
+
 // 16 bytes of logits: N values, their largest, and the pattern of a value that counts for nothing.
 template <typename T>
 struct Vec;
 template <>
 struct Vec<float> {
   static constexpr int N = 4;
+  static __device__ __forceinline__ uint4 nothing() { return make_uint4(NOTHING, NOTHING, NOTHING, NOTHING); }
   static constexpr uint32_t NOTHING = 0xff800000u;
   static __device__ __forceinline__ float value(float v) { return v; }
   static __device__ __forceinline__ float round(float v) { return v; }
@@ -64,6 +79,7 @@ struct Vec<float> {
 template <>
 struct Vec<__nv_bfloat16> {
   static constexpr int N = 8;
+  static __device__ __forceinline__ uint4 nothing() { return make_uint4(NOTHING, NOTHING, NOTHING, NOTHING); }
   static constexpr uint32_t NOTHING = 0xff80ff80u;
   static __device__ __forceinline__ float value(__nv_bfloat16 v) { return __bfloat162float(v); }
   static __device__ __forceinline__ __nv_bfloat16 round(float v) { return __float2bfloat16(v); }
@@ -90,6 +106,7 @@ struct Vec<__nv_bfloat16> {
 template <>
 struct Vec<__half> {
   static constexpr int N = 8;
+  static __device__ __forceinline__ uint4 nothing() { return make_uint4(NOTHING, NOTHING, NOTHING, NOTHING); }
   static constexpr uint32_t NOTHING = 0xfc00fc00u;
   static __device__ __forceinline__ float value(__half v) { return __half2float(v); }
   static __device__ __forceinline__ __half round(float v) { return __float2half(v); }
@@ -121,6 +138,13 @@ struct Vec<__half> {
   }
 };
 
+// Logits are read once in each direction and are gone by then: they pass the L1 by.
+__device__ __forceinline__ uint4 load_once(const uint4* p) {
+  uint4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
+
 struct LogitRows {
   long long rows, inner;             // row r is (r / inner, r % inner)
   long long stride_outer, stride_inner;
@@ -133,14 +157,28 @@ struct LogitRows {
   }
 };
 
-// tanh(z / c) out of E = e^(-2 |z| / c) <= 1, so that the slope 1 - tanh^2 = 4 E / (1 + E)^2 keeps its bits where tanh is close to one
-// (two special-function calls; off by 2^-23 of one).
+// tanh(z / c) out of E = e^(-2 |z| / c) <= 1, so that the slope 1 - tanh^2 = 4 E / (1 + E)^2 keeps its bits where tanh is close to one;
+// off by 2^-22 of one.
 template <bool CAP>
 __device__ __forceinline__ float capped(float z, float inv_cap, float* slope = nullptr) {
   if (!CAP) return z;
   const float e = fast_ex2(fabsf(z) * (-2.f * LOG2E * inv_cap)), r = fast_rcp(1.f + e);
   if (slope) *slope = 4.f * e * r * r;
   return copysignf((1.f - e) * r, z);
+}
+// Two at once, 1 / (1 + E) by Newton's iteration from a parabola through it at E = 0, 1/2 and 1 (off by 0.009, then by 1e-4 and 1e-8):
+// two calls of the special-function unit for an element instead of three, which is what bounds the forward pass.
+template <bool CAP>
+__device__ __forceinline__ Pair capped2(float x, float y, float inv_cap) {
+  if (!CAP) return Pair(x, y);
+  const float f = -2.f * LOG2E * inv_cap;
+  const Pair e(fast_ex2(fabsf(x) * f), fast_ex2(fabsf(y) * f)), one(1.f, 1.f), two(2.f, 2.f), minus(-1.f, -1.f);
+  const Pair d = (e + one) * minus;
+  Pair r = fma2(e, fma2(e, Pair(1.f / 3.f, 1.f / 3.f), Pair(-5.f / 6.f, -5.f / 6.f)), one);
+  r = r * fma2(d, r, two);
+  r = r * fma2(d, r, two);
+  const float2 t = (fma2(e, minus, one) * r).get();
+  return Pair(copysignf(t.x, x), copysignf(t.y, y));
 }
 
 struct Softmax {
@@ -165,82 +203,141 @@ struct Softmax {
   }
 };
 
+// u of one value, where m is a finite maximum or there is none yet; never below LP_LOWEST, so that u 2^u is zero where 2^u is.
+__device__ __forceinline__ float exponent(float v, float m, float k2) { return max_nan(k2 * (v - (m == -INFINITY ? 0.f : m)), LP_LOWEST); }
+
+template <bool CAP, bool ENT>
+__device__ __forceinline__ void add_value(Softmax& acc, float z, float k2, float inv_cap) {
+  const float v = capped<CAP>(z, inv_cap);
+  acc.raise<ENT>(max_nan(acc.m, v), k2);
+  const float t = exponent(v, acc.m, k2), e = fast_ex2(t);
+  acc.s += e;
+  if (ENT) acc.u += t * e;
+}
+
+// Adds N 16-byte vectors to a thread's (m, S, U).  An entropy's 0 * -inf (logits of -inf) shows as NaN; it is then summed again with
+// exponents that are bounded below.
+template <typename T, bool CAP, bool ENT, int N>
+__device__ __forceinline__ void add_vectors(Softmax& acc, const uint4* r, float k2, float inv_cap) {
+  using W = Vec<T>;
+  const float top = max_nan(acc.m, capped<CAP>(W::largest(r, N), inv_cap));
+  acc.raise<ENT>(top, k2);
+  const float m = top == -INFINITY ? 0.f : top;
+  const Pair minus(-m, -m), k(k2, k2);
+  Pair s(0.f, 0.f), u(0.f, 0.f);
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    float f[W::N];
+    W::unpack(r[j], f);
+#pragma unroll
+    for (int e = 0; e < W::N; e += 2) {
+      const Pair t = (capped2<CAP>(f[e], f[e + 1], inv_cap) + minus) * k;
+      const float2 x = t.get();
+      const Pair p(fast_ex2(x.x), fast_ex2(x.y));
+      s = s + p;
+      if (ENT) u = fma2(t, p, u);
+    }
+  }
+  const float2 x = s.get();
+  acc.s += x.x + x.y;
+  if (!ENT) return;
+  const float2 y = u.get();
+  float extra = y.x + y.y;
+  if (extra != extra) {
+    extra = 0.f;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      float f[W::N];
+      W::unpack(r[j], f);
+#pragma unroll 1
+      for (int e = 0; e < W::N; ++e) {
+        const float t = exponent(capped<CAP>(f[e], inv_cap), top, k2);
+        extra += t * fast_ex2(t);
+      }
+    }
+  }
+  acc.u += extra;
+}
+
+template <bool ENT>
+__device__ __forceinline__ void join_warp(Softmax& x, float k2) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) {
+    Softmax b;
+    b.m = __shfl_xor_sync(0xffffffffu, x.m, o);
+    b.s = __shfl_xor_sync(0xffffffffu, x.s, o);
+    if (ENT) b.u = __shfl_xor_sync(0xffffffffu, x.u, o);
+    x.join<ENT>(b, k2);
+  }
+}
+
+// A row: values before its first 16-byte boundary, vectors, values behind the last.
+template <typename T>
+struct Row {
+  const T* z;
+  int head, vectors, V;
+  __device__ __forceinline__ Row(const T* at, int n) : z(at), V(n) {
+    head = min(n, static_cast<int>((16 - (reinterpret_cast<uintptr_t>(at) & 15)) & 15) / static_cast<int>(sizeof(T)));
+    vectors = (n - head) / Vec<T>::N;
+  }
+  __device__ __forceinline__ const uint4* body() const { return reinterpret_cast<const uint4*>(z + head); }
+  __device__ __forceinline__ int extra() const { return V - vectors * Vec<T>::N; }            // fewer than two vectors
+  __device__ __forceinline__ int lone(int i) const { return i < head ? i : i + vectors * Vec<T>::N; }
+};
+
+// What a row's (m, S, U) come to.
+template <typename T, bool CAP>
+__device__ __forceinline__ void row_results(const Softmax& x, const Row<T>& row, long long r, long long label, const LogitRows& a,
+                                            float* logp, float* entropy, float4* kept) {
+  const bool outside = label < 0 || label >= a.V;
+  // a row whose largest logit is +inf, -inf or NaN has no distribution
+  const bool proper = x.m - x.m == 0.f;
+  const float v = outside ? NAN : capped<CAP>(Vec<T>::value(row.z[label]), a.inv_cap);
+  logp[r] = proper ? a.k * (v - x.m) - logf(x.s) : v - x.m;
+  const float H = proper ? logf(x.s) - LN2 * (x.u / x.s) : NAN;
+  if (entropy) entropy[r] = H;
+  if (kept) kept[r] = make_float4(x.m, x.s, H, 0.f);
+}
+__device__ __forceinline__ void ignored_row(long long r, float* logp, float* entropy, float4* kept) {
+  logp[r] = 0.f;
+  if (entropy) entropy[r] = 0.f;
+  if (kept) kept[r] = make_float4(0.f, 1.f, 0.f, 0.f);
+}
+
 // One block per row, or a cluster of them.
 template <typename T, bool CAP, bool ENT>
-__global__ void __launch_bounds__(LP_THREADS) logprob_fwd_kernel(const T* __restrict__ logits, const long long* __restrict__ labels,
+__global__ void __launch_bounds__(LP_THREADS) logprob_row_kernel(const T* __restrict__ logits, const long long* __restrict__ labels,
                                                                  float* __restrict__ logp, float* __restrict__ entropy,
                                                                  float4* __restrict__ kept, LogitRows a) {
-  using W = Vec<T>;
   namespace cg = cooperative_groups;
   cg::cluster_group cluster = cg::this_cluster();
   const int rank = static_cast<int>(cluster.block_rank()), parts = static_cast<int>(cluster.num_blocks());
   __shared__ Softmax by_warp[LP_THREADS / 32];
   __shared__ Softmax by_block[LP_SPLIT];
-  const long long row = blockIdx.x / parts;
-  const long long label = labels[row];
+  const long long r = blockIdx.x / parts, label = labels[r];
   if (label == a.ignore) {
-    if (threadIdx.x == 0 && rank == 0) {
-      logp[row] = 0.f;
-      if (entropy) entropy[row] = 0.f;
-      if (kept) kept[row] = make_float4(0.f, 1.f, 0.f, 0.f);
-    }
+    if (threadIdx.x == 0 && rank == 0) ignored_row(r, logp, entropy, kept);
     return;                                   // (the whole cluster: it has one row)
   }
-  const T* z = logits + a.offset(row);
-  // values before the first 16-byte boundary, vectors, values after the last one
-  const int head = min(a.V, static_cast<int>((16 - (reinterpret_cast<uintptr_t>(z) & 15)) & 15) / static_cast<int>(sizeof(T)));
-  const int vectors = (a.V - head) / W::N, tail = head + vectors * W::N;
-  const uint4* body = reinterpret_cast<const uint4*>(z + head);
-  const int begin = static_cast<int>(static_cast<long long>(vectors) * rank / parts);
-  const int end = static_cast<int>(static_cast<long long>(vectors) * (rank + 1) / parts);
-  const uint4 nothing = make_uint4(W::NOTHING, W::NOTHING, W::NOTHING, W::NOTHING);
-
+  const Row<T> row(logits + a.offset(r), a.V);
+  const uint4* body = row.body();
+  const int begin = static_cast<int>(static_cast<long long>(row.vectors) * rank / parts);
+  const int end = static_cast<int>(static_cast<long long>(row.vectors) * (rank + 1) / parts);
   Softmax acc;
-  auto add = [&](float v, float m) {
-    const float t = a.k2 * (v - m), e = fast_ex2(t);
-    acc.s += e;
-    if (ENT) acc.u += max_nan(t, LP_LOWEST) * e;
-  };
   for (int i = begin + static_cast<int>(threadIdx.x); i < end; i += LP_THREADS * LP_FLIGHT) {
-    uint4 r[LP_FLIGHT];
+    uint4 v[LP_FLIGHT];
 #pragma unroll
-    for (int j = 0; j < LP_FLIGHT; ++j) r[j] = i + j * LP_THREADS < end ? __ldg(body + i + j * LP_THREADS) : nothing;
-    const float top = max_nan(acc.m, capped<CAP>(W::largest(r, LP_FLIGHT), a.inv_cap));
-    acc.raise<ENT>(top, a.k2);
-    const float m = top == -INFINITY ? 0.f : top;
-#pragma unroll
-    for (int j = 0; j < LP_FLIGHT; ++j) {
-      float f[W::N];
-      W::unpack(r[j], f);
-#pragma unroll
-      for (int e = 0; e < W::N; ++e) add(capped<CAP>(f[e], a.inv_cap), m);
-    }
+    for (int j = 0; j < LP_FLIGHT; ++j) v[j] = i + j * LP_THREADS < end ? load_once(body + i + j * LP_THREADS) : Vec<T>::nothing();
+    add_vectors<T, CAP, ENT, LP_FLIGHT>(acc, v, a.k2, a.inv_cap);
   }
-  if (rank == 0) {
-    const int extra = a.V - vectors * W::N;   // fewer than two vectors
-    if (static_cast<int>(threadIdx.x) < extra) {
-      const int i = static_cast<int>(threadIdx.x) < head ? threadIdx.x : tail + (threadIdx.x - head);
-      const float v = capped<CAP>(W::value(z[i]), a.inv_cap);
-      acc.raise<ENT>(max_nan(acc.m, v), a.k2);
-      add(v, acc.m == -INFINITY ? 0.f : acc.m);
-    }
-  }
-  auto join_warp = [&](Softmax& x) {
-#pragma unroll
-    for (int o = 16; o; o >>= 1) {
-      Softmax b;
-      b.m = __shfl_xor_sync(0xffffffffu, x.m, o);
-      b.s = __shfl_xor_sync(0xffffffffu, x.s, o);
-      if (ENT) b.u = __shfl_xor_sync(0xffffffffu, x.u, o);
-      x.join<ENT>(b, a.k2);
-    }
-  };
-  join_warp(acc);
+  if (rank == 0 && static_cast<int>(threadIdx.x) < row.extra())
+    add_value<CAP, ENT>(acc, Vec<T>::value(row.z[row.lone(threadIdx.x)]), a.k2, a.inv_cap);
+  join_warp<ENT>(acc, a.k2);
   if ((threadIdx.x & 31) == 0) by_warp[threadIdx.x >> 5] = acc;
   __syncthreads();
   if (threadIdx.x < 32) {
     acc = threadIdx.x < LP_THREADS / 32 ? by_warp[threadIdx.x] : Softmax();
-    join_warp(acc);
+    join_warp<ENT>(acc, a.k2);
   }
   if (parts > 1) {
     if (threadIdx.x == 0) *cluster.map_shared_rank(by_block + rank, 0) = acc;
@@ -251,21 +348,80 @@ __global__ void __launch_bounds__(LP_THREADS) logprob_fwd_kernel(const T* __rest
       for (int i = 1; i < parts; ++i) acc.join<ENT>(by_block[i], a.k2);
     }
   }
-  if (threadIdx.x == 0) {
-    const bool outside = label < 0 || label >= a.V;
-    // a row whose largest logit is +inf, -inf or NaN has no distribution
-    const bool proper = acc.m - acc.m == 0.f;
-    const float v = outside ? NAN : capped<CAP>(W::value(z[label]), a.inv_cap);
-    logp[row] = proper ? a.k * (v - acc.m) - logf(acc.s) : v - acc.m;
-    const float H = proper ? logf(acc.s) - LN2 * (acc.u / acc.s) : NAN;
-    if (entropy) entropy[row] = H;
-    if (kept) kept[row] = make_float4(acc.m, acc.s, H, 0.f);
-  }
+  if (threadIdx.x == 0) row_results<T, CAP>(acc, row, r, label, a, logp, entropy, kept);
 }
 
-// A block takes LP_THREADS * LP_FLIGHT vectors of one row.
+// A warp per part of a row: LP_PART vectors of it, or all where that is one part.
 template <typename T, bool CAP, bool ENT>
-__global__ void __launch_bounds__(LP_THREADS) logprob_bwd_kernel(const T* __restrict__ logits, const long long* __restrict__ labels,
+__global__ void __launch_bounds__(LP_PART_THREADS) logprob_part_kernel(const T* __restrict__ logits, const long long* __restrict__ labels,
+                                                                       Softmax* __restrict__ partial, float* __restrict__ logp,
+                                                                       float* __restrict__ entropy, float4* __restrict__ kept,
+                                                                       LogitRows a, int parts) {
+  constexpr int step = 32 * LP_PART_FLIGHT;
+  const long long unit = blockIdx.x * static_cast<long long>(LP_PART_THREADS / 32) + (threadIdx.x >> 5), r = unit / parts;
+  const int lane = threadIdx.x & 31;
+  if (r >= a.rows) return;
+  const long long label = labels[r];
+  if (label == a.ignore) {
+    if (parts == 1 && lane == 0) ignored_row(r, logp, entropy, kept);
+    return;
+  }
+  const Row<T> row(logits + a.offset(r), a.V);
+  const int begin = static_cast<int>(unit - r * parts) * LP_PART, end = parts == 1 ? row.vectors : min(row.vectors, begin + LP_PART);
+  const uint4* body = row.body() + lane;
+  Softmax acc;
+  uint4 v[LP_PART_FLIGHT], next[LP_PART_FLIGHT];
+  int i = begin;
+  if (i + step <= end) {
+#pragma unroll
+    for (int j = 0; j < LP_PART_FLIGHT; ++j) next[j] = load_once(body + i + j * 32);
+    for (; i + step <= end; i += step) {
+#pragma unroll
+      for (int j = 0; j < LP_PART_FLIGHT; ++j) v[j] = next[j];
+      if (i + 2 * step <= end)
+#pragma unroll
+        for (int j = 0; j < LP_PART_FLIGHT; ++j) next[j] = load_once(body + i + step + j * 32);
+      add_vectors<T, CAP, ENT, LP_PART_FLIGHT>(acc, v, a.k2, a.inv_cap);
+    }
+  }
+  if (i < end) {
+#pragma unroll
+    for (int j = 0; j < LP_PART_FLIGHT; ++j) v[j] = i + lane + j * 32 < end ? load_once(body + i + j * 32) : Vec<T>::nothing();
+    add_vectors<T, CAP, ENT, LP_PART_FLIGHT>(acc, v, a.k2, a.inv_cap);
+  }
+  if (parts == 1 && lane < row.extra()) add_value<CAP, ENT>(acc, Vec<T>::value(row.z[row.lone(lane)]), a.k2, a.inv_cap);
+  join_warp<ENT>(acc, a.k2);
+  if (lane != 0) return;
+  if (parts == 1) row_results<T, CAP>(acc, row, r, label, a, logp, entropy, kept);
+  else partial[unit] = acc;
+}
+
+// A warp per row joins its parts, and the values that are not in a vector.
+template <typename T, bool CAP, bool ENT>
+__global__ void __launch_bounds__(LP_PART_THREADS) logprob_join_kernel(const T* __restrict__ logits, const long long* __restrict__ labels,
+                                                                       const Softmax* __restrict__ partial, float* __restrict__ logp,
+                                                                       float* __restrict__ entropy, float4* __restrict__ kept,
+                                                                       LogitRows a, int parts) {
+  const long long r = blockIdx.x * static_cast<long long>(LP_PART_THREADS / 32) + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  if (r >= a.rows) return;
+  grid_wait();
+  const long long label = labels[r];
+  if (label == a.ignore) {
+    if (lane == 0) ignored_row(r, logp, entropy, kept);
+    return;
+  }
+  const Row<T> row(logits + a.offset(r), a.V);
+  Softmax acc;
+  if (lane < row.extra()) add_value<CAP, ENT>(acc, Vec<T>::value(row.z[row.lone(lane)]), a.k2, a.inv_cap);
+  for (int i = lane; i < parts; i += 32) acc.join<ENT>(partial[r * parts + i], a.k2);
+  join_warp<ENT>(acc, a.k2);
+  if (lane == 0) row_results<T, CAP>(acc, row, r, label, a, logp, entropy, kept);
+}
+
+// A block takes LP_BACK_THREADS * LP_BACK_FLIGHT vectors of one row.
+template <typename T, bool CAP, bool ENT>
+__global__ void __launch_bounds__(LP_BACK_THREADS) logprob_bwd_kernel(const T* __restrict__ logits, const long long* __restrict__ labels,
                                                                  const float4* __restrict__ kept, const float* __restrict__ grad_logp,
                                                                  const float* __restrict__ grad_entropy, T* __restrict__ grad,
                                                                  LogitRows a, int parts) {
@@ -281,22 +437,22 @@ __global__ void __launch_bounds__(LP_THREADS) logprob_bwd_kernel(const T* __rest
   const int head = min(a.V, static_cast<int>((16 - (reinterpret_cast<uintptr_t>(d) & 15)) & 15) / static_cast<int>(sizeof(T)));
   const int vectors = (a.V - head) / W::N, tail = head + vectors * W::N;
   uint4* out = reinterpret_cast<uint4*>(d + head);
-  const int first = part * (LP_THREADS * LP_FLIGHT) + static_cast<int>(threadIdx.x);
+  const int first = part * (LP_BACK_THREADS * LP_BACK_FLIGHT) + static_cast<int>(threadIdx.x);
   const int extra = part == 0 ? a.V - vectors * W::N : 0;
   const int lone = static_cast<int>(threadIdx.x) < head ? threadIdx.x : tail + (threadIdx.x - head);
   if (still) {
 #pragma unroll
-    for (int j = 0; j < LP_FLIGHT; ++j)
-      if (first + j * LP_THREADS < vectors) out[first + j * LP_THREADS] = make_uint4(0, 0, 0, 0);
+    for (int j = 0; j < LP_BACK_FLIGHT; ++j)
+      if (first + j * LP_BACK_THREADS < vectors) out[first + j * LP_BACK_THREADS] = make_uint4(0, 0, 0, 0);
     if (static_cast<int>(threadIdx.x) < extra) d[lone] = W::round(0.f);
     return;
   }
   const bool aligned = ((reinterpret_cast<uintptr_t>(z) ^ reinterpret_cast<uintptr_t>(d)) & 15) == 0;
   const uint4* body = reinterpret_cast<const uint4*>(z + head);
-  uint4 r[LP_FLIGHT];
+  uint4 r[LP_BACK_FLIGHT];
   if (aligned) {
 #pragma unroll
-    for (int j = 0; j < LP_FLIGHT; ++j) r[j] = first + j * LP_THREADS < vectors ? __ldg(body + first + j * LP_THREADS) : make_uint4(0, 0, 0, 0);
+    for (int j = 0; j < LP_BACK_FLIGHT; ++j) r[j] = first + j * LP_BACK_THREADS < vectors ? load_once(body + first + j * LP_BACK_THREADS) : make_uint4(0, 0, 0, 0);
   }
   const float4 k = kept[row];
   const float m = k.x, f = a.k * (CAP ? a.inv_cap : 1.f);
@@ -304,13 +460,25 @@ __global__ void __launch_bounds__(LP_THREADS) logprob_bwd_kernel(const T* __rest
   const float tilt = ENT ? f * h * LN2 / k.y : 0.f, flat = f * (g + (ENT ? h * (k.z - logf(k.y)) : 0.f)) / k.y, fg = f * g;
   auto slope_of = [&](float value, bool chosen) {
     float slope = 1.f;
-    const float u = a.k2 * (capped<CAP>(value, a.inv_cap, &slope) - m);
-    const float r = (chosen ? fg : 0.f) - fast_ex2(u) * (ENT ? flat + tilt * max_nan(u, LP_LOWEST) : flat);
+    const float u = exponent(capped<CAP>(value, a.inv_cap, &slope), m, a.k2);
+    const float r = (chosen ? fg : 0.f) - fast_ex2(u) * (ENT ? flat + tilt * u : flat);
     return CAP ? slope * r : r;
   };
+  const Pair minus(-m, -m), k2(a.k2, a.k2), flat2(-flat, -flat), tilt2(-tilt, -tilt);
+  auto slope_of_two = [&](float x, float y) {
+    float sx = 1.f, sy = 1.f;
+    Pair t = (Pair(capped<CAP>(x, a.inv_cap, &sx), capped<CAP>(y, a.inv_cap, &sy)) + minus) * k2;
+    float2 u = t.get();
+    if (ENT) {
+      u.x = max_nan(u.x, LP_LOWEST), u.y = max_nan(u.y, LP_LOWEST);
+      t = Pair(u.x, u.y);
+    }
+    const Pair r = Pair(fast_ex2(u.x), fast_ex2(u.y)) * (ENT ? fma2(tilt2, t, flat2) : flat2);
+    return (CAP ? r * Pair(sx, sy) : r).get();
+  };
 #pragma unroll
-  for (int j = 0; j < LP_FLIGHT; ++j) {
-    const int i = first + j * LP_THREADS;
+  for (int j = 0; j < LP_BACK_FLIGHT; ++j) {
+    const int i = first + j * LP_BACK_THREADS;
     if (i >= vectors) break;
     float v[W::N], o[W::N];
     if (aligned) {
@@ -320,14 +488,18 @@ __global__ void __launch_bounds__(LP_THREADS) logprob_bwd_kernel(const T* __rest
       for (int e = 0; e < W::N; ++e) v[e] = W::value(z[head + i * W::N + e]);
     }
 #pragma unroll
-    for (int e = 0; e < W::N; ++e) o[e] = slope_of(v[e], false);
+    for (int e = 0; e < W::N; e += 2) {
+      const float2 t = slope_of_two(v[e], v[e + 1]);
+      o[e] = t.x;
+      o[e + 1] = t.y;
+    }
     const long long at = label - head - static_cast<long long>(i) * W::N;
     if (at >= 0 && at < W::N) {
 #pragma unroll
       for (int e = 0; e < W::N; ++e)
         if (e == at) o[e] = slope_of(v[e], true);
     }
-    out[i] = W::pack(o);
+    __stcs(out + i, W::pack(o));
   }
   if (static_cast<int>(threadIdx.x) < extra) d[lone] = W::round(slope_of(W::value(z[lone]), lone == label));
 }
@@ -361,22 +533,46 @@ using namespace ts;
 
 TS_DEFINE_ERROR_API(ts_logprob)
 
-// dtype: 0 bf16, 1 fp16, 2 fp32.  kept: (m, S, H, unused) of every row, for the backward pass; H counts only with `with_entropy`.
+// Parts of a row that warps of their own take; 0: a block or a cluster takes the row.  Rows have blocks of their own while those are
+// fewer than two to an SM.
+static int row_parts(long long rows, int V, int dtype) {
+  const long long vectors = static_cast<long long>(V) * (dtype == 2 ? 4 : 2) / 16;
+  return rows < 2 * sm_count() ? 0 : static_cast<int>((vectors + LP_PART - 1) / LP_PART) + (vectors == 0);
+}
+
+// Bytes of workspace that ts_logprob_fwd needs.
+extern "C" long long ts_logprob_workspace(long long rows, int V, int dtype) {
+  const int parts = row_parts(rows, V, dtype);
+  return parts > 1 ? rows * parts * static_cast<long long>(sizeof(Softmax)) : 0;
+}
+
+// dtype: 0 bf16, 1 fp16, 2 fp32.  kept: (m, S, H, unused) of every row, for the backward pass; H counts only with an entropy.
 // entropy and kept may be null.
 extern "C" int ts_logprob_fwd(const void* logits, int dtype, const long long* labels, float* logp, float* entropy, float4* kept,
-                              long long rows, long long inner, long long stride_outer, long long stride_inner, int V, float factor,
-                              float cap, long long ignore, void* stream) {
-  if (rows <= 0 || inner <= 0 || V <= 0 || rows > 0x7fffffffll / LP_SPLIT) return -1;
+                              void* workspace, long long rows, long long inner, long long stride_outer, long long stride_inner, int V,
+                              float factor, float cap, long long ignore, void* stream) {
+  constexpr int warps = LP_PART_THREADS / 32;
+  const int units = row_parts(rows, V, dtype);
+  if (rows <= 0 || inner <= 0 || V <= 0 || rows > 0x7fffffffll / (units > LP_SPLIT ? units : LP_SPLIT)) return -1;
   const LogitRows a = logit_rows(rows, inner, stride_outer, stride_inner, V, factor, cap, ignore);
-  // a row is split while blocks are fewer than two to an SM and a part has a vector for every thread
-  int parts = 1;
-  const long long vectors = static_cast<long long>(V) * (dtype == 2 ? 4 : 2) / 16;
-  while (parts < LP_SPLIT && rows * parts < 2 * sm_count() && vectors / parts >= 2 * LP_THREADS) parts *= 2;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
   return by_type(dtype, cap > 0.f, entropy != nullptr, [&](auto* t, auto c, auto e) {
     using T = std::remove_pointer_t<decltype(t)>;
-    return launch_chained(logprob_fwd_kernel<T, decltype(c)::value, decltype(e)::value>, dim3(static_cast<unsigned>(rows * parts)),
-                          dim3(LP_THREADS), 0, static_cast<cudaStream_t>(stream), parts, false, static_cast<const T*>(logits), labels,
-                          logp, entropy, kept, a);
+    constexpr bool CAP = decltype(c)::value, ENT = decltype(e)::value;
+    const T* z = static_cast<const T*>(logits);
+    if (units) {
+      Softmax* partial = static_cast<Softmax*>(workspace);
+      logprob_part_kernel<T, CAP, ENT><<<static_cast<unsigned>((rows * units + warps - 1) / warps), LP_PART_THREADS, 0, st>>>(
+          z, labels, partial, logp, entropy, kept, a, units);
+      if (units == 1) return static_cast<int>(cudaGetLastError());
+      return launch_chained(logprob_join_kernel<T, CAP, ENT>, dim3(static_cast<unsigned>((rows + warps - 1) / warps)), dim3(LP_PART_THREADS), 0,
+                            st, 1, true, z, labels, partial, logp, entropy, kept, a, units);
+    }
+    int parts = 1;                       // of a cluster, each with a vector or two for every thread
+    const long long vectors = static_cast<long long>(V) * static_cast<int>(sizeof(T)) / 16;
+    while (parts < LP_SPLIT && rows * parts < 2 * sm_count() && vectors / parts >= 2 * LP_THREADS) parts *= 2;
+    return launch_chained(logprob_row_kernel<T, CAP, ENT>, dim3(static_cast<unsigned>(rows * parts)), dim3(LP_THREADS), 0, st, parts, false,
+                          z, labels, logp, entropy, kept, a);
   });
 }
 
@@ -385,13 +581,13 @@ extern "C" int ts_logprob_bwd(const void* logits, int dtype, const long long* la
                               const float* grad_entropy, void* grad, long long rows, long long inner, long long stride_outer,
                               long long stride_inner, int V, float factor, float cap, long long ignore, void* stream) {
   const long long vectors = static_cast<long long>(V) * (dtype == 2 ? 4 : 2) / 16;
-  const long long parts = vectors / (LP_THREADS * LP_FLIGHT) + 1;
+  const long long parts = vectors / (LP_BACK_THREADS * LP_BACK_FLIGHT) + 1;
   if (rows <= 0 || inner <= 0 || V <= 0 || rows > 0x7fffffffll / parts || !kept) return -1;
   const LogitRows a = logit_rows(rows, inner, stride_outer, stride_inner, V, factor, cap, ignore);
   return by_type(dtype, cap > 0.f, grad_entropy != nullptr, [&](auto* t, auto c, auto e) {
     using T = std::remove_pointer_t<decltype(t)>;
     logprob_bwd_kernel<T, decltype(c)::value, decltype(e)::value>
-        <<<static_cast<unsigned>(rows * parts), LP_THREADS, 0, static_cast<cudaStream_t>(stream)>>>(
+        <<<static_cast<unsigned>(rows * parts), LP_BACK_THREADS, 0, static_cast<cudaStream_t>(stream)>>>(
             static_cast<const T*>(logits), labels, kept, grad_logp, grad_entropy, static_cast<T*>(grad), a, static_cast<int>(parts));
     return static_cast<int>(cudaGetLastError());
   });

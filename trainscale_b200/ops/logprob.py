@@ -5,6 +5,7 @@ is fp32.  Reference behaviour: data_pipeline/trainer/rl_training.py:95-191 (soft
 """
 from __future__ import annotations
 
+import functools
 import math
 
 import torch
@@ -66,13 +67,21 @@ def _tail(rows, V, factor, cap, ignore_index):
 _fns: dict = {}
 
 
+@functools.lru_cache(maxsize=None)
+def _workspace():
+    from ctypes import c_int, c_longlong
+    fn = _lib.load("logprob").ts_logprob_workspace
+    fn.argtypes, fn.restype = [c_longlong, c_int, c_int], c_longlong
+    return fn
+
+
 def _call(name: str, *args) -> None:
     fn = _fns.get(name)
     if fn is None:
         from ctypes import c_float, c_int, c_longlong, c_void_p
         fn = getattr(_lib.load("logprob"), name)
         shape = [c_longlong] * 4 + [c_int, c_float, c_float, c_longlong, c_void_p]
-        fn.argtypes = [c_void_p, c_int] + [c_void_p] * (4 if name == "ts_logprob_fwd" else 5) + shape
+        fn.argtypes = [c_void_p, c_int] + [c_void_p] * 5 + shape
         _fns[name] = fn
     _lib.check(fn(*args), name)
 
@@ -83,8 +92,10 @@ def _forward(logits, labels, factor, cap, ignore_index, entropy: bool, keep: boo
     logp = torch.empty(labels.shape, **f32)
     H = torch.empty(labels.shape, **f32) if entropy else None
     kept = torch.empty(labels.numel(), 4, **f32) if keep else None
+    need = _workspace()(labels.numel(), x.shape[-1], _DTYPES[x.dtype])
+    work = torch.empty(need, dtype=torch.uint8, device=logits.device) if need else None
     _call("ts_logprob_fwd", _lib.ptr(x), _DTYPES[x.dtype], _lib.ptr(labels), _lib.ptr(logp), _lib.ptr(H), _lib.ptr(kept),
-          *_tail(rows, x.shape[-1], factor, cap, ignore_index))
+          _lib.ptr(work), *_tail(rows, x.shape[-1], factor, cap, ignore_index))
     return logp, H, kept
 
 
