@@ -110,7 +110,7 @@ def test_nothing_to_learn_from():
 def test_refusals():
     z, y = torch.zeros(2, 3, 5), torch.zeros(2, 3, dtype=torch.long)
     for kw in (dict(temperature=0.0), dict(temperature=math.inf), dict(temperature=-1.0), dict(logit_softcapping=-1.0),
-               dict(logit_scale=-2.0), dict(logit_softcapping=math.nan)):
+               dict(logit_scale=-2.0), dict(logit_softcapping=math.nan), dict(temperature=1e-35), dict(logit_scale=1e20, logit_softcapping=1e15)):
         with pytest.raises(ValueError):
             token_log_probs(z, y, **kw)
     with pytest.raises(ValueError):

@@ -134,6 +134,85 @@ def test_logits_that_are_not_finite_or_far_apart(dtype):
     assert (lp[:2] == 0).all() and lp[2:4].isnan().all()
 
 
+@pytest.mark.parametrize("cap", [0.5, 5.0, 300.0, 1e6])
+def test_caps_far_below_and_above_the_logits(cap):
+    """A capped logit is off by 2^-21 of its own size, however large the cap."""
+    from trainscale_b200.rl import token_log_probs
+    z = torch.randn(400, 999, device=DEV, generator=_gen(8)) * 4
+    z[0] *= 1e-3
+    y = torch.randint(0, 999, (400,), device=DEV, generator=_gen(9))
+    v = cap * torch.tanh(z.double() / cap)
+    want = torch.log_softmax(v, -1).gather(1, y.unsqueeze(1)).squeeze(1)
+    tol = F32 * (24 * v.abs().amax(1) + 64) + F32 * want.abs()
+    for rows in (400, 3):                                   # a warp per part of a row, and a block per row
+        _near(token_log_probs(z[:rows], y[:rows], logit_softcapping=cap), want[:rows], tol[:rows])
+
+
+def test_offsets_that_pass_32_bits():
+    from trainscale_b200.rl import token_log_probs
+    rows, V = 16500, 131080                                 # 2.16e9 logits
+    z = torch.zeros(rows, V, device=DEV, dtype=torch.bfloat16)
+    some = torch.tensor([0, 1, 16383, 16384, rows - 1], device=DEV)
+    z[some] = (torch.randn(5, V, device=DEV, generator=_gen(1)) * 2).bfloat16()
+    y = torch.randint(0, V, (rows,), device=DEV, generator=_gen(2))
+    x = z.requires_grad_()
+    logp = token_log_probs(x, y)
+    want = torch.log_softmax(z[some].detach().double(), -1)
+    _near(logp[some].detach(), want.gather(1, y[some].unsqueeze(1)).squeeze(1), F32 * 1000)
+    (d,) = torch.autograd.grad(logp.sum(), x)
+    one = torch.zeros_like(want).scatter_(1, y[some].unsqueeze(1), 1.0)
+    _near(d[some], one - want.exp(), 2e-4 * want.exp() + HALF[torch.bfloat16] * (one - want.exp()).abs() * 1.01)
+    assert float(logp[777]) == pytest.approx(-math.log(V), rel=1e-6)
+    del x, z, d
+    stride = (1 << 31) + 8                                  # rows of losses that lie that far apart
+    far = torch.empty(3 * stride + 100, device=DEV, dtype=torch.bfloat16).as_strided((4, 100), (stride, 1))
+    logp, old, adv, mask, ref = _policy_case(4, 100, torch.bfloat16, torch.bool, 3)
+    _check_policy(far.copy_(logp), old, adv, mask, ref)
+    lp, rf, m = _pair_case(2, 100, torch.bfloat16, torch.bool, 3)
+    _check_pairs(far.copy_(lp), rf, m)
+    del far
+    g = torch.full(((1 << 31) + 77,), 2.0, device=DEV, dtype=torch.bfloat16)
+    assert float(_clip([g], 1.0)) == pytest.approx(2 * math.sqrt(g.numel()), rel=1e-6)
+    want = 1.0 / math.sqrt(g.numel())
+    assert float(g[0]) == pytest.approx(want, rel=4e-3) and float(g[-1]) == float(g[0]) == float(g[1 << 31])
+
+
+def test_constants_made_in_inference_mode():
+    from trainscale_b200.rl import clipped_policy_loss, preference_loss, token_log_probs
+    logp, old, adv, mask, ref = _policy_case(6, 50, torch.float32, torch.bool, 3)
+    with torch.inference_mode():
+        a = [t.clone() for t in (old, adv, mask, ref)]
+        y = torch.arange(6, device=DEV)
+    x = logp.clone().requires_grad_()
+    loss = clipped_policy_loss(x, *a, beta=0.1)
+    loss.backward()
+    z = logp.clone().requires_grad_()
+    clipped_policy_loss(z, old, adv, mask, ref, beta=0.1).backward()
+    assert torch.equal(x.grad, z.grad)
+    x = logp.clone().requires_grad_()
+    preference_loss(x, a[3], a[2])[0].backward()
+    w = torch.randn(6, 9, device=DEV, requires_grad=True)
+    token_log_probs(w, y).sum().backward()
+    with torch.inference_mode():
+        clipped_policy_loss(logp, *a, beta=0.1)
+        token_log_probs(w, y, return_entropy=True)
+
+
+def test_inputs_changed_before_their_gradient():
+    from trainscale_b200.rl import clipped_policy_loss
+    logp, old, adv, mask, ref = _policy_case(6, 50, torch.float32, torch.bool, 3, spoil=False)
+    x = logp.clone().requires_grad_()
+    loss = clipped_policy_loss(x, old, adv, mask, ref, beta=0.1)
+    (a,) = torch.autograd.grad(loss, x, retain_graph=True)
+    old.zero_()                                             # a second pass would need it
+    with pytest.raises(RuntimeError, match="changed in place"):
+        torch.autograd.grad(loss, x)
+    loss = clipped_policy_loss(x, old, adv, mask, ref, beta=0.1)
+    loss.backward()
+    with pytest.raises(RuntimeError, match="second time"):
+        loss.backward()
+
+
 def test_rows_without_an_upstream_gradient_and_unused_results():
     from trainscale_b200.rl import token_log_probs
     z = torch.randn(6, 300, device=DEV, requires_grad=True)
@@ -494,6 +573,12 @@ def test_clip_lists_that_go_tensor_by_tensor():
     assert float(_clip([torch.ones(4, device=DEV, dtype=torch.float64)], 1.0)) == pytest.approx(2.0)
     assert float(_clip([torch.ones(8, device=DEV)], 1.0, 3.0)) == pytest.approx(2.0, rel=1e-6)
     assert _clip([torch.ones(8, device=DEV, dtype=torch.bfloat16)], 1.0, math.inf).dtype == torch.bfloat16
+    from trainscale_b200.ops.optim import GradList
+    assert GradList.of([torch.ones(4, 4, device=DEV).to_sparse()], 2.0) is None
+    assert GradList.of([torch.ones(4, 4, device=DEV).to_sparse_csr()], 2.0) is None
+    assert GradList.of([torch.ones(4), torch.ones(4, device=DEV)], 2.0) is None
+    assert GradList.of([torch.ones(4, device=DEV), torch.ones(4)], 2.0) is None
+    assert GradList.of([torch.zeros(0, device=DEV)], 2.0) is None
 
 
 def test_clip_of_extreme_gradients():

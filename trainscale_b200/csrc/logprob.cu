@@ -157,28 +157,34 @@ struct LogitRows {
   }
 };
 
-// tanh(z / c) out of E = e^(-2 |z| / c) <= 1, so that the slope 1 - tanh^2 = 4 E / (1 + E)^2 keeps its bits where tanh is close to one;
-// off by 2^-22 of one.
+// tanh(x), x = z / c, out of E = e^(-2 |x|) <= 1, so that the slope 1 - tanh^2 = 4 E / (1 + E)^2 keeps its bits where tanh is close to
+// one; below 0.15, where 1 - E would lose them, a power series (x^9 is the first term left out: 6e-9).  Off by 2^-21 of its value.
+__device__ __forceinline__ float tanh_series(float x) {
+  const float q = x * x;
+  return x * fmaf(q, fmaf(q, fmaf(q, -17.f / 315.f, 2.f / 15.f), -1.f / 3.f), 1.f);
+}
 template <bool CAP>
 __device__ __forceinline__ float capped(float z, float inv_cap, float* slope = nullptr) {
   if (!CAP) return z;
-  const float e = fast_ex2(fabsf(z) * (-2.f * LOG2E * inv_cap)), r = fast_rcp(1.f + e);
+  const float x = z * inv_cap, e = fast_ex2(fabsf(x) * (-2.f * LOG2E)), r = fast_rcp(1.f + e);
   if (slope) *slope = 4.f * e * r * r;
-  return copysignf((1.f - e) * r, z);
+  return fabsf(x) < 0.15f ? tanh_series(x) : copysignf((1.f - e) * r, x);
 }
-// Two at once, 1 / (1 + E) by Newton's iteration from a parabola through it at E = 0, 1/2 and 1 (off by 0.009, then by 1e-4 and 1e-8):
+// Two at once, 1 / (1 + E) by Newton's iteration from a parabola through it at E = 0, 1/2 and 1 (off by 0.016, then by 3e-4 and 7e-8):
 // two calls of the special-function unit for an element instead of three, which is what bounds the forward pass.
 template <bool CAP>
-__device__ __forceinline__ Pair capped2(float x, float y, float inv_cap) {
-  if (!CAP) return Pair(x, y);
-  const float f = -2.f * LOG2E * inv_cap;
-  const Pair e(fast_ex2(fabsf(x) * f), fast_ex2(fabsf(y) * f)), one(1.f, 1.f), two(2.f, 2.f), minus(-1.f, -1.f);
-  const Pair d = (e + one) * minus;
+__device__ __forceinline__ Pair capped2(float z, float w, float inv_cap) {
+  if (!CAP) return Pair(z, w);
+  const Pair v = Pair(z, w) * Pair(inv_cap, inv_cap), q = v * v, one(1.f, 1.f), two(2.f, 2.f), minus(-1.f, -1.f);
+  const float2 x = v.get();
+  const float2 series = (v * fma2(q, fma2(q, fma2(q, Pair(-17.f / 315.f, -17.f / 315.f), Pair(2.f / 15.f, 2.f / 15.f)),
+                                          Pair(-1.f / 3.f, -1.f / 3.f)), one)).get();
+  const Pair e(fast_ex2(fabsf(x.x) * (-2.f * LOG2E)), fast_ex2(fabsf(x.y) * (-2.f * LOG2E))), d = (e + one) * minus;
   Pair r = fma2(e, fma2(e, Pair(1.f / 3.f, 1.f / 3.f), Pair(-5.f / 6.f, -5.f / 6.f)), one);
   r = r * fma2(d, r, two);
   r = r * fma2(d, r, two);
   const float2 t = (fma2(e, minus, one) * r).get();
-  return Pair(copysignf(t.x, x), copysignf(t.y, y));
+  return Pair(fabsf(x.x) < 0.15f ? series.x : copysignf(t.x, x.x), fabsf(x.y) < 0.15f ? series.y : copysignf(t.y, x.y));
 }
 
 struct Softmax {
@@ -215,10 +221,11 @@ __device__ __forceinline__ void add_value(Softmax& acc, float z, float k2, float
   if (ENT) acc.u += t * e;
 }
 
-// Adds N 16-byte vectors to a thread's (m, S, U).  An entropy's 0 * -inf (logits of -inf) shows as NaN; it is then summed again with
+// Adds the first `n` of N 16-byte vectors to a thread's (m, S, U); the others hold values of -inf, which count for nothing unless a cap
+// makes them finite.  An entropy's 0 * -inf (logits of -inf) shows as NaN; it is then summed again with
 // exponents that are bounded below.
 template <typename T, bool CAP, bool ENT, int N>
-__device__ __forceinline__ void add_vectors(Softmax& acc, const uint4* r, float k2, float inv_cap) {
+__device__ __forceinline__ void add_vectors(Softmax& acc, const uint4* r, int n, float k2, float inv_cap) {
   using W = Vec<T>;
   const float top = max_nan(acc.m, capped<CAP>(W::largest(r, N), inv_cap));
   acc.raise<ENT>(top, k2);
@@ -227,6 +234,7 @@ __device__ __forceinline__ void add_vectors(Softmax& acc, const uint4* r, float 
   Pair s(0.f, 0.f), u(0.f, 0.f);
 #pragma unroll
   for (int j = 0; j < N; ++j) {
+    if (CAP && j >= n) break;
     float f[W::N];
     W::unpack(r[j], f);
 #pragma unroll
@@ -247,6 +255,7 @@ __device__ __forceinline__ void add_vectors(Softmax& acc, const uint4* r, float 
     extra = 0.f;
 #pragma unroll
     for (int j = 0; j < N; ++j) {
+      if (CAP && j >= n) break;
       float f[W::N];
       W::unpack(r[j], f);
 #pragma unroll 1
@@ -328,7 +337,7 @@ __global__ void __launch_bounds__(LP_THREADS) logprob_row_kernel(const T* __rest
     uint4 v[LP_FLIGHT];
 #pragma unroll
     for (int j = 0; j < LP_FLIGHT; ++j) v[j] = i + j * LP_THREADS < end ? load_once(body + i + j * LP_THREADS) : Vec<T>::nothing();
-    add_vectors<T, CAP, ENT, LP_FLIGHT>(acc, v, a.k2, a.inv_cap);
+    add_vectors<T, CAP, ENT, LP_FLIGHT>(acc, v, (end - i + LP_THREADS - 1) / LP_THREADS, a.k2, a.inv_cap);
   }
   if (rank == 0 && static_cast<int>(threadIdx.x) < row.extra())
     add_value<CAP, ENT>(acc, Vec<T>::value(row.z[row.lone(threadIdx.x)]), a.k2, a.inv_cap);
@@ -381,13 +390,13 @@ __global__ void __launch_bounds__(LP_PART_THREADS) logprob_part_kernel(const T* 
       if (i + 2 * step <= end)
 #pragma unroll
         for (int j = 0; j < LP_PART_FLIGHT; ++j) next[j] = load_once(body + i + step + j * 32);
-      add_vectors<T, CAP, ENT, LP_PART_FLIGHT>(acc, v, a.k2, a.inv_cap);
+      add_vectors<T, CAP, ENT, LP_PART_FLIGHT>(acc, v, LP_PART_FLIGHT, a.k2, a.inv_cap);
     }
   }
   if (i < end) {
 #pragma unroll
     for (int j = 0; j < LP_PART_FLIGHT; ++j) v[j] = i + lane + j * 32 < end ? load_once(body + i + j * 32) : Vec<T>::nothing();
-    add_vectors<T, CAP, ENT, LP_PART_FLIGHT>(acc, v, a.k2, a.inv_cap);
+    add_vectors<T, CAP, ENT, LP_PART_FLIGHT>(acc, v, (end - i - lane + 31) / 32, a.k2, a.inv_cap);
   }
   if (parts == 1 && lane < row.extra()) add_value<CAP, ENT>(acc, Vec<T>::value(row.z[row.lone(lane)]), a.k2, a.inv_cap);
   join_warp<ENT>(acc, a.k2);
@@ -426,8 +435,10 @@ __global__ void __launch_bounds__(LP_BACK_THREADS) logprob_bwd_kernel(const T* _
                                                                  const float* __restrict__ grad_entropy, T* __restrict__ grad,
                                                                  LogitRows a, int parts) {
   using W = Vec<T>;
-  const long long row = blockIdx.x / parts;
-  const int part = static_cast<int>(blockIdx.x - row * parts);
+  // (last rows first: the forward pass has left them in the L2)
+  const unsigned unit = gridDim.x - 1 - blockIdx.x;
+  const long long row = unit / parts;
+  const int part = static_cast<int>(unit - row * parts);
   const long long label = labels[row];
   const T* z = logits + a.offset(row);
   T* d = grad + row * a.V;

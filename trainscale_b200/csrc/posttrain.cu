@@ -586,7 +586,7 @@ extern "C" long long ts_policy_workspace(long long rows, long long T) {
 
 extern "C" int ts_policy_loss(const PolicyCall* c, void* stream) {
   const long long n = c->rows * c->T;
-  if (c->rows <= 0 || c->T <= 0 || c->rows > 0x7fffffffll / POLICY_SPLIT || c->T > 0x7fffffffll || c->reduction < 0 || c->reduction > 2 ||
+  if (c->rows <= 0 || c->T <= 0 || c->rows > 0x7fffffffll / POLICY_SPLIT || c->T > 0x3fffffffll || c->reduction < 0 || c->reduction > 2 ||
       c->mask_kind < 0 || c->mask_kind > 5 || c->dtype < 0 || c->dtype > 2)
     return -1;
   cudaStream_t st = static_cast<cudaStream_t>(stream);

@@ -25,7 +25,7 @@ def on_this_gpu(*tensors) -> bool:
 
 
 def native(logits: torch.Tensor, labels: torch.Tensor) -> bool:
-    return logits.dtype in _DTYPES and on_this_gpu(logits, labels) and logits.numel() > 0
+    return logits.dtype in _DTYPES and on_this_gpu(logits, labels) and logits.numel() > 0 and logits.shape[-1] < 1 << 31
 
 
 def plain(logits, labels, factor: float, cap: float, ignore_index: int | None, entropy: bool):
@@ -143,6 +143,7 @@ def token_log_probs(logits: torch.Tensor, labels: torch.Tensor, factor: float = 
         return plain(logits, labels, factor, cap, ignore_index, entropy)
     labels = labels.to(torch.int64).contiguous()
     if torch.is_grad_enabled() and logits.requires_grad:
+        labels = labels.clone() if labels.is_inference() else labels      # (such tensors cannot be kept for a backward pass)
         return _TokenLogProbs.apply(logits, labels, factor, cap, ignore_index, entropy)
     logp, H, _ = _forward(logits, labels, factor, cap, ignore_index, entropy, False)
     return (logp, H) if entropy else logp

@@ -99,7 +99,7 @@ def scale_cast_(dst: torch.Tensor, src: torch.Tensor, mul: float = 1.0, accumula
 # The global norm of a list of gradients, and their clipping (library "gradnorm")
 # ---------------------------------------------------------------------------------------------------------------
 _GRAD_TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
-_DTYPE, _LAYOUT = operator.attrgetter("dtype"), operator.attrgetter("layout")
+_DTYPE = operator.attrgetter("dtype")
 _NORMS = {2.0: 0, 1.0: 1, float("inf"): 2}
 
 
@@ -129,13 +129,14 @@ class GradList:
             return None
         if not grads[0].is_cuda or set(map(torch.Tensor.get_device, grads)) != {torch._C._cuda_getDevice()}:
             return None
-        codes = list(map(_GRAD_TYPES.get, map(_DTYPE, grads)))
-        if None in codes or set(map(_LAYOUT, grads)) != {torch.strided}:
+        try:
+            codes = bytes(map(_GRAD_TYPES.__getitem__, map(_DTYPE, grads)))
+            if not all(map(torch.Tensor.is_contiguous, grads)):
+                if not all(g.is_contiguous() or (g.dim() == 2 and g.t().is_contiguous()) for g in grads):
+                    return None
+            listed = GradList(grads, codes)
+        except (KeyError, RuntimeError):                    # another type; a layout that has no single block of memory
             return None
-        if not all(map(torch.Tensor.is_contiguous, grads)):
-            if not all(g.is_contiguous() or (g.dim() == 2 and g.t().is_contiguous()) for g in grads):
-                return None
-        listed = GradList(grads, bytes(codes))
         return listed if any(listed.size) else None
 
     def norm(self, norm_type) -> torch.Tensor | None:

@@ -58,8 +58,12 @@ def _place(x: torch.Tensor | None) -> tuple[int, int]:
 
 def _one_type(first, *more):
     """Rows that are dense within themselves, all in the first one's type, or all in fp32 where they differ."""
-    same = all(t is None or t.dtype == first.dtype for t in more)
-    return [t if t is None else _rows_of(t if same else t.float()) for t in (first, *more)]
+    out = [first, *more]
+    for t in more:
+        if t is not None and t.dtype != first.dtype:
+            out = [u if u is None else u.float() for u in out]
+            break
+    return [t if t is None else _rows_of(t) for t in out]
 
 
 def _mask_of(mask: torch.Tensor) -> torch.Tensor:
@@ -68,6 +72,10 @@ def _mask_of(mask: torch.Tensor) -> torch.Tensor:
 
 def _empty(like: torch.Tensor, *shape: int) -> torch.Tensor:
     return torch.empty(shape, dtype=torch.float32, device=like.device)
+
+
+def _changed(tensors) -> tuple:
+    return tuple([None if t is None or t.is_inference() else t._version for t in tensors])
 
 
 class _Loss(torch.autograd.Function):
@@ -80,8 +88,9 @@ class _Loss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logp, op, *constants):
         loss, rest, ctx.grad = op(logp, *constants, grad=True)
-        ctx.save_for_backward(logp, *constants)
-        ctx.op, ctx.captured = op, torch.cuda.is_current_stream_capturing()
+        ctx.save_for_backward(logp)
+        ctx.op, ctx.constants, ctx.versions = op, constants, _changed(constants)
+        ctx.captured = torch.cuda.is_current_stream_capturing()
         if rest is not None:
             ctx.mark_non_differentiable(rest)
         ctx.set_materialize_grads(False)
@@ -89,20 +98,24 @@ class _Loss(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, g, _):
-        logp, *constants = ctx.saved_tensors          # (refuses a freed graph, and inputs that were changed since)
+        (logp,), constants = ctx.saved_tensors, ctx.constants       # (refuses a freed graph, and log-probabilities changed since)
         none = (None,) * (1 + len(constants))
         if g is None:
             return None, *none
-        if torch.is_grad_enabled():                   # this gradient will be differentiated itself
-            return torch.autograd.grad(ctx.op.plain(logp, *constants)[0], logp, g, create_graph=True)[0], *none
+        again = torch.is_grad_enabled()               # this gradient will be differentiated itself
         grad, ctx.grad = ctx.grad, None
+        if grad is None or again or ctx.captured != torch.cuda.is_current_stream_capturing() or grad.dtype != torch.float32:
+            if _changed(constants) != ctx.versions:
+                raise RuntimeError("an input of a policy or preference loss was changed in place before its gradient was computed")
+        if again:
+            return torch.autograd.grad(ctx.op.plain(logp, *constants)[0], logp, g, create_graph=True)[0], *none
         if ctx.captured != torch.cuda.is_current_stream_capturing():
             grad = None
         if grad is not None and grad.dtype == torch.float32:
             _lib.check(_library().ts_scale_by(grad.data_ptr(), g.data_ptr(), grad.numel(), _lib.stream_ptr()), "ts_scale_by")
         else:
             grad = ctx.op(logp, *constants, grad=True if grad is None else grad, factor=g)[2]
-        return grad.to(logp.dtype), *none
+        return grad if grad.dtype == logp.dtype else grad.to(logp.dtype), *none
 
 
 def native(logp, *others) -> bool:

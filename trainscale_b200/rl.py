@@ -41,8 +41,11 @@ def token_log_probs(logits: torch.Tensor, labels: torch.Tensor, *, temperature: 
     for name, value, least in (("temperature", temperature, None), ("logit_softcapping", logit_softcapping, 0), ("logit_scale", logit_scale, 0)):
         if not math.isfinite(value) or (value <= 0 if least is None else value < least):
             raise ValueError(f"{name} is {value}: it must be finite and {'positive' if least is None else 'not negative'}")
-    return lp_ops.token_log_probs(logits, labels, (logit_scale or 1.0) / temperature, float(logit_softcapping), ignore_index,
-                                  return_entropy)
+    factor = (logit_scale or 1.0) / temperature
+    if not 1e-30 < factor < 1e30 or not factor * (logit_softcapping or 1.0) < 1e30:
+        raise ValueError(f"a logit scale of {logit_scale}, a cap of {logit_softcapping} and a temperature of {temperature} leave the range "
+                         "of fp32")
+    return lp_ops.token_log_probs(logits, labels, factor, float(logit_softcapping), ignore_index, return_entropy)
 
 
 @reference_kwargs(input_ids="index")
@@ -161,17 +164,18 @@ def clipped_policy_loss(logp: torch.Tensor, old_logp: torch.Tensor, advantages: 
     "constant" (sum over B * max_len; max_len is T by default); a mask that leaves nothing counts as one token.
     `old_logp`, `advantages` and `ref_logp` are constants.  `return_stats`: (loss, `PolicyStats`), on the device.
     On the GPU the loss and the gradient of fp32, bf16 or fp16 log-probabilities come out of one pass, summed in fp64."""
-    if logp.dim() != 2:
-        raise ValueError(f"log-probabilities are [sequences, tokens], not {tuple(logp.shape)}")
+    shape = logp.shape
+    if len(shape) != 2:
+        raise ValueError(f"log-probabilities are [sequences, tokens], not {tuple(shape)}")
+    if old_logp.shape != shape or mask.shape != shape or (ref_logp is not None and ref_logp.shape != shape):
+        raise ValueError(f"old_logp {tuple(old_logp.shape)}, mask {tuple(mask.shape)} and ref_logp "
+                         f"{None if ref_logp is None else tuple(ref_logp.shape)} have the shape of the log-probabilities, {tuple(shape)}")
+    if advantages.shape != shape[:1] and advantages.shape != shape:
+        raise ValueError(f"advantages of shape {tuple(advantages.shape)} for log-probabilities of shape {tuple(shape)}")
     if reduction not in policy_ops.REDUCTIONS:
         raise ValueError(f"unknown reduction {reduction!r}; one of {sorted(policy_ops.REDUCTIONS)}")
-    for name, t in (("old_logp", old_logp), ("mask", mask), ("ref_logp", ref_logp)):
-        if t is not None and t.shape != logp.shape:
-            raise ValueError(f"{name} of shape {tuple(t.shape)} for log-probabilities of shape {tuple(logp.shape)}")
-    if advantages.shape not in (logp.shape, logp.shape[:1]):
-        raise ValueError(f"advantages of shape {tuple(advantages.shape)} for log-probabilities of shape {tuple(logp.shape)}")
     high = clip if clip_high is None else clip_high
-    if not (math.isfinite(clip) and math.isfinite(high) and clip >= 0 and high >= 0):
+    if not (0 <= clip < math.inf and 0 <= high < math.inf):
         raise ValueError(f"clip ranges are finite and not negative, not {clip} and {high}")
     if not math.isfinite(beta):
         raise ValueError(f"beta is {beta}")
@@ -179,8 +183,7 @@ def clipped_policy_loss(logp: torch.Tensor, old_logp: torch.Tensor, advantages: 
         raise ValueError("a KL term needs ref_logp")
     if max_len is not None and max_len <= 0:
         raise ValueError(f"max_len is {max_len}")
-    loss, stats = policy_ops.policy_loss(logp, old_logp, advantages, mask, ref_logp, float(clip), float(high), float(beta), reduction,
-                                         max_len, return_stats)
+    loss, stats = policy_ops.policy_loss(logp, old_logp, advantages, mask, ref_logp, clip, high, beta, reduction, max_len, return_stats)
     return (loss, PolicyStats(*stats.unbind())) if return_stats else loss
 
 
