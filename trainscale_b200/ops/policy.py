@@ -43,17 +43,21 @@ def _library():
     return lib
 
 
+def _stream() -> int:
+    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
+
+
 def _address(t: torch.Tensor | None) -> int:
     return 0 if t is None else t.data_ptr()
-
-
-def _rows_of(x: torch.Tensor) -> torch.Tensor:
-    return x if x.stride(1) == 1 or x.shape[1] == 1 else x.contiguous()
 
 
 def _place(x: torch.Tensor | None) -> tuple[int, int]:
     """Address and elements between rows."""
     return (0, 0) if x is None else (x.data_ptr(), x.stride(0))
+
+
+def _rows_of(x: torch.Tensor) -> torch.Tensor:
+    return x if x.stride(1) == 1 or x.shape[1] == 1 else x.contiguous()
 
 
 def _one_type(first, *more):
@@ -70,8 +74,8 @@ def _mask_of(mask: torch.Tensor) -> torch.Tensor:
     return _rows_of(mask if mask.dtype in _MASKS else mask.float())
 
 
-def _empty(like: torch.Tensor, *shape: int) -> torch.Tensor:
-    return torch.empty(shape, dtype=torch.float32, device=like.device)
+def _gradient(p: torch.Tensor) -> torch.Tensor:
+    return torch.empty_like(p, memory_format=torch.contiguous_format)
 
 
 def _changed(tensors) -> tuple:
@@ -90,7 +94,7 @@ class _Loss(torch.autograd.Function):
         loss, rest, ctx.grad = op(logp, *constants, grad=True)
         ctx.save_for_backward(logp)
         ctx.op, ctx.constants, ctx.versions = op, constants, _changed(constants)
-        ctx.captured = torch.cuda.is_current_stream_capturing()
+        ctx.captured = torch._C._cuda_isCurrentStreamCapturing()
         if rest is not None:
             ctx.mark_non_differentiable(rest)
         ctx.set_materialize_grads(False)
@@ -104,18 +108,17 @@ class _Loss(torch.autograd.Function):
             return None, *none
         again = torch.is_grad_enabled()               # this gradient will be differentiated itself
         grad, ctx.grad = ctx.grad, None
-        if grad is None or again or ctx.captured != torch.cuda.is_current_stream_capturing() or grad.dtype != torch.float32:
+        if ctx.captured != torch._C._cuda_isCurrentStreamCapturing():
+            grad = None
+        if grad is not None and grad.dtype is torch.float32 and not again:
+            _lib.check(_library().ts_scale_by(grad.data_ptr(), g.data_ptr(), grad.numel(), _stream()), "ts_scale_by")
+        else:
             if _changed(constants) != ctx.versions:
                 raise RuntimeError("an input of a policy or preference loss was changed in place before its gradient was computed")
-        if again:
-            return torch.autograd.grad(ctx.op.plain(logp, *constants)[0], logp, g, create_graph=True)[0], *none
-        if ctx.captured != torch.cuda.is_current_stream_capturing():
-            grad = None
-        if grad is not None and grad.dtype == torch.float32:
-            _lib.check(_library().ts_scale_by(grad.data_ptr(), g.data_ptr(), grad.numel(), _lib.stream_ptr()), "ts_scale_by")
-        else:
+            if again:
+                return torch.autograd.grad(ctx.op.plain(logp, *constants)[0], logp, g, create_graph=True)[0], *none
             grad = ctx.op(logp, *constants, grad=True if grad is None else grad, factor=g)[2]
-        return grad if grad.dtype == logp.dtype else grad.to(logp.dtype), *none
+        return grad if grad.dtype is logp.dtype else grad.to(logp.dtype), *none
 
 
 def native(logp, *others) -> bool:
@@ -148,19 +151,22 @@ class PolicyLoss:
         p, old, ref = _one_type(logp, old, ref)
         mask, advantages = _mask_of(mask), advantages.float().contiguous()
         B, T = p.shape
-        lib = _library()
-        loss = _empty(p) if factor is None else None
-        stats = _empty(p, 3) if factor is None and self.stats else None
-        out = torch.empty(p.shape, dtype=p.dtype, device=p.device) if grad is True else grad
+        lib, low, high = _library(), self.low, self.high
+        loss = stats = work = None
+        if factor is None:
+            loss = p.new_empty((), dtype=torch.float32)
+            if self.stats:
+                stats = p.new_empty(3, dtype=torch.float32)
+        out = _gradient(p) if grad is True else grad
         need = lib.ts_policy_workspace(B, T)
-        work = torch.empty(need, dtype=torch.float64, device=p.device) if need else None
-        low, high = self.low, self.high
+        if need:
+            work = p.new_empty(need, dtype=torch.float64)
         call = _POLICY_CALL.pack(
             _DTYPES[p.dtype], *_place(p), *_place(old), *_place(ref), advantages.data_ptr(), advantages.dim() == 2, *_place(mask),
             _MASKS[mask.dtype], B, T, math.log1p(-low) if low < 1 else -math.inf, math.log1p(high), 1 - low, 1 + high, self.beta,
             REDUCTIONS[self.reduction], 1.0 / (B * (self.length or T)), _address(out), _address(loss), _address(stats), _address(factor),
             grad is True, _address(work))
-        _lib.check(lib.ts_policy_loss(call, _lib.stream_ptr()), "ts_policy_loss")
+        _lib.check(lib.ts_policy_loss(call, _stream()), "ts_policy_loss")
         return loss, stats, out
 
     def plain(self, logp, old_logp, advantages, mask, ref_logp):
@@ -208,14 +214,16 @@ class PairLoss:
         p, ref = _one_type(logp, ref)
         mask = _mask_of(mask)
         R, T = p.shape
-        loss, rewards = (_empty(p), _empty(p, R)) if factor is None else (None, None)
-        out = torch.empty(p.shape, dtype=p.dtype, device=p.device) if grad is True else grad
-        work = torch.empty(R // 2, dtype=torch.float64, device=p.device)
+        loss = rewards = None
+        if factor is None:
+            loss, rewards = p.new_empty((), dtype=torch.float32), p.new_empty(R, dtype=torch.float32)
+        out = _gradient(p) if grad is True else grad
+        work = p.new_empty(R // 2, dtype=torch.float64)
         call = _PAIRS_CALL.pack(
             _DTYPES[p.dtype], *_place(p), *_place(ref), *_place(mask), _MASKS[mask.dtype], R // 2, T, self.beta, self.gamma,
             self.smoothing, self.nll, KINDS[self.kind], self.normalized, _address(out), _address(loss), _address(rewards),
             _address(factor), grad is True, work.data_ptr())
-        _lib.check(_library().ts_preference_loss(call, _lib.stream_ptr()), "ts_preference_loss")
+        _lib.check(_library().ts_preference_loss(call, _stream()), "ts_preference_loss")
         return loss, rewards, out
 
     def plain(self, logp, ref_logp, mask):
