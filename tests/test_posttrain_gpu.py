@@ -231,6 +231,33 @@ def test_rows_without_an_upstream_gradient_and_unused_results():
     (logp.sum() + H.sum()).backward()
 
 
+@pytest.mark.parametrize("T,V,chunk", [(37, 1000, 16), (700, 4003, 4096), (1, 129, 4)])
+def test_log_probs_of_the_fused_head(T, V, chunk):
+    """The chunked head on the same kernels, the gradient written over the logits; labels outside the vocabulary are ignored there."""
+    from trainscale_b200.ops.cross_entropy import fused_linear_token_logprobs
+    h = (torch.randn(T, 128, device=DEV, generator=_gen(1))).bfloat16().requires_grad_()
+    w = (torch.randn(V, 128, device=DEV, generator=_gen(2)) * 0.3).bfloat16().requires_grad_()
+    y = torch.randint(0, V, (T,), device=DEV, generator=_gen(3))
+    if T > 3:
+        y[0], y[1], y[2] = -100, V, -1
+    g = torch.randn(T, device=DEV, generator=_gen(4))
+    logp = fused_linear_token_logprobs(h, w, y, chunk_tokens=chunk)
+    dh, dw = torch.autograd.grad(logp, (h, w), g)
+    a, b = h.detach().double().requires_grad_(), w.detach().double().requires_grad_()
+    z = a @ b.t()
+    z = z + (z.bfloat16().double() - z).detach()            # logits are held in bf16
+    used = (y >= 0) & (y < V)
+    want = torch.log_softmax(z, -1).gather(1, y.where(used, 0).unsqueeze(1)).squeeze(1).where(used, 0.0)
+    # (a logit that lies on a border of bf16 may fall to either side: 2^-8 of its size)
+    _near(logp, want, 2.0 ** -8 * z.detach().abs().amax(1) * 2)
+    ea, eb = torch.autograd.grad(want, (a, b), g.double())
+    for d, e in ((dh, ea), (dw, eb)):
+        assert float((d.double() - e).norm()) <= 2.0 ** -6 * float(e.norm())
+    assert torch.equal(logp[~used], torch.zeros_like(logp[~used])) and (dh[~used] == 0).all()
+    with torch.no_grad():
+        assert torch.equal(logp, fused_linear_token_logprobs(h, w, y, chunk_tokens=chunk))
+
+
 def test_selective_log_softmax_keeps_its_results():
     from trainscale_b200.rl import selective_log_softmax
     y = torch.randint(0, 999, (4, 5), device=DEV)

@@ -774,33 +774,6 @@ __global__ void __launch_bounds__(CE_THREADS) cross_entropy_kernel(__nv_bfloat16
   }
 }
 
-// Per-row log-probability of the label token (DPO / SimPO / GRPO): logp[row] = z[label] - lse, 0 if ignored.
-__global__ void __launch_bounds__(CE_THREADS) token_logprob_kernel(const __nv_bfloat16* __restrict__ logits,
-                                                                   const long long* __restrict__ labels,
-                                                                   float* __restrict__ logp, float* __restrict__ lse_out,
-                                                                   int V, long long ld, int ignore_index) {
-  __shared__ float scratch[32];
-  const size_t row = blockIdx.x;
-  const __nv_bfloat16* z = logits + row * ld;
-  const long long label = labels[row];
-  const bool ignored = (label == ignore_index) || label < 0 || label >= V;
-  float m = -INFINITY, s = 0.f;
-  for (int i = threadIdx.x; i < V; i += CE_THREADS) {
-    const float f = __bfloat162float(z[i]);
-    const float lm = fmaxf(m, f);
-    s = s * __expf(m - lm) + __expf(f - lm);
-    m = lm;
-  }
-  const float gm = block_max(m, scratch);
-  s = (m == -INFINITY) ? 0.f : s * __expf(m - gm);
-  s = block_sum(s, scratch);
-  if (threadIdx.x == 0) {
-    const float lse = gm + __logf(s);
-    if (lse_out) lse_out[row] = lse;
-    logp[row] = ignored ? 0.f : __bfloat162float(z[label]) - lse;
-  }
-}
-
 // ---------------------------------------------------------------------------------------------------
 // Optimizer kernels
 // ---------------------------------------------------------------------------------------------------
@@ -1254,14 +1227,6 @@ extern "C" int ts_cross_entropy(void* logits, const long long* labels, float* lo
   cross_entropy_kernel<<<(unsigned)rows, CE_THREADS, 0, ST(stream)>>>((bf16*)logits, labels, loss, lse, V, ld,
                                                                       ignore_index, label_smoothing, logit_scale,
                                                                       softcap, gscale_ptr, gscale_mul, row_gscale, write_grad);
-  return (int)cudaGetLastError();
-}
-
-extern "C" int ts_token_logprob(const void* logits, const long long* labels, float* logp, float* lse, long long rows,
-                                int V, long long ld, int ignore_index, void* stream) {
-  if (rows <= 0) return 0;
-  token_logprob_kernel<<<(unsigned)rows, CE_THREADS, 0, ST(stream)>>>((const bf16*)logits, labels, logp, lse, V, ld,
-                                                                      ignore_index);
   return (int)cudaGetLastError();
 }
 

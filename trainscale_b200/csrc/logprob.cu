@@ -152,6 +152,8 @@ struct LogitRows {
   float k, k2;                       // f or f c: y = k v; the same times log2(e)
   float inv_cap;                     // 1 / c, or 0
   long long ignore;
+  int lenient;                       // labels outside the vocabulary count as ignored
+  __device__ __forceinline__ bool ignored(long long label) const { return label == ignore || (lenient && (label < 0 || label >= V)); }
   __device__ __forceinline__ long long offset(long long r) const {
     return (r / inner) * stride_outer + (r % inner) * stride_inner;
   }
@@ -324,7 +326,7 @@ __global__ void __launch_bounds__(LP_THREADS) logprob_row_kernel(const T* __rest
   __shared__ Softmax by_warp[LP_THREADS / 32];
   __shared__ Softmax by_block[LP_SPLIT];
   const long long r = blockIdx.x / parts, label = labels[r];
-  if (label == a.ignore) {
+  if (a.ignored(label)) {
     if (threadIdx.x == 0 && rank == 0) ignored_row(r, logp, entropy, kept);
     return;                                   // (the whole cluster: it has one row)
   }
@@ -371,7 +373,7 @@ __global__ void __launch_bounds__(LP_PART_THREADS) logprob_part_kernel(const T* 
   const int lane = threadIdx.x & 31;
   if (r >= a.rows) return;
   const long long label = labels[r];
-  if (label == a.ignore) {
+  if (a.ignored(label)) {
     if (parts == 1 && lane == 0) ignored_row(r, logp, entropy, kept);
     return;
   }
@@ -416,7 +418,7 @@ __global__ void __launch_bounds__(LP_PART_THREADS) logprob_join_kernel(const T* 
   if (r >= a.rows) return;
   grid_wait();
   const long long label = labels[r];
-  if (label == a.ignore) {
+  if (a.ignored(label)) {
     if (lane == 0) ignored_row(r, logp, entropy, kept);
     return;
   }
@@ -428,12 +430,13 @@ __global__ void __launch_bounds__(LP_PART_THREADS) logprob_join_kernel(const T* 
   if (lane == 0) row_results<T, CAP>(acc, row, r, label, a, logp, entropy, kept);
 }
 
-// A block takes LP_BACK_THREADS * LP_BACK_FLIGHT vectors of one row.
+// A block takes LP_BACK_THREADS * LP_BACK_FLIGHT vectors of one row.  A thread has read what it writes over before it writes,
+// and no other thread reads that: the gradient may replace the logits.
 template <typename T, bool CAP, bool ENT>
-__global__ void __launch_bounds__(LP_BACK_THREADS) logprob_bwd_kernel(const T* __restrict__ logits, const long long* __restrict__ labels,
+__global__ void __launch_bounds__(LP_BACK_THREADS) logprob_bwd_kernel(const T* logits, const long long* __restrict__ labels,
                                                                  const float4* __restrict__ kept, const float* __restrict__ grad_logp,
-                                                                 const float* __restrict__ grad_entropy, T* __restrict__ grad,
-                                                                 LogitRows a, int parts) {
+                                                                 const float* __restrict__ grad_entropy, T* grad,
+                                                                 LogitRows a, long long grad_stride, int parts) {
   using W = Vec<T>;
   // (last rows first: the forward pass has left them in the L2)
   const unsigned unit = gridDim.x - 1 - blockIdx.x;
@@ -441,9 +444,9 @@ __global__ void __launch_bounds__(LP_BACK_THREADS) logprob_bwd_kernel(const T* _
   const int part = static_cast<int>(unit - row * parts);
   const long long label = labels[row];
   const T* z = logits + a.offset(row);
-  T* d = grad + row * a.V;
+  T* d = grad + row * grad_stride;
   const float g = grad_logp ? grad_logp[row] : 0.f, h = ENT ? grad_entropy[row] : 0.f;
-  const bool still = label == a.ignore || (g == 0.f && h == 0.f);       // nothing flows back: the row is not read
+  const bool still = a.ignored(label) || (g == 0.f && h == 0.f);       // nothing flows back: the row is not read
   // vectors start on the boundaries of the gradient; logits that lie otherwise are read one by one
   const int head = min(a.V, static_cast<int>((16 - (reinterpret_cast<uintptr_t>(d) & 15)) & 15) / static_cast<int>(sizeof(T)));
   const int vectors = (a.V - head) / W::N, tail = head + vectors * W::N;
@@ -533,9 +536,9 @@ static int by_type(int dtype, bool cap, bool entropy, F&& launch) {
 }
 
 static LogitRows logit_rows(long long rows, long long inner, long long stride_outer, long long stride_inner, int V, float factor,
-                            float cap, long long ignore) {
+                            float cap, long long ignore, int lenient) {
   const float k = factor * (cap > 0.f ? cap : 1.f);
-  return {rows, inner, stride_outer, stride_inner, V, k, k * LOG2E, cap > 0.f ? 1.f / cap : 0.f, ignore};
+  return {rows, inner, stride_outer, stride_inner, V, k, k * LOG2E, cap > 0.f ? 1.f / cap : 0.f, ignore, lenient};
 }
 
 }  // namespace ts
@@ -558,14 +561,14 @@ extern "C" long long ts_logprob_workspace(long long rows, int V, int dtype) {
 }
 
 // dtype: 0 bf16, 1 fp16, 2 fp32.  kept: (m, S, H, unused) of every row, for the backward pass; H counts only with an entropy.
-// entropy and kept may be null.
+// entropy and kept may be null.  lenient: labels outside the vocabulary count as ignored; otherwise they give NaN.
 extern "C" int ts_logprob_fwd(const void* logits, int dtype, const long long* labels, float* logp, float* entropy, float4* kept,
                               void* workspace, long long rows, long long inner, long long stride_outer, long long stride_inner, int V,
-                              float factor, float cap, long long ignore, void* stream) {
+                              float factor, float cap, long long ignore, int lenient, void* stream) {
   constexpr int warps = LP_PART_THREADS / 32;
   const int units = row_parts(rows, V, dtype);
   if (rows <= 0 || inner <= 0 || V <= 0 || rows > 0x7fffffffll / (units > LP_SPLIT ? units : LP_SPLIT)) return -1;
-  const LogitRows a = logit_rows(rows, inner, stride_outer, stride_inner, V, factor, cap, ignore);
+  const LogitRows a = logit_rows(rows, inner, stride_outer, stride_inner, V, factor, cap, ignore, lenient);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   return by_type(dtype, cap > 0.f, entropy != nullptr, [&](auto* t, auto c, auto e) {
     using T = std::remove_pointer_t<decltype(t)>;
@@ -587,19 +590,20 @@ extern "C" int ts_logprob_fwd(const void* logits, int dtype, const long long* la
   });
 }
 
-// grad is dense [rows][V]; grad_logp / grad_entropy may be null (zero).
+// Rows of grad are grad_stride elements apart; it may be the logits themselves, where their rows are.  grad_logp / grad_entropy may be
+// null (zero).
 extern "C" int ts_logprob_bwd(const void* logits, int dtype, const long long* labels, const float4* kept, const float* grad_logp,
-                              const float* grad_entropy, void* grad, long long rows, long long inner, long long stride_outer,
-                              long long stride_inner, int V, float factor, float cap, long long ignore, void* stream) {
+                              const float* grad_entropy, void* grad, long long grad_stride, long long rows, long long inner, long long stride_outer,
+                              long long stride_inner, int V, float factor, float cap, long long ignore, int lenient, void* stream) {
   const long long vectors = static_cast<long long>(V) * (dtype == 2 ? 4 : 2) / 16;
   const long long parts = vectors / (LP_BACK_THREADS * LP_BACK_FLIGHT) + 1;
-  if (rows <= 0 || inner <= 0 || V <= 0 || rows > 0x7fffffffll / parts || !kept) return -1;
-  const LogitRows a = logit_rows(rows, inner, stride_outer, stride_inner, V, factor, cap, ignore);
+  if (rows <= 0 || inner <= 0 || V <= 0 || rows > 0x7fffffffll / parts || !kept || grad_stride < V) return -1;
+  const LogitRows a = logit_rows(rows, inner, stride_outer, stride_inner, V, factor, cap, ignore, lenient);
   return by_type(dtype, cap > 0.f, grad_entropy != nullptr, [&](auto* t, auto c, auto e) {
     using T = std::remove_pointer_t<decltype(t)>;
     logprob_bwd_kernel<T, decltype(c)::value, decltype(e)::value>
         <<<static_cast<unsigned>(rows * parts), LP_BACK_THREADS, 0, static_cast<cudaStream_t>(stream)>>>(
-            static_cast<const T*>(logits), labels, kept, grad_logp, grad_entropy, static_cast<T*>(grad), a, static_cast<int>(parts));
+            static_cast<const T*>(logits), labels, kept, grad_logp, grad_entropy, static_cast<T*>(grad), a, grad_stride, static_cast<int>(parts));
     return static_cast<int>(cudaGetLastError());
   });
 }

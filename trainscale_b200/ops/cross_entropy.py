@@ -16,7 +16,7 @@ import ctypes
 import torch
 import torch.nn.functional as F
 
-from . import _lib
+from . import _lib, logprob
 from .gemm import matmul_nn, matmul_nt, matmul_tn
 
 DEFAULT_CHUNK_TOKENS = 4096
@@ -238,33 +238,31 @@ def linear_cross_entropy_reference(hidden, weight, labels, ignore_index=-100, la
 
 
 class _FusedLinearLogProb(torch.autograd.Function):
-    """Per-token log p(label) from hidden states; logits recomputed chunk by chunk in backward."""
+    """Per-token log p(label) from hidden states; logits recomputed chunk by chunk in backward, whose rows keep their softmax
+    statistics from the forward pass and are read once more, to be overwritten with their gradient."""
 
     @staticmethod
     def forward(ctx, hidden, weight, labels, ignore_index, chunk_tokens):
         T, H = hidden.shape
         V = weight.shape[0]
-        lib = _lib.load("elementwise")
         labels = labels.reshape(-1).to(torch.int64)
         chunk = min(chunk_tokens, T)
         buf = torch.empty(chunk, _pad_ld(V), dtype=torch.bfloat16, device=hidden.device)
         logp = torch.empty(T, dtype=torch.float32, device=hidden.device)
+        kept = torch.empty(T, 4, dtype=torch.float32, device=hidden.device) if any(ctx.needs_input_grad) else None
         for s in range(0, T, chunk):
             e = min(s + chunk, T)
             logits = buf[: e - s, :V]
             matmul_nt(hidden[s:e], weight, out=logits)
-            rc = lib.ts_token_logprob(_lib.ptr(logits), _lib.ptr(labels[s:e]), _lib.ptr(logp[s:e]), None,
-                                      ctypes.c_longlong(e - s), V, ctypes.c_longlong(logits.stride(0)), ignore_index,
-                                      _lib.stream_ptr())
-            _lib.check(rc, "ts_token_logprob")
-        ctx.save_for_backward(hidden, weight, labels)
+            logprob.rows_forward(logits, labels[s:e], logp[s:e], None if kept is None else kept[s:e], ignore_index)
+        ctx.save_for_backward(hidden, weight, labels, kept)
         ctx.ignore_index = ignore_index
         ctx.chunk = chunk
         return logp
 
     @staticmethod
     def backward(ctx, g):
-        hidden, weight, labels = ctx.saved_tensors
+        hidden, weight, labels, kept = ctx.saved_tensors
         T, H = hidden.shape
         V = weight.shape[0]
         dev = hidden.device
@@ -281,15 +279,12 @@ class _FusedLinearLogProb(torch.autograd.Function):
             else:
                 dw = torch.empty(V, H, dtype=torch.float32, device=dev)
         buf = torch.empty(ctx.chunk, _pad_ld(V), dtype=torch.bfloat16, device=dev)
-        scratch = torch.empty(ctx.chunk, dtype=torch.float32, device=dev)
-        neg_g = (-g.float()).contiguous()
+        g = g.float().contiguous()
         for s in range(0, T, ctx.chunk):
             e = min(s + ctx.chunk, T)
             logits = buf[: e - s, :V]
             matmul_nt(hidden[s:e], weight, out=logits)
-            # (softmax - onehot) * (-g)  ==  g * d logp / d logits
-            _ce_rows(logits, labels[s:e], scratch[: e - s], None, ctx.ignore_index, 0.0, 1.0, 0.0, None, 1.0,
-                     neg_g[s:e], True)
+            logprob.rows_backward_(logits, labels[s:e], kept[s:e], g[s:e], ctx.ignore_index)
             matmul_nn(logits, weight, out=dh[s:e])
             if need_dw:
                 matmul_tn(logits, hidden[s:e], out=dw, accumulate=(acc0 or s > 0))

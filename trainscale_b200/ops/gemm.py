@@ -31,7 +31,7 @@ def gemm_raw(a: torch.Tensor, b: torch.Tensor, out: torch.Tensor, M: int, N: int
 
 
 def _rows2d(t: torch.Tensor) -> torch.Tensor:
-    t = t.reshape(-1, t.shape[-1])
+    t = t if t.dim() == 2 else t.reshape(-1, t.shape[-1])       # (reshape would forget the pitch of a single row)
     if t.stride(-1) != 1 or (t.stride(0) * t.element_size()) % 16 != 0 or t.data_ptr() % 16 != 0:
         t = t.contiguous()
     return t

@@ -58,10 +58,10 @@ def _rows(logits: torch.Tensor):
     return logits, 1, 1, 0, 0
 
 
-def _tail(rows, V, factor, cap, ignore_index):
+def _tail(rows, V, factor, cap, ignore_index, lenient=False):
     n, inner, outer_stride, inner_stride = rows
     ignore = -(1 << 63) if ignore_index is None else ignore_index
-    return (n, inner, outer_stride, inner_stride, V, factor, cap, ignore, _lib.stream_ptr())
+    return (n, inner, outer_stride, inner_stride, V, factor, cap, ignore, lenient, _lib.stream_ptr())
 
 
 _fns: dict = {}
@@ -80,8 +80,8 @@ def _call(name: str, *args) -> None:
     if fn is None:
         from ctypes import c_float, c_int, c_longlong, c_void_p
         fn = getattr(_lib.load("logprob"), name)
-        shape = [c_longlong] * 4 + [c_int, c_float, c_float, c_longlong, c_void_p]
-        fn.argtypes = [c_void_p, c_int] + [c_void_p] * 5 + shape
+        shape = [c_longlong] * 4 + [c_int, c_float, c_float, c_longlong, c_int, c_void_p]
+        fn.argtypes = [c_void_p, c_int] + [c_void_p] * 5 + ([c_longlong] if name == "ts_logprob_bwd" else []) + shape
         _fns[name] = fn
     _lib.check(fn(*args), name)
 
@@ -97,6 +97,23 @@ def _forward(logits, labels, factor, cap, ignore_index, entropy: bool, keep: boo
     _call("ts_logprob_fwd", _lib.ptr(x), _DTYPES[x.dtype], _lib.ptr(labels), _lib.ptr(logp), _lib.ptr(H), _lib.ptr(kept),
           _lib.ptr(work), *_tail(rows, x.shape[-1], factor, cap, ignore_index))
     return logp, H, kept
+
+
+def rows_forward(logits: torch.Tensor, labels: torch.Tensor, logp: torch.Tensor, kept: torch.Tensor | None, ignore_index: int) -> None:
+    """logp [n] = log softmax(logits [n, V])[labels], kept [n, 4] for `rows_backward_`, of CUDA rows that are dense within themselves.
+    Labels outside the vocabulary count as ignored."""
+    n, V = logits.shape
+    need = _workspace()(n, V, _DTYPES[logits.dtype])
+    work = torch.empty(need, dtype=torch.uint8, device=logits.device) if need else None
+    _call("ts_logprob_fwd", _lib.ptr(logits), _DTYPES[logits.dtype], _lib.ptr(labels), _lib.ptr(logp), None, _lib.ptr(kept), _lib.ptr(work),
+          *_tail((n, n, 0, logits.stride(0)), V, 1.0, 0.0, ignore_index, True))
+
+
+def rows_backward_(logits: torch.Tensor, labels: torch.Tensor, kept: torch.Tensor, g: torch.Tensor, ignore_index: int) -> None:
+    """The logits become the gradient of (g * logp).sum()."""
+    n, V = logits.shape
+    _call("ts_logprob_bwd", _lib.ptr(logits), _DTYPES[logits.dtype], _lib.ptr(labels), _lib.ptr(kept), _lib.ptr(g), None, _lib.ptr(logits),
+          logits.stride(0), *_tail((n, n, 0, logits.stride(0)), V, 1.0, 0.0, ignore_index, True))
 
 
 class _TokenLogProbs(torch.autograd.Function):
@@ -124,7 +141,7 @@ class _TokenLogProbs(torch.autograd.Function):
         grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
         g, h = (None if d is None else d.float().contiguous() for d in (g, h))
         _call("ts_logprob_bwd", _lib.ptr(x), _DTYPES[x.dtype], _lib.ptr(labels), _lib.ptr(kept), _lib.ptr(g), _lib.ptr(h),
-              _lib.ptr(grad), *_tail(rows, x.shape[-1], factor, cap, ignore_index))
+              _lib.ptr(grad), x.shape[-1], *_tail(rows, x.shape[-1], factor, cap, ignore_index))
         return grad, *none
 
 
