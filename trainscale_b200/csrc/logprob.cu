@@ -138,10 +138,11 @@ struct Vec<__half> {
   }
 };
 
-// Logits are read once in each direction and are gone by then: they pass the L1 by.
+// Logits are read once in each direction and are gone by then: they pass the L1 by.  (Not by the read-only path: a gradient may take
+// their place.)
 __device__ __forceinline__ uint4 load_once(const uint4* p) {
   uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
   return v;
 }
 
@@ -330,6 +331,7 @@ __global__ void __launch_bounds__(LP_THREADS) logprob_row_kernel(const T* __rest
     if (threadIdx.x == 0 && rank == 0) ignored_row(r, logp, entropy, kept);
     return;                                   // (the whole cluster: it has one row)
   }
+  if (parts > 1) cluster.barrier_arrive();    // (no block writes to another's shared memory before that one has begun)
   const Row<T> row(logits + a.offset(r), a.V);
   const uint4* body = row.body();
   const int begin = static_cast<int>(static_cast<long long>(row.vectors) * rank / parts);
@@ -351,6 +353,7 @@ __global__ void __launch_bounds__(LP_THREADS) logprob_row_kernel(const T* __rest
     join_warp<ENT>(acc, a.k2);
   }
   if (parts > 1) {
+    cluster.barrier_wait();
     if (threadIdx.x == 0) *cluster.map_shared_rank(by_block + rank, 0) = acc;
     cluster.sync();
     if (rank != 0) return;

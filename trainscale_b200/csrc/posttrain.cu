@@ -302,12 +302,14 @@ __global__ void __launch_bounds__(PT_THREADS) policy_count_kernel(Policy a, floa
     if (threadIdx.x == 0) counts[blockIdx.x] = n[0];
     return;
   }
+  if (parts > 1) cluster.barrier_arrive();      // (no block writes to another's shared memory before that one has begun)
   const long long row = blockIdx.x / parts, part = (a.T / VEC + parts - 1) / parts * VEC;
   const long long begin = row * a.T + rank * part, end = rank == parts - 1 ? (row + 1) * a.T : min((row + 1) * a.T, begin + part);
   // (a row that starts between vectors is counted token by token)
   double n[1] = {(row * a.T | a.T) % VEC == 0 ? mask_run<VEC>(a, begin, end) : mask_run<1>(a, begin, end)};
   block_sums<1>(n, scratch);
   if (parts > 1) {
+    cluster.barrier_wait();
     if (threadIdx.x == 0) *cluster.map_shared_rank(by_block + rank, 0) = n[0];
     cluster.sync();
     if (rank != 0) return;
@@ -393,8 +395,13 @@ __global__ void __launch_bounds__(POLICY_ALONE_THREADS) policy_alone_kernel(Poli
 __global__ void __launch_bounds__(PT_THREADS) scale_kernel(float* __restrict__ grad, const float* __restrict__ factor, long long n) {
   const float f = *factor;
   if (f == 1.f) return;
-  for (long long i = blockIdx.x * static_cast<long long>(PT_THREADS) + threadIdx.x; i < n; i += gridDim.x * static_cast<long long>(PT_THREADS))
-    grad[i] *= f;
+  const long long step = gridDim.x * static_cast<long long>(PT_THREADS), first = blockIdx.x * static_cast<long long>(PT_THREADS) + threadIdx.x;
+  float4* fours = reinterpret_cast<float4*>(grad);
+  for (long long i = first; i < n / 4; i += step) {
+    const float4 v = fours[i];
+    fours[i] = make_float4(v.x * f, v.y * f, v.z * f, v.w * f);
+  }
+  if (first < n % 4) grad[n - 1 - first] *= f;
 }
 
 // ---------------------------------------------------------------------------------------------------
@@ -456,6 +463,7 @@ __global__ void __launch_bounds__(PT_THREADS) pair_kernel(Pairs a, T* __restrict
   cg::cluster_group cluster = cg::this_cluster();
   if (up.done()) return;
   const int parts = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
+  if (parts > 1) cluster.barrier_arrive();      // (no block writes to another's shared memory before that one has begun)
   const long long p = blockIdx.x / parts;
   const long long begin = a.T * rank / parts, end = a.T * (rank + 1) / parts;
   double sums[5] = {};                   // score and tokens of the chosen, of the rejected row; the chosen's own log-probability
@@ -480,6 +488,7 @@ __global__ void __launch_bounds__(PT_THREADS) pair_kernel(Pairs a, T* __restrict
   }
   block_sums<5>(sums, scratch);
   if (parts > 1) {
+    cluster.barrier_wait();
     if (static_cast<int>(threadIdx.x) < parts) {
       double* to = cluster.map_shared_rank(&by_block[rank][0], threadIdx.x);
 #pragma unroll
@@ -641,10 +650,10 @@ extern "C" int ts_policy_loss(const PolicyCall* c, void* stream) {
   });
 }
 
-// grad [n] *= *factor.
+// grad [n] *= *factor; grad starts on a 16-byte boundary.
 extern "C" int ts_scale_by(float* grad, const float* factor, long long n, void* stream) {
-  if (n <= 0) return -1;
-  const long long blocks = (n + PT_THREADS * 4 - 1) / (PT_THREADS * 4), most = sm_count() * 8ll;
+  if (n <= 0 || !on_boundary(grad, 16)) return -1;
+  const long long blocks = (n + PT_THREADS * 8 - 1) / (PT_THREADS * 8), most = sm_count() * 8ll;
   scale_kernel<<<static_cast<unsigned>(blocks < most ? blocks : most), PT_THREADS, 0, static_cast<cudaStream_t>(stream)>>>(grad, factor, n);
   return static_cast<int>(cudaGetLastError());
 }
