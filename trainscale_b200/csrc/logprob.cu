@@ -538,12 +538,6 @@ static int by_type(int dtype, bool cap, bool entropy, F&& launch) {
   }
 }
 
-static LogitRows logit_rows(long long rows, long long inner, long long stride_outer, long long stride_inner, int V, float factor,
-                            float cap, long long ignore, int lenient) {
-  const float k = factor * (cap > 0.f ? cap : 1.f);
-  return {rows, inner, stride_outer, stride_inner, V, k, k * LOG2E, cap > 0.f ? 1.f / cap : 0.f, ignore, lenient};
-}
-
 }  // namespace ts
 
 using namespace ts;
@@ -552,61 +546,82 @@ TS_DEFINE_ERROR_API(ts_logprob)
 
 // Parts of a row that warps of their own take; 0: a block or a cluster takes the row.  Rows have blocks of their own while those are
 // fewer than two to an SM.
-static int row_parts(long long rows, int V, int dtype) {
-  const long long vectors = static_cast<long long>(V) * (dtype == 2 ? 4 : 2) / 16;
+static int row_parts(long long rows, long long V, int dtype) {
+  const long long vectors = V * (dtype == 2 ? 4 : 2) / 16;
   return rows < 2 * sm_count() ? 0 : static_cast<int>((vectors + LP_PART - 1) / LP_PART) + (vectors == 0);
 }
 
 // Bytes of workspace that ts_logprob_fwd needs.
-extern "C" long long ts_logprob_workspace(long long rows, int V, int dtype) {
+extern "C" long long ts_logprob_workspace(long long rows, long long V, int dtype) {
   const int parts = row_parts(rows, V, dtype);
   return parts > 1 ? rows * parts * static_cast<long long>(sizeof(Softmax)) : 0;
 }
 
-// dtype: 0 bf16, 1 fp16, 2 fp32.  kept: (m, S, H, unused) of every row, for the backward pass; H counts only with an entropy.
-// entropy and kept may be null.  lenient: labels outside the vocabulary count as ignored; otherwise they give NaN.
-extern "C" int ts_logprob_fwd(const void* logits, int dtype, const long long* labels, float* logp, float* entropy, float4* kept,
-                              void* workspace, long long rows, long long inner, long long stride_outer, long long stride_inner, int V,
-                              float factor, float cap, long long ignore, int lenient, void* stream) {
+// The arguments of a call, eight bytes each (ops/logprob.py packs them).  dtype: 0 bf16, 1 fp16, 2 fp32.  lenient: labels outside the
+// vocabulary count as ignored; otherwise they give NaN.  kept: (m, S, H, unused) of every row, for the backward pass; H counts only with
+// an entropy.  Forward: logp and, where they are not null, entropy and kept are results.  Backward: logp and entropy are what flows into
+// them (null: zero), grad the result, its rows grad_stride elements apart; it may be the logits themselves, where their rows are.
+struct LogprobCall {
+  const void* logits;
+  long long dtype;
+  const long long* labels;
+  float *logp, *entropy;
+  float4* kept;
+  void *workspace, *grad;
+  long long grad_stride, rows, inner, stride_outer, stride_inner, V;
+  double factor, cap;
+  long long ignore, lenient;
+};
+
+static bool valid(const LogprobCall* c, long long units) {
+  return c->rows > 0 && c->inner > 0 && c->V > 0 && c->V <= 0x7fffffffll && c->rows <= 0x7fffffffll / units && c->dtype >= 0 && c->dtype <= 2;
+}
+static LogitRows logit_rows(const LogprobCall* c) {
+  const double k = c->factor * (c->cap > 0.0 ? c->cap : 1.0);
+  return {c->rows, c->inner, c->stride_outer, c->stride_inner, static_cast<int>(c->V), static_cast<float>(k),
+          static_cast<float>(k * 1.4426950408889634), c->cap > 0.0 ? static_cast<float>(1.0 / c->cap) : 0.f, c->ignore,
+          static_cast<int>(c->lenient)};
+}
+
+extern "C" int ts_logprob_fwd(const LogprobCall* c, void* stream) {
   constexpr int warps = LP_PART_THREADS / 32;
-  const int units = row_parts(rows, V, dtype);
-  if (rows <= 0 || inner <= 0 || V <= 0 || rows > 0x7fffffffll / (units > LP_SPLIT ? units : LP_SPLIT)) return -1;
-  const LogitRows a = logit_rows(rows, inner, stride_outer, stride_inner, V, factor, cap, ignore, lenient);
+  const int dtype = static_cast<int>(c->dtype), units = row_parts(c->rows, c->V, dtype);
+  if (!valid(c, units > LP_SPLIT ? units : LP_SPLIT)) return -1;
+  const LogitRows a = logit_rows(c);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return by_type(dtype, cap > 0.f, entropy != nullptr, [&](auto* t, auto c, auto e) {
+  return by_type(dtype, c->cap > 0.0, c->entropy != nullptr, [&](auto* t, auto cap, auto e) {
     using T = std::remove_pointer_t<decltype(t)>;
-    constexpr bool CAP = decltype(c)::value, ENT = decltype(e)::value;
-    const T* z = static_cast<const T*>(logits);
+    constexpr bool CAP = decltype(cap)::value, ENT = decltype(e)::value;
+    const T* z = static_cast<const T*>(c->logits);
     if (units) {
-      Softmax* partial = static_cast<Softmax*>(workspace);
-      logprob_part_kernel<T, CAP, ENT><<<static_cast<unsigned>((rows * units + warps - 1) / warps), LP_PART_THREADS, 0, st>>>(
-          z, labels, partial, logp, entropy, kept, a, units);
+      Softmax* partial = static_cast<Softmax*>(c->workspace);
+      logprob_part_kernel<T, CAP, ENT><<<static_cast<unsigned>((a.rows * units + warps - 1) / warps), LP_PART_THREADS, 0, st>>>(
+          z, c->labels, partial, c->logp, c->entropy, c->kept, a, units);
       if (units == 1) return static_cast<int>(cudaGetLastError());
-      return launch_chained(logprob_join_kernel<T, CAP, ENT>, dim3(static_cast<unsigned>((rows + warps - 1) / warps)), dim3(LP_PART_THREADS), 0,
-                            st, 1, true, z, labels, partial, logp, entropy, kept, a, units);
+      const int rc = static_cast<int>(cudaGetLastError());
+      if (rc) return rc;
+      return launch_chained(logprob_join_kernel<T, CAP, ENT>, dim3(static_cast<unsigned>((a.rows + warps - 1) / warps)), dim3(LP_PART_THREADS), 0,
+                            st, 1, true, z, c->labels, partial, c->logp, c->entropy, c->kept, a, units);
     }
     int parts = 1;                       // of a cluster, each with a vector or two for every thread
-    const long long vectors = static_cast<long long>(V) * static_cast<int>(sizeof(T)) / 16;
-    while (parts < LP_SPLIT && rows * parts < 2 * sm_count() && vectors / parts >= 2 * LP_THREADS) parts *= 2;
-    return launch_chained(logprob_row_kernel<T, CAP, ENT>, dim3(static_cast<unsigned>(rows * parts)), dim3(LP_THREADS), 0, st, parts, false,
-                          z, labels, logp, entropy, kept, a);
+    const long long vectors = c->V * static_cast<int>(sizeof(T)) / 16;
+    while (parts < LP_SPLIT && a.rows * parts < 2 * sm_count() && vectors / parts >= 2 * LP_THREADS) parts *= 2;
+    return launch_chained(logprob_row_kernel<T, CAP, ENT>, dim3(static_cast<unsigned>(a.rows * parts)), dim3(LP_THREADS), 0, st, parts, false,
+                          z, c->labels, c->logp, c->entropy, c->kept, a);
   });
 }
 
-// Rows of grad are grad_stride elements apart; it may be the logits themselves, where their rows are.  grad_logp / grad_entropy may be
-// null (zero).
-extern "C" int ts_logprob_bwd(const void* logits, int dtype, const long long* labels, const float4* kept, const float* grad_logp,
-                              const float* grad_entropy, void* grad, long long grad_stride, long long rows, long long inner, long long stride_outer,
-                              long long stride_inner, int V, float factor, float cap, long long ignore, int lenient, void* stream) {
-  const long long vectors = static_cast<long long>(V) * (dtype == 2 ? 4 : 2) / 16;
-  const long long parts = vectors / (LP_BACK_THREADS * LP_BACK_FLIGHT) + 1;
-  if (rows <= 0 || inner <= 0 || V <= 0 || rows > 0x7fffffffll / parts || !kept || grad_stride < V) return -1;
-  const LogitRows a = logit_rows(rows, inner, stride_outer, stride_inner, V, factor, cap, ignore, lenient);
-  return by_type(dtype, cap > 0.f, grad_entropy != nullptr, [&](auto* t, auto c, auto e) {
+extern "C" int ts_logprob_bwd(const LogprobCall* c, void* stream) {
+  const int dtype = static_cast<int>(c->dtype);
+  const long long vectors = c->V * (dtype == 2 ? 4 : 2) / 16, parts = vectors / (LP_BACK_THREADS * LP_BACK_FLIGHT) + 1;
+  if (!valid(c, parts) || !c->kept || c->grad_stride < c->V) return -1;
+  const LogitRows a = logit_rows(c);
+  return by_type(dtype, c->cap > 0.0, c->entropy != nullptr, [&](auto* t, auto cap, auto e) {
     using T = std::remove_pointer_t<decltype(t)>;
-    logprob_bwd_kernel<T, decltype(c)::value, decltype(e)::value>
-        <<<static_cast<unsigned>(rows * parts), LP_BACK_THREADS, 0, static_cast<cudaStream_t>(stream)>>>(
-            static_cast<const T*>(logits), labels, kept, grad_logp, grad_entropy, static_cast<T*>(grad), a, grad_stride, static_cast<int>(parts));
+    logprob_bwd_kernel<T, decltype(cap)::value, decltype(e)::value>
+        <<<static_cast<unsigned>(a.rows * parts), LP_BACK_THREADS, 0, static_cast<cudaStream_t>(stream)>>>(
+            static_cast<const T*>(c->logits), c->labels, c->kept, c->logp, c->entropy, static_cast<T*>(c->grad), a, c->grad_stride,
+            static_cast<int>(parts));
     return static_cast<int>(cudaGetLastError());
   });
 }

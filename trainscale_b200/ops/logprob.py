@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import functools
 import math
+import struct
 
 import torch
 
@@ -14,6 +15,8 @@ from . import _lib
 
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 _PLAIN = (torch.Tensor, torch.nn.Parameter)
+_CALL = struct.Struct("=14q2d2q")                # LogprobCall of csrc/logprob.cu
+_NEVER = -(1 << 63)                              # no label: nothing is ignored
 
 
 def on_this_gpu(*tensors) -> bool:
@@ -45,104 +48,95 @@ def plain(logits, labels, factor: float, cap: float, ignore_index: int | None, e
 
 
 def _rows(logits: torch.Tensor):
-    """The logits as (tensor, rows, rows of an inner run, its strides): up to three dimensions are read where they lie."""
+    """The logits as a tensor, and (rows, rows of an inner run, its strides): up to three dimensions are read where they lie."""
     if logits.stride(-1) != 1 and logits.shape[-1] > 1:
         logits = logits.contiguous()
     if logits.dim() > 3:
         logits = logits.reshape(-1, *logits.shape[-2:])
     shape, stride = logits.shape, logits.stride()
-    if logits.dim() == 3:
-        return logits, shape[0] * shape[1], shape[1], stride[0], stride[1]
-    if logits.dim() == 2:
-        return logits, shape[0], shape[0], 0, stride[0]
-    return logits, 1, 1, 0, 0
-
-
-def _tail(rows, V, factor, cap, ignore_index, lenient=False):
-    n, inner, outer_stride, inner_stride = rows
-    ignore = -(1 << 63) if ignore_index is None else ignore_index
-    return (n, inner, outer_stride, inner_stride, V, factor, cap, ignore, lenient, _lib.stream_ptr())
-
-
-_fns: dict = {}
+    if len(shape) == 3:
+        return logits, (shape[0] * shape[1], shape[1], stride[0], stride[1])
+    return logits, (shape[0], shape[0], 0, stride[0]) if len(shape) == 2 else (1, 1, 0, 0)
 
 
 @functools.lru_cache(maxsize=None)
-def _workspace():
-    from ctypes import c_int, c_longlong
-    fn = _lib.load("logprob").ts_logprob_workspace
-    fn.argtypes, fn.restype = [c_longlong, c_int, c_int], c_longlong
-    return fn
+def _library():
+    from ctypes import c_char_p, c_int, c_longlong, c_void_p
+    lib = _lib.load("logprob")
+    lib.ts_logprob_fwd.argtypes = lib.ts_logprob_bwd.argtypes = [c_char_p, c_void_p]
+    lib.ts_logprob_workspace.argtypes, lib.ts_logprob_workspace.restype = [c_longlong, c_longlong, c_int], c_longlong
+    return lib
 
 
-def _call(name: str, *args) -> None:
-    fn = _fns.get(name)
-    if fn is None:
-        from ctypes import c_float, c_int, c_longlong, c_void_p
-        fn = getattr(_lib.load("logprob"), name)
-        shape = [c_longlong] * 4 + [c_int, c_float, c_float, c_longlong, c_int, c_void_p]
-        fn.argtypes = [c_void_p, c_int] + [c_void_p] * 5 + ([c_longlong] if name == "ts_logprob_bwd" else []) + shape
-        _fns[name] = fn
-    _lib.check(fn(*args), name)
+def _address(t: torch.Tensor | None) -> int:
+    return 0 if t is None else t.data_ptr()
 
 
-def _forward(logits, labels, factor, cap, ignore_index, entropy: bool, keep: bool):
-    x, *rows = _rows(logits)
-    f32 = dict(dtype=torch.float32, device=logits.device)
-    logp = torch.empty(labels.shape, **f32)
-    H = torch.empty(labels.shape, **f32) if entropy else None
-    kept = torch.empty(labels.numel(), 4, **f32) if keep else None
-    need = _workspace()(labels.numel(), x.shape[-1], _DTYPES[x.dtype])
-    work = torch.empty(need, dtype=torch.uint8, device=logits.device) if need else None
-    _call("ts_logprob_fwd", _lib.ptr(x), _DTYPES[x.dtype], _lib.ptr(labels), _lib.ptr(logp), _lib.ptr(H), _lib.ptr(kept),
-          _lib.ptr(work), *_tail(rows, x.shape[-1], factor, cap, ignore_index))
+def _stream() -> int:
+    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
+
+
+def _run_forward(x, rows, labels, logp, H, kept, factor=1.0, cap=0.0, ignore_index=None, lenient=False) -> None:
+    lib, V, kind = _library(), x.shape[-1], _DTYPES[x.dtype]
+    need = lib.ts_logprob_workspace(rows[0], V, kind)
+    work = x.new_empty(need, dtype=torch.uint8) if need else None
+    call = _CALL.pack(x.data_ptr(), kind, labels.data_ptr(), logp.data_ptr(), _address(H), _address(kept), _address(work), 0, 0, *rows, V,
+                      factor, cap, _NEVER if ignore_index is None else ignore_index, lenient)
+    _lib.check(lib.ts_logprob_fwd(call, _stream()), "ts_logprob_fwd")
+
+
+def _run_backward(x, rows, labels, kept, g, h, grad, pitch, factor=1.0, cap=0.0, ignore_index=None, lenient=False) -> None:
+    call = _CALL.pack(x.data_ptr(), _DTYPES[x.dtype], labels.data_ptr(), _address(g), _address(h), kept.data_ptr(), 0, grad.data_ptr(), pitch,
+                      *rows, x.shape[-1], factor, cap, _NEVER if ignore_index is None else ignore_index, lenient)
+    _lib.check(_library().ts_logprob_bwd(call, _stream()), "ts_logprob_bwd")
+
+
+def _forward(logits, labels, how, entropy: bool, keep: bool):
+    x, rows = _rows(logits)
+    logp = x.new_empty(labels.shape, dtype=torch.float32)
+    H = x.new_empty(labels.shape, dtype=torch.float32) if entropy else None
+    kept = x.new_empty((rows[0], 4), dtype=torch.float32) if keep else None
+    _run_forward(x, rows, labels, logp, H, kept, *how)
     return logp, H, kept
 
 
 def rows_forward(logits: torch.Tensor, labels: torch.Tensor, logp: torch.Tensor, kept: torch.Tensor | None, ignore_index: int) -> None:
-    """logp [n] = log softmax(logits [n, V])[labels], kept [n, 4] for `rows_backward_`, of CUDA rows that are dense within themselves.
-    Labels outside the vocabulary count as ignored."""
-    n, V = logits.shape
-    need = _workspace()(n, V, _DTYPES[logits.dtype])
-    work = torch.empty(need, dtype=torch.uint8, device=logits.device) if need else None
-    _call("ts_logprob_fwd", _lib.ptr(logits), _DTYPES[logits.dtype], _lib.ptr(labels), _lib.ptr(logp), None, _lib.ptr(kept), _lib.ptr(work),
-          *_tail((n, n, 0, logits.stride(0)), V, 1.0, 0.0, ignore_index, True))
+    """logp [n] = log softmax(logits [n, V])[labels], kept [n, 4] for `rows_backward_`, of rows on the current GPU that are dense within
+    themselves.  Labels outside the vocabulary count as ignored."""
+    n, pitch = logits.shape[0], logits.stride(0)
+    _run_forward(logits, (n, n, 0, pitch), labels, logp, None, kept, ignore_index=ignore_index, lenient=True)
 
 
 def rows_backward_(logits: torch.Tensor, labels: torch.Tensor, kept: torch.Tensor, g: torch.Tensor, ignore_index: int) -> None:
     """The logits become the gradient of (g * logp).sum()."""
-    n, V = logits.shape
-    _call("ts_logprob_bwd", _lib.ptr(logits), _DTYPES[logits.dtype], _lib.ptr(labels), _lib.ptr(kept), _lib.ptr(g), None, _lib.ptr(logits),
-          logits.stride(0), *_tail((n, n, 0, logits.stride(0)), V, 1.0, 0.0, ignore_index, True))
+    n, pitch = logits.shape[0], logits.stride(0)
+    _run_backward(logits, (n, n, 0, pitch), labels, kept, g, None, logits, pitch, ignore_index=ignore_index, lenient=True)
 
 
 class _TokenLogProbs(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logits, labels, factor, cap, ignore_index, entropy):
-        logp, H, kept = _forward(logits, labels, factor, cap, ignore_index, entropy, True)
+    def forward(ctx, logits, labels, how, entropy):
+        logp, H, kept = _forward(logits, labels, how, entropy, True)
         ctx.save_for_backward(logits, labels, kept)
-        ctx.how = (factor, cap, ignore_index, entropy)
+        ctx.how, ctx.entropy = how, entropy
         ctx.set_materialize_grads(False)
         return (logp, H) if entropy else logp
 
     @staticmethod
     def backward(ctx, g, h=None):
         logits, labels, kept = ctx.saved_tensors
-        factor, cap, ignore_index, entropy = ctx.how
-        none = (None,) * 5
         if g is None and h is None:
-            return None, *none
+            return None, None, None, None
         if torch.is_grad_enabled():                      # this gradient will be differentiated itself
-            out = plain(logits, labels, factor, cap, ignore_index, entropy)
-            pairs = [(o, d) for o, d in zip(out if entropy else (out,), (g, h)) if d is not None]
+            out = plain(logits, labels, *ctx.how, ctx.entropy)
+            pairs = [(o, d) for o, d in zip(out if ctx.entropy else (out,), (g, h)) if d is not None]
             (grad,) = torch.autograd.grad([o for o, _ in pairs], logits, [d for _, d in pairs], create_graph=True)
-            return grad, *none
-        x, *rows = _rows(logits)
-        grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+            return grad, None, None, None
+        x, rows = _rows(logits)
+        grad = torch.empty_like(logits, memory_format=torch.contiguous_format)
         g, h = (None if d is None else d.float().contiguous() for d in (g, h))
-        _call("ts_logprob_bwd", _lib.ptr(x), _DTYPES[x.dtype], _lib.ptr(labels), _lib.ptr(kept), _lib.ptr(g), _lib.ptr(h),
-              _lib.ptr(grad), x.shape[-1], *_tail(rows, x.shape[-1], factor, cap, ignore_index))
-        return grad, *none
+        _run_backward(x, rows, labels, kept, g, h, grad, x.shape[-1], *ctx.how)
+        return grad, None, None, None
 
 
 def token_log_probs(logits: torch.Tensor, labels: torch.Tensor, factor: float = 1.0, cap: float = 0.0,
@@ -150,17 +144,18 @@ def token_log_probs(logits: torch.Tensor, labels: torch.Tensor, factor: float = 
     """log softmax(factor * cap tanh(logits / cap))[labels] in fp32 (and the distribution's entropy)."""
     if labels.shape != logits.shape[:-1]:
         raise ValueError(f"labels of shape {tuple(labels.shape)} for logits of shape {tuple(logits.shape)}")
-    if labels.dtype not in (torch.int64, torch.int32):
+    if labels.dtype != torch.int64 and labels.dtype != torch.int32:
         raise TypeError(f"labels are int64 or int32, not {labels.dtype}")
     if not logits.is_floating_point():
         raise TypeError(f"logits are floating point, not {logits.dtype}")
     if logits.shape[-1] == 0:
         raise ValueError("logits of an empty vocabulary")
+    how = (factor, cap, ignore_index)
     if not native(logits, labels):
-        return plain(logits, labels, factor, cap, ignore_index, entropy)
+        return plain(logits, labels, *how, entropy)
     labels = labels.to(torch.int64).contiguous()
     if torch.is_grad_enabled() and logits.requires_grad:
         labels = labels.clone() if labels.is_inference() else labels      # (such tensors cannot be kept for a backward pass)
-        return _TokenLogProbs.apply(logits, labels, factor, cap, ignore_index, entropy)
-    logp, H, _ = _forward(logits, labels, factor, cap, ignore_index, entropy, False)
+        return _TokenLogProbs.apply(logits, labels, how, entropy)
+    logp, H, _ = _forward(logits, labels, how, entropy, False)
     return (logp, H) if entropy else logp

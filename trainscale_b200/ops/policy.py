@@ -16,7 +16,7 @@ import torch
 import torch.nn.functional as F
 
 from . import _lib
-from .logprob import _DTYPES, on_this_gpu
+from .logprob import _DTYPES, _address, _stream, on_this_gpu
 
 _MASKS = {torch.bool: 0, torch.uint8: 0, torch.int32: 1, torch.int64: 2, torch.float32: 3, torch.bfloat16: 4, torch.float16: 5}
 REDUCTIONS = {"sequence": 0, "token": 1, "constant": 2}
@@ -41,14 +41,6 @@ def _library():
     lib.ts_scale_by.argtypes = [c_void_p, c_void_p, c_longlong, c_void_p]
     lib.ts_policy_workspace.argtypes, lib.ts_policy_workspace.restype = [c_longlong, c_longlong], c_longlong
     return lib
-
-
-def _stream() -> int:
-    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
-
-
-def _address(t: torch.Tensor | None) -> int:
-    return 0 if t is None else t.data_ptr()
 
 
 def _place(x: torch.Tensor | None) -> tuple[int, int]:

@@ -38,9 +38,9 @@ def token_log_probs(logits: torch.Tensor, labels: torch.Tensor, *, temperature: 
     `return_entropy`: (log-probabilities, entropy of each row's distribution), both differentiable; logits of -inf are tokens of no
     probability.  bf16, fp16 and fp32 logits with rows that are dense within themselves (also of a slice such as `logits[:, :-1]`) are
     read in place, once in each direction."""
-    for name, value, least in (("temperature", temperature, None), ("logit_softcapping", logit_softcapping, 0), ("logit_scale", logit_scale, 0)):
-        if not math.isfinite(value) or (value <= 0 if least is None else value < least):
-            raise ValueError(f"{name} is {value}: it must be finite and {'positive' if least is None else 'not negative'}")
+    if not (0 < temperature < math.inf and 0 <= logit_softcapping < math.inf and 0 <= logit_scale < math.inf):
+        raise ValueError(f"the temperature is finite and positive, the cap and the scale are finite and not negative; not {temperature}, "
+                         f"{logit_softcapping} and {logit_scale}")
     factor = (logit_scale or 1.0) / temperature
     if not 1e-30 < factor < 1e30 or not factor * (logit_softcapping or 1.0) < 1e30:
         raise ValueError(f"a logit scale of {logit_scale}, a cap of {logit_softcapping} and a temperature of {temperature} leave the range "
