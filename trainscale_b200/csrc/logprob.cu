@@ -544,11 +544,13 @@ using namespace ts;
 
 TS_DEFINE_ERROR_API(ts_logprob)
 
-// Parts of a row that warps of their own take; 0: a block or a cluster takes the row.  Rows have blocks of their own while those are
-// fewer than two to an SM.
+// Parts of a row that warps of their own take; 0: a block or a cluster takes the row.  A row of one part always has a warp (4 rows of
+// 2000: 2.9 us, in blocks 3.2; 1200: 3.8 and 11).  Longer rows have blocks of their own while those are fewer than four to an SM, and need no
+// second launch (rows of 128256 in blocks and in warps: 9.3 and 9.6 us for 100, 21.6 and 23.9 for 400, 33.3 and 31.7 for 600; of 32000: 7.5
+// and 8.1, 8.4 and 9.7, 11.8 and 12.1).
 static int row_parts(long long rows, long long V, int dtype) {
-  const long long vectors = V * (dtype == 2 ? 4 : 2) / 16;
-  return rows < 2 * sm_count() ? 0 : static_cast<int>((vectors + LP_PART - 1) / LP_PART) + (vectors == 0);
+  const long long vectors = V * (dtype == 2 ? 4 : 2) / 16, parts = (vectors + LP_PART - 1) / LP_PART;
+  return parts <= 1 ? 1 : rows < 4 * sm_count() ? 0 : static_cast<int>(parts);
 }
 
 // Bytes of workspace that ts_logprob_fwd needs.

@@ -68,20 +68,77 @@ __device__ __forceinline__ void put(T* p, const float* f) {
   *reinterpret_cast<Few<T, N>*>(p) = v;
 }
 
+// N values of a mask.  They are loaded as they are and become fp32 when they are needed: a branch on their type that waited for them
+// would keep the other loads waiting too.
+template <int N>
+struct MaskBits {
+  uint32_t w[2 * N];
+};
+template <typename T, int N>
+__device__ __forceinline__ float mask_value(const MaskBits<N>& b, int i) {
+  if constexpr (sizeof(T) == 8) return static_cast<float>(static_cast<long long>(b.w[2 * i] | static_cast<unsigned long long>(b.w[2 * i + 1]) << 32));
+  constexpr int in_word = 4 / sizeof(T) > 0 ? 4 / sizeof(T) : 1;
+  const uint32_t word = b.w[i / in_word] >> (i % in_word * (32 / in_word));
+  if constexpr (sizeof(T) == 1) return static_cast<float>(word & 0xff);
+  if constexpr (sizeof(T) == 2) {
+    const unsigned short half = static_cast<unsigned short>(word);
+    return pt_f32(*reinterpret_cast<const T*>(&half));
+  }
+  return pt_f32(*reinterpret_cast<const T*>(&word));
+}
+
 struct Mask {
   const void* p;
   long long stride;                      // elements between rows
   int kind;                              // 0 bool / uint8, 1 int32, 2 int64, 3 fp32, 4 bf16, 5 fp16
+  int shift;                             // log2 of their bytes
+  template <int N>
+  __device__ __forceinline__ void load(long long i, MaskBits<N>& b) const {
+    const char* at = static_cast<const char*>(p) + (i << shift);
+    if (shift == 0) {
+      if (N == 4) b.w[0] = *reinterpret_cast<const uint32_t*>(at);
+      else b.w[0] = *reinterpret_cast<const unsigned char*>(at);
+    } else if (shift == 1) {
+      if (N == 4) {
+        const uint2 v = *reinterpret_cast<const uint2*>(at);
+        b.w[0] = v.x, b.w[1] = v.y;
+      } else {
+        b.w[0] = *reinterpret_cast<const unsigned short*>(at);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        if (j == 1 && shift == 2) break;
+        if (N == 4) {
+          const uint4 v = *reinterpret_cast<const uint4*>(at + 16 * j);
+          b.w[4 * j] = v.x, b.w[4 * j + 1] = v.y, b.w[4 * j + 2] = v.z, b.w[4 * j + 3] = v.w;
+        } else {
+          b.w[j] = *reinterpret_cast<const uint32_t*>(at + 4 * j);
+        }
+      }
+    }
+  }
+  template <typename T, int N>
+  static __device__ __forceinline__ void values_of(const MaskBits<N>& b, float* f) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) f[i] = mask_value<T, N>(b, i);
+  }
+  template <int N>
+  __device__ __forceinline__ void values(const MaskBits<N>& b, float* f) const {
+    switch (kind) {
+      case 0: return values_of<unsigned char, N>(b, f);
+      case 1: return values_of<int, N>(b, f);
+      case 2: return values_of<long long, N>(b, f);
+      case 3: return values_of<float, N>(b, f);
+      case 4: return values_of<__nv_bfloat16, N>(b, f);
+      default: return values_of<__half, N>(b, f);
+    }
+  }
   template <int N>
   __device__ __forceinline__ void get(long long i, float* f) const {
-    switch (kind) {
-      case 0: return fetch<N>(static_cast<const unsigned char*>(p) + i, f);
-      case 1: return fetch<N>(static_cast<const int*>(p) + i, f);
-      case 2: return fetch<N>(static_cast<const long long*>(p) + i, f);
-      case 3: return fetch<N>(static_cast<const float*>(p) + i, f);
-      case 4: return fetch<N>(static_cast<const __nv_bfloat16*>(p) + i, f);
-      default: return fetch<N>(static_cast<const __half*>(p) + i, f);
-    }
+    MaskBits<N> b;
+    load<N>(i, b);
+    values<N>(b, f);
   }
 };
 
@@ -106,12 +163,14 @@ __device__ __forceinline__ void block_sums(double* v, double (*scratch)[N]) {
 #pragma unroll
     for (int k = 0; k < N; ++k) scratch[warp][k] = v[k];
   __syncthreads();
-#pragma unroll
-  for (int k = 0; k < N; ++k) {
-    v[k] = lane < nwarp ? scratch[lane][k] : 0.0;
-#pragma unroll
-    for (int o = 16; o; o >>= 1) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
+  if (threadIdx.x < N) {
+    double t = scratch[0][threadIdx.x];
+    for (int w = 1; w < nwarp; ++w) t += scratch[w][threadIdx.x];
+    scratch[0][threadIdx.x] = t;
   }
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < N; ++k) v[k] = scratch[0][k];
 }
 
 // ---------------------------------------------------------------------------------------------------
@@ -160,10 +219,10 @@ struct Place {
   __device__ __forceinline__ long long in(long long stride) const { return row * stride + t; }
 };
 
-// Sum of the mask over tokens [begin, end), which lie in one row or are `flat`.
-template <int VEC>
-__device__ __forceinline__ double mask_run(const Policy& a, long long begin, long long end) {
-  const long long at = a.flat ? 0 : begin / a.T * (a.mask.stride - a.T), width = static_cast<long long>(blockDim.x) * VEC;
+// Sum of the mask's values [begin, end) by a block, four vectors of a thread in flight.
+template <typename M, int VEC>
+__device__ __forceinline__ double sum_values(const M* p, long long begin, long long end) {
+  const long long width = static_cast<long long>(blockDim.x) * VEC;
   double n = 0.0;
   for (long long i = begin + static_cast<long long>(threadIdx.x) * VEC; i < end; i += 4 * width) {
     float m[4][VEC], s = 0.f;
@@ -171,7 +230,7 @@ __device__ __forceinline__ double mask_run(const Policy& a, long long begin, lon
     for (int j = 0; j < 4; ++j) {
 #pragma unroll
       for (int e = 0; e < VEC; ++e) m[j][e] = 0.f;
-      if (i + j * width < end) a.mask.get<VEC>(at + i + j * width, m[j]);
+      if (i + j * width < end) fetch<VEC>(p + i + j * width, m[j]);
     }
 #pragma unroll
     for (int j = 0; j < 4; ++j)
@@ -180,6 +239,20 @@ __device__ __forceinline__ double mask_run(const Policy& a, long long begin, lon
     n += s;
   }
   return n;
+}
+
+// Sum of the mask over tokens [begin, end), which lie in one row or are `flat`.
+template <int VEC>
+__device__ __forceinline__ double mask_run(const Policy& a, long long begin, long long end) {
+  const long long at = a.flat ? 0 : begin / a.T * (a.mask.stride - a.T);
+  switch (a.mask.kind) {
+    case 0: return sum_values<unsigned char, VEC>(static_cast<const unsigned char*>(a.mask.p) + at, begin, end);
+    case 1: return sum_values<int, VEC>(static_cast<const int*>(a.mask.p) + at, begin, end);
+    case 2: return sum_values<long long, VEC>(static_cast<const long long*>(a.mask.p) + at, begin, end);
+    case 3: return sum_values<float, VEC>(static_cast<const float*>(a.mask.p) + at, begin, end);
+    case 4: return sum_values<__nv_bfloat16, VEC>(static_cast<const __nv_bfloat16*>(a.mask.p) + at, begin, end);
+    default: return sum_values<__half, VEC>(static_cast<const __half*>(a.mask.p) + at, begin, end);
+  }
 }
 
 // The same of any tokens.
@@ -207,18 +280,19 @@ __device__ __forceinline__ void policy_tokens(const Policy& a, long long begin, 
   const bool whole = a.T % VEC == 0;     // a thread's tokens are in one row
   long long next = begin + static_cast<long long>(threadIdx.x) * VEC;
   Place ahead(next, width, a.T);
-  float coming[VEC];                     // the mask is read a step ahead: tokens that it leaves out are not read at all
-  if (next < end) a.mask.get<VEC>(FLAT ? next : ahead.in(a.mask.stride), coming);
+  MaskBits<VEC> coming;                  // the mask is read a step ahead: tokens that it leaves out are not read at all
+  if (next < end) a.mask.load<VEC>(FLAT ? next : ahead.in(a.mask.stride), coming);
   while (next < end) {
     const long long i = next;
     const Place at = ahead;
     float logp[VEC], old[VEC], ref[VEC], m[VEC], adv[VEC], w[VEC], slope[VEC], part[POLICY_SUMS] = {};
     bool any = false;
+    a.mask.values<VEC>(coming, m);
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) m[e] = coming[e], any |= m[e] != 0.f, slope[e] = 0.f;
+    for (int e = 0; e < VEC; ++e) any |= m[e] != 0.f, slope[e] = 0.f;
     next += width;
     ahead.step();
-    if (next < end) a.mask.get<VEC>(FLAT ? next : ahead.in(a.mask.stride), coming);
+    if (next < end) a.mask.load<VEC>(FLAT ? next : ahead.in(a.mask.stride), coming);
     if (!any) {
       if (grad) put<VEC>(grad + i, slope);
       continue;
@@ -366,16 +440,17 @@ __global__ void __launch_bounds__(POLICY_ALONE_THREADS) policy_alone_kernel(Poli
   if (up.done()) return;
   float uniform = static_cast<float>(a.constant);
   if (a.reduction == 0) {
-    const int lane = threadIdx.x & 31;
-    for (int r = threadIdx.x >> 5; r < a.rows; r += POLICY_ALONE_THREADS / 32) {
+    const int lanes = a.T >= 32 ? 32 : 1, lane = threadIdx.x % lanes;      // a warp counts a row, or a thread a short one
+    for (int r = threadIdx.x / lanes; r < a.rows; r += POLICY_ALONE_THREADS / lanes) {
       double n = 0.0;
-      for (long long t = lane; t < a.T; t += 32) {
+      for (long long t = lane; t < a.T; t += lanes) {
         float m;
         a.mask.get<1>(r * a.mask.stride + t, &m);
         n += m;
       }
+      if (lanes == 32)
 #pragma unroll
-      for (int o = 16; o; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
+        for (int o = 16; o; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
       if (lane == 0) weights[r] = static_cast<float>(1.0 / (fmax(n, 1.0) * static_cast<double>(a.rows)));
     }
     __syncthreads();
@@ -444,22 +519,19 @@ __device__ __forceinline__ double pair_loss(const Pairs& a, double x, double* sl
 // boundary and behind the last, VEC at a time between them.
 template <int VEC, typename F>
 __device__ __forceinline__ void over_row(long long begin, long long end, int phase, F&& f) {
-  if (VEC == 1) {
-    for (long long t = begin + threadIdx.x; t < end; t += PT_THREADS) f(t, std::integral_constant<int, 1>());
-    return;
-  }
   const long long first = min(end, begin + (VEC - (begin + phase) % VEC) % VEC), past = first + (end - first) / VEC * VEC;
   for (long long t = first + static_cast<long long>(threadIdx.x) * VEC; t < past; t += PT_THREADS * VEC) f(t, std::integral_constant<int, VEC>());
-  const long long lone = threadIdx.x < first - begin ? begin + threadIdx.x : past + (threadIdx.x - (first - begin));
-  if (lone < end && threadIdx.x < (first - begin) + (end - past)) f(lone, std::integral_constant<int, 1>());
+  const int before = static_cast<int>(first - begin), singles = before + static_cast<int>(end - past), i = threadIdx.x;
+  if (i < singles) f(i < before ? begin + i : past + (i - before), std::integral_constant<int, 1>());
 }
 
 // A block, or a cluster of them, per pair: scores, loss, rewards, and the gradient of both rows.
 template <typename T, int VEC>
-__global__ void __launch_bounds__(PT_THREADS) pair_kernel(Pairs a, T* __restrict__ grad, double* __restrict__ loss,
+__global__ void __launch_bounds__(PT_THREADS, 5) pair_kernel(Pairs a, T* __restrict__ grad, double* __restrict__ loss,
                                                           float* __restrict__ rewards, Upstream up) {
   __shared__ double scratch[32][5];
   __shared__ double by_block[PAIR_SPLIT][5];
+  __shared__ float weights[2];           // of the gradient's rows
   cg::cluster_group cluster = cg::this_cluster();
   if (up.done()) return;
   const int parts = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
@@ -473,14 +545,17 @@ __global__ void __launch_bounds__(PT_THREADS) pair_kernel(Pairs a, T* __restrict
     over_row<VEC>(begin, end, static_cast<int>(row * a.T % VEC), [&](long long t, auto n) {
       constexpr int N = decltype(n)::value;
       float m[N], v[N], r[N];
-      a.mask.get<N>(row * a.mask.stride + t, m);
+      MaskBits<N> bits;
+      a.mask.load<N>(row * a.mask.stride + t, bits);
       fetch<N>(static_cast<const T*>(a.logp) + row * a.s_logp + t, v);
       if (a.ref) fetch<N>(static_cast<const T*>(a.ref) + row * a.s_ref + t, r);
+      a.mask.values<N>(bits, m);
 #pragma unroll
       for (int e = 0; e < N; ++e) {
-        if (m[e] == 0.f) continue;       // whatever a masked token holds reaches nothing
-        const double w = m[e], x = v[e];
-        sums[2 * side] += w * (a.ref ? x - r[e] : x);
+        // whatever a masked token holds reaches nothing (no branch: the next loads would wait behind it)
+        const bool used = m[e] != 0.f;
+        const double w = m[e], x = used ? v[e] : 0.f;
+        sums[2 * side] += w * (a.ref ? x - (used ? r[e] : 0.f) : x);
         sums[2 * side + 1] += w;
         if (side == 0) sums[4] += w * x;
       }
@@ -495,28 +570,31 @@ __global__ void __launch_bounds__(PT_THREADS) pair_kernel(Pairs a, T* __restrict
       for (int k = 0; k < 5; ++k) to[k] = sums[k];
     }
     cluster.sync();
-#pragma unroll
-    for (int k = 0; k < 5; ++k) {
-      sums[k] = 0.0;
-      for (int i = 0; i < parts; ++i) sums[k] += by_block[i][k];
-    }
   }
-  const double count[2] = {fmax(sums[1], 1.0), fmax(sums[3], 1.0)};
-  const double score[2] = {a.normalized ? sums[0] / count[0] : sums[0], a.normalized ? sums[2] / count[1] : sums[2]};
-  double slope;
-  const double value = pair_loss(a, score[0] - score[1], &slope) - (a.nll != 0.0 ? a.nll * sums[4] / count[0] : 0.0);
-  if (threadIdx.x == 0 && rank == 0 && rewards) {
-    loss[p] = value;
-    rewards[p] = static_cast<float>(a.beta * score[0]);
-    rewards[p + a.pairs] = static_cast<float>(a.beta * score[1]);
+  // (one thread: the pipe for fp64 would keep a block's worth of exponentials for a microsecond)
+  if (threadIdx.x == 0) {
+    for (int i = 0; parts > 1 && i < parts; ++i)
+#pragma unroll
+      for (int k = 0; k < 5; ++k) sums[k] = (i ? sums[k] : 0.0) + by_block[i][k];
+    const double count[2] = {fmax(sums[1], 1.0), fmax(sums[3], 1.0)};
+    const double score[2] = {a.normalized ? sums[0] / count[0] : sums[0], a.normalized ? sums[2] / count[1] : sums[2]};
+    double slope;
+    const double value = pair_loss(a, score[0] - score[1], &slope) - (a.nll != 0.0 ? a.nll * sums[4] / count[0] : 0.0);
+    if (rank == 0 && rewards) {
+      loss[p] = value;
+      rewards[p] = static_cast<float>(a.beta * score[0]);
+      rewards[p + a.pairs] = static_cast<float>(a.beta * score[1]);
+    }
+    const double scale = up.get() / static_cast<double>(a.pairs);
+    weights[0] = static_cast<float>(((a.normalized ? slope / count[0] : slope) - a.nll / count[0]) * scale);
+    weights[1] = static_cast<float>((a.normalized ? -slope / count[1] : -slope) * scale);
   }
   if (!grad) return;
+  __syncthreads();
 #pragma unroll
   for (int side = 0; side < 2; ++side) {
     const long long row = p + side * a.pairs;
-    double w = (side ? -slope : slope) / (a.normalized ? count[side] : 1.0);
-    if (side == 0) w -= a.nll / count[0];
-    const float weight = static_cast<float>(w * up.get() / static_cast<double>(a.pairs));
+    const float weight = weights[side];
     over_row<VEC>(begin, end, static_cast<int>(row * a.T % VEC), [&](long long t, auto n) {
       constexpr int N = decltype(n)::value;
       float m[N];
@@ -548,9 +626,9 @@ static int pt_by_type(int dtype, F&& launch) {
 }
 
 static bool on_boundary(const void* p, int bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
-static int mask_bytes(int kind) {
-  static const int bytes[6] = {1, 4, 8, 4, 2, 2};
-  return bytes[kind];
+static Mask mask_of(const void* p, long long stride, long long kind) {
+  static const int shift[6] = {0, 2, 3, 2, 1, 1};
+  return {p, stride, static_cast<int>(kind), shift[kind]};
 }
 static int type_bytes(int dtype) { return dtype == 2 ? 4 : 2; }
 static double high_part(double v) { return static_cast<double>(static_cast<float>(v)); }
@@ -603,14 +681,14 @@ extern "C" int ts_policy_loss(const PolicyCall* c, void* stream) {
   a.logp = c->logp, a.old = c->old, a.ref = c->ref;
   a.s_logp = c->s_logp, a.s_old = c->s_old, a.s_ref = c->s_ref;
   a.advantages = c->advantages, a.per_token = static_cast<int>(c->per_token);
-  a.mask = {c->mask, c->s_mask, static_cast<int>(c->mask_kind)};
+  a.mask = mask_of(c->mask, c->s_mask, c->mask_kind);
   a.rows = c->rows, a.T = c->T, a.tokens = n;
   a.constant = c->constant, a.reduction = static_cast<int>(c->reduction);
   a.bound_low[0] = static_cast<float>(c->log_low), a.bound_low[1] = c->log_low < -1e30 ? 0.f : static_cast<float>(c->log_low - high_part(c->log_low));
   a.bound_high[0] = static_cast<float>(c->log_high), a.bound_high[1] = static_cast<float>(c->log_high - high_part(c->log_high));
   a.low = static_cast<float>(c->low), a.high = static_cast<float>(c->high), a.beta = static_cast<float>(c->beta);
   // four tokens at a time where they lie together and on a boundary in every tensor: rows without gaps, or rows of whole fours
-  const int e = type_bytes(static_cast<int>(c->dtype)), m = mask_bytes(a.mask.kind);
+  const int e = type_bytes(static_cast<int>(c->dtype)), m = 1 << a.mask.shift;
   a.flat = a.s_logp == a.T && a.s_old == a.T && (!a.ref || a.s_ref == a.T) && a.mask.stride == a.T;
   const bool fours = (a.flat || ((a.T | a.s_logp | a.s_old | (a.ref ? a.s_ref : 0) | a.mask.stride) & 3) == 0) && on_boundary(a.logp, 4 * e) &&
                      on_boundary(a.old, 4 * e) && on_boundary(a.ref, 4 * e) && on_boundary(a.mask.p, m == 8 ? 16 : 4 * m) &&
@@ -682,10 +760,10 @@ extern "C" int ts_preference_loss(const PairsCall* c, void* stream) {
       c->mask_kind > 5 || c->dtype < 0 || c->dtype > 2)
     return -1;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const Pairs a{c->logp, c->ref, c->s_logp, c->s_ref, {c->mask, c->s_mask, static_cast<int>(c->mask_kind)}, c->pairs, c->T,
+  const Pairs a{c->logp, c->ref, c->s_logp, c->s_ref, mask_of(c->mask, c->s_mask, c->mask_kind), c->pairs, c->T,
                 c->beta, c->gamma, c->smoothing, c->nll, static_cast<int>(c->kind), static_cast<int>(c->normalized)};
   // four tokens at a time where all tensors start on a boundary and their rows are as far behind one (the gradient's rows are T long)
-  const int e = type_bytes(static_cast<int>(c->dtype)), m = mask_bytes(a.mask.kind);
+  const int e = type_bytes(static_cast<int>(c->dtype)), m = 1 << a.mask.shift;
   const bool fours = ((a.s_logp ^ a.T) & 3) == 0 && (!a.ref || ((a.s_ref ^ a.T) & 3) == 0) && ((a.mask.stride ^ a.T) & 3) == 0 &&
                      on_boundary(a.logp, 4 * e) && on_boundary(a.ref, 4 * e) && on_boundary(a.mask.p, m == 8 ? 16 : 4 * m) &&
                      on_boundary(c->grad, 4 * e);
