@@ -4,6 +4,10 @@
 // kept between calls.  Norms: 2 (sqrt of the sum of squares), 1, inf.  A thread sums the 64 values that it has in flight in fp32
 // and adds the sum to an fp64 one; where that sum leaves the range in which fp32 squares keep their bits it is made again in
 // fp64.  The order of all sums depends on the sizes alone.
+//
+// Bounds: the memory.  1.05 GB of bf16 gradients: norm 163 to 170 us (6.2 to 6.4 TB/s), scaling 317 (6.6 TB/s); a norm below the
+// limit ends the second kernel at its first instruction.  Blocks of 512 threads with eight vectors each in flight; plain loads of
+// single values took 326 and 930. 128 tensors of 10 KB to 0.5 MB: 17 us on the GPU, 75 to 90 for the list's way through Python.
 #include <algorithm>
 #include <vector>
 
@@ -199,7 +203,8 @@ __global__ void __launch_bounds__(GN_THREADS) grad_norm_kernel(const __grid_cons
   if (threadIdx.x == 0) partial[blockIdx.x] = s;
 }
 
-__global__ void __launch_bounds__(1024) grad_norm_finish_kernel(const double* __restrict__ partial, int n, int kind, float* __restrict__ norm) {
+__global__ void __launch_bounds__(1024) grad_norm_finish_kernel(const double* __restrict__ partial, int n, int kind,
+                                                                float* __restrict__ norm) {
   __shared__ double scratch[32];
   double s = 0.0;
   for (int i = threadIdx.x; i < n; i += blockDim.x) s = join(partial[i], s, kind);
@@ -231,7 +236,8 @@ __device__ __forceinline__ void span_scale(const Span<T>& c, float factor) {
 
 // The coefficient stays fp32 and the product is rounded once.  Last chunks first: the norm has left them in the L2.
 template <typename Table>
-__global__ void __launch_bounds__(GN_THREADS) grad_scale_kernel(const __grid_constant__ Table t, const float* __restrict__ norm, float limit) {
+__global__ void __launch_bounds__(GN_THREADS) grad_scale_kernel(const __grid_constant__ Table t, const float* __restrict__ norm,
+                                                                float limit) {
   const float f = limit / (*norm + 1e-6f);
   if (f >= 1.f) return;                    // (NaN goes on: it makes every gradient NaN)
   for (int c = t.first[t.count] - 1 - static_cast<int>(blockIdx.x); c >= 0; c -= gridDim.x) {

@@ -8,9 +8,16 @@
 // logits cost no bits and rows of a type's lowest value do not overflow.  S = sum 2^u and U = sum u 2^u give
 // logp = k ln2 (v_label - m) - ln S and H = ln S - ln2 U / S, both terms of which are positive: nothing cancels.
 //
-// Forward reads the logits once: a thread keeps a running (m, S, U) over 16-byte vectors and raises m once for the vectors that it
-// has in flight.  Few rows: a block or a cluster per row, one launch.  Many: a warp per part of a row, all of them alike, so that
-// blocks end evenly and nothing waits inside a block; a second launch joins a row's parts.
+// Forward reads the logits once: a thread keeps a running (m, S, U) over 16-byte vectors and raises m once for the vectors that
+// it has in flight.  Few rows: a block or a cluster per row, one launch.  Many: a warp per part of a row, all of them alike, so
+// that blocks end evenly and nothing waits inside a block; a second launch joins a row's parts.
+//
+// Bounds: 2 bytes of a logit and an exponential for each of them; at the memory's rate the special-function unit is busy 70 % of
+// the time and the schedulers 60 %.  1644 rows of 128256 bf16 logits (421 MB) take 72 us, 79 with the entropy (5.8 and 5.3 TB/s,
+// joining included; a plain copy moves 6.5).  A block of 512 threads a row took 89: 1.4 to 1.7 rounds of blocks, and waits at
+// each row's end; clusters of two or four blocks 93 and 120; eight vectors in flight 105, parts of 512 vectors 89.  A quarter of
+// the exponentials as polynomials freed the special-function unit and cost as much in instructions.  A cap asks for 15
+// instructions an element: 2103 rows of 32001 fp32 logits (269 MB) take 67 us, 41 of them the memory's.
 #include <cooperative_groups.h>
 
 #include "common.cuh"
@@ -138,8 +145,8 @@ struct Vec<__half> {
   }
 };
 
-// Logits are read once in each direction and are gone by then: they pass the L1 by.  (Not by the read-only path: a gradient may take
-// their place.)
+// Logits are read once in each direction and are gone by then: they pass the L1 by.  (Not by the read-only path: a gradient may
+// take their place.)
 __device__ __forceinline__ uint4 load_once(const uint4* p) {
   uint4 v;
   asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
@@ -160,8 +167,9 @@ struct LogitRows {
   }
 };
 
-// tanh(x), x = z / c, out of E = e^(-2 |x|) <= 1, so that the slope 1 - tanh^2 = 4 E / (1 + E)^2 keeps its bits where tanh is close to
-// one; below 0.15, where 1 - E would lose them, a power series (x^9 is the first term left out: 6e-9).  Off by 2^-21 of its value.
+// tanh(x), x = z / c, out of E = e^(-2 |x|) <= 1, so that the slope 1 - tanh^2 = 4 E / (1 + E)^2 keeps its bits where tanh is
+// close to one; below 0.15, where 1 - E would lose them, a power series (x^9 is the first term left out: 6e-9).  Off by 2^-21 of
+// its value.
 __device__ __forceinline__ float tanh_series(float x) {
   const float q = x * x;
   return x * fmaf(q, fmaf(q, fmaf(q, -17.f / 315.f, 2.f / 15.f), -1.f / 3.f), 1.f);
@@ -173,8 +181,8 @@ __device__ __forceinline__ float capped(float z, float inv_cap, float* slope = n
   if (slope) *slope = 4.f * e * r * r;
   return fabsf(x) < 0.15f ? tanh_series(x) : copysignf((1.f - e) * r, x);
 }
-// Two at once, 1 / (1 + E) by Newton's iteration from a parabola through it at E = 0, 1/2 and 1 (off by 0.016, then by 3e-4 and 7e-8):
-// two calls of the special-function unit for an element instead of three, which is what bounds the forward pass.
+// Two at once, 1 / (1 + E) by Newton's iteration from a parabola through it at E = 0, 1/2 and 1 (off by 0.016, then by 3e-4 and
+// 7e-8): two calls of the special-function unit for an element instead of three, which is what bounds the forward pass.
 template <bool CAP>
 __device__ __forceinline__ Pair capped2(float z, float w, float inv_cap) {
   if (!CAP) return Pair(z, w);
@@ -224,9 +232,9 @@ __device__ __forceinline__ void add_value(Softmax& acc, float z, float k2, float
   if (ENT) acc.u += t * e;
 }
 
-// Adds the first `n` of N 16-byte vectors to a thread's (m, S, U); the others hold values of -inf, which count for nothing unless a cap
-// makes them finite.  An entropy's 0 * -inf (logits of -inf) shows as NaN; it is then summed again with
-// exponents that are bounded below.
+// Adds the first `n` of N 16-byte vectors to a thread's (m, S, U); the others hold values of -inf, which count for nothing unless
+// a cap makes them finite.  An entropy's 0 * -inf (logits of -inf) shows as NaN; it is then summed again with exponents that are
+// bounded below.
 template <typename T, bool CAP, bool ENT, int N>
 __device__ __forceinline__ void add_vectors(Softmax& acc, const uint4* r, int n, float k2, float inv_cap) {
   using W = Vec<T>;
@@ -433,8 +441,10 @@ __global__ void __launch_bounds__(LP_PART_THREADS) logprob_join_kernel(const T* 
   if (lane == 0) row_results<T, CAP>(acc, row, r, label, a, logp, entropy, kept);
 }
 
-// A block takes LP_BACK_THREADS * LP_BACK_FLIGHT vectors of one row.  A thread has read what it writes over before it writes,
-// and no other thread reads that: the gradient may replace the logits.
+// A block takes LP_BACK_THREADS * LP_BACK_FLIGHT vectors of one row: small blocks that start with all their loads.  The gradient
+// of the rows above (946 MB) takes 141 us, 6.7 TB/s; 512 threads with four vectors took 174, 128 with two 193, 64 with sixteen
+// 151.  Streaming stores take 62 to 60 us off the gradient of 2934 rows of 32000.  A thread has read what it writes over before
+// it writes, and no other thread reads that: the gradient may replace the logits.
 template <typename T, bool CAP, bool ENT>
 __global__ void __launch_bounds__(LP_BACK_THREADS) logprob_bwd_kernel(const T* logits, const long long* __restrict__ labels,
                                                                  const float4* __restrict__ kept, const float* __restrict__ grad_logp,
@@ -469,7 +479,10 @@ __global__ void __launch_bounds__(LP_BACK_THREADS) logprob_bwd_kernel(const T* l
   uint4 r[LP_BACK_FLIGHT];
   if (aligned) {
 #pragma unroll
-    for (int j = 0; j < LP_BACK_FLIGHT; ++j) r[j] = first + j * LP_BACK_THREADS < vectors ? load_once(body + first + j * LP_BACK_THREADS) : make_uint4(0, 0, 0, 0);
+    for (int j = 0; j < LP_BACK_FLIGHT; ++j) {
+      const int i = first + j * LP_BACK_THREADS;
+      r[j] = i < vectors ? load_once(body + i) : make_uint4(0, 0, 0, 0);
+    }
   }
   const float4 k = kept[row];
   const float m = k.x, f = a.k * (CAP ? a.inv_cap : 1.f);
@@ -544,10 +557,10 @@ using namespace ts;
 
 TS_DEFINE_ERROR_API(ts_logprob)
 
-// Parts of a row that warps of their own take; 0: a block or a cluster takes the row.  A row of one part always has a warp (4 rows of
-// 2000: 2.9 us, in blocks 3.2; 1200: 3.8 and 11).  Longer rows have blocks of their own while those are fewer than four to an SM, and need no
-// second launch (rows of 128256 in blocks and in warps: 9.3 and 9.6 us for 100, 21.6 and 23.9 for 400, 33.3 and 31.7 for 600; of 32000: 7.5
-// and 8.1, 8.4 and 9.7, 11.8 and 12.1).
+// Parts of a row that warps of their own take; 0: a block or a cluster takes the row.  A row of one part always has a warp (4
+// rows of 2000: 2.9 us, in blocks 3.2; 1200: 3.8 and 11).  Longer rows have blocks of their own while those are fewer than four
+// to an SM, and need no second launch (rows of 128256 in blocks and in warps: 9.3 and 9.6 us for 100, 21.6 and 23.9 for 400, 33.3
+// and 31.7 for 600; of 32000: 7.5 and 8.1, 8.4 and 9.7, 11.8 and 12.1).
 static int row_parts(long long rows, long long V, int dtype) {
   const long long vectors = V * (dtype == 2 ? 4 : 2) / 16, parts = (vectors + LP_PART - 1) / LP_PART;
   return parts <= 1 ? 1 : rows < 4 * sm_count() ? 0 : static_cast<int>(parts);
@@ -559,10 +572,11 @@ extern "C" long long ts_logprob_workspace(long long rows, long long V, int dtype
   return parts > 1 ? rows * parts * static_cast<long long>(sizeof(Softmax)) : 0;
 }
 
-// The arguments of a call, eight bytes each (ops/logprob.py packs them).  dtype: 0 bf16, 1 fp16, 2 fp32.  lenient: labels outside the
-// vocabulary count as ignored; otherwise they give NaN.  kept: (m, S, H, unused) of every row, for the backward pass; H counts only with
-// an entropy.  Forward: logp and, where they are not null, entropy and kept are results.  Backward: logp and entropy are what flows into
-// them (null: zero), grad the result, its rows grad_stride elements apart; it may be the logits themselves, where their rows are.
+// The arguments of a call, eight bytes each (ops/logprob.py packs them).  dtype: 0 bf16, 1 fp16, 2 fp32.  lenient: labels outside
+// the vocabulary count as ignored; otherwise they give NaN.  kept: (m, S, H, unused) of every row, for the backward pass; H
+// counts only with an entropy.  Forward: logp and, where they are not null, entropy and kept are results.  Backward: logp and
+// entropy are what flows into them (null: zero), grad the result, its rows grad_stride elements apart; it may be the logits
+// themselves, where their rows are.
 struct LogprobCall {
   const void* logits;
   long long dtype;
@@ -576,7 +590,8 @@ struct LogprobCall {
 };
 
 static bool valid(const LogprobCall* c, long long units) {
-  return c->rows > 0 && c->inner > 0 && c->V > 0 && c->V <= 0x7fffffffll && c->rows <= 0x7fffffffll / units && c->dtype >= 0 && c->dtype <= 2;
+  return c->rows > 0 && c->inner > 0 && c->V > 0 && c->V <= 0x7fffffffll && c->rows <= 0x7fffffffll / units && c->dtype >= 0 &&
+         c->dtype <= 2;
 }
 static LogitRows logit_rows(const LogprobCall* c) {
   const double k = c->factor * (c->cap > 0.0 ? c->cap : 1.0);
@@ -602,14 +617,16 @@ extern "C" int ts_logprob_fwd(const LogprobCall* c, void* stream) {
       if (units == 1) return static_cast<int>(cudaGetLastError());
       const int rc = static_cast<int>(cudaGetLastError());
       if (rc) return rc;
-      return launch_chained(logprob_join_kernel<T, CAP, ENT>, dim3(static_cast<unsigned>((a.rows + warps - 1) / warps)), dim3(LP_PART_THREADS), 0,
-                            st, 1, true, z, c->labels, partial, c->logp, c->entropy, c->kept, a, units);
+      const dim3 joining(static_cast<unsigned>((a.rows + warps - 1) / warps));
+      return launch_chained(logprob_join_kernel<T, CAP, ENT>, joining, dim3(LP_PART_THREADS), 0, st, 1, true, z, c->labels,
+                            partial, c->logp, c->entropy, c->kept, a, units);
     }
     int parts = 1;                       // of a cluster, each with a vector or two for every thread
     const long long vectors = c->V * static_cast<int>(sizeof(T)) / 16;
     while (parts < LP_SPLIT && a.rows * parts < 2 * sm_count() && vectors / parts >= 2 * LP_THREADS) parts *= 2;
-    return launch_chained(logprob_row_kernel<T, CAP, ENT>, dim3(static_cast<unsigned>(a.rows * parts)), dim3(LP_THREADS), 0, st, parts, false,
-                          z, c->labels, c->logp, c->entropy, c->kept, a);
+    const dim3 blocks(static_cast<unsigned>(a.rows * parts));
+    return launch_chained(logprob_row_kernel<T, CAP, ENT>, blocks, dim3(LP_THREADS), 0, st, parts, false, z, c->labels,
+                          c->logp, c->entropy, c->kept, a);
   });
 }
 

@@ -5,9 +5,9 @@
 //   r = e^(logp - old),  clipped = a > 0 ? r > 1 + high : a < 0 and r < 1 - low,  d = ref - logp
 //   token = -a (clipped ? bound : r) + beta (e^d - 1 - d),  d token / d logp = (clipped ? 0 : -a r) - beta (e^d - 1)
 //   loss  = sum m w token,  w = 1 / (rows sum_row m), 1 / sum m or 1 / (rows length); the sums of m are at least 1
-// A token's gradient jumps at a bound, so the side that it is on is decided by logp - old without rounding (two fp32 numbers whose
-// sum is the difference).  e^d - 1 - d is a power series near zero, where the difference would cancel.  Sums of four or eight
-// tokens are fp32, sums of those fp64, in an order that depends on the sizes alone.
+// A token's gradient jumps at a bound, so the side that it is on is decided by logp - old without rounding (two fp32 numbers
+// whose sum is the difference).  e^d - 1 - d is a power series near zero, where the difference would cancel.  Sums of four or
+// eight tokens are fp32, sums of those fp64, in an order that depends on the sizes alone.
 //
 // Pairs, rows p (chosen) and P + p (rejected), of scores s = sum m (logp - ref), divided by max(sum m, 1) where asked:
 //   x = s_p - s_(P + p),  q = beta x - gamma
@@ -15,8 +15,14 @@
 //   ipo (x - 1 / (2 beta))^2;  and nll * the mean of -logp over the chosen row's tokens
 // The scores are long sums whose difference decides: they, and all that is done per pair, are fp64.
 //
-// Gradients leave with the loss, for an upstream gradient of one.  Where it turns out to be another, fp32 gradients are multiplied
-// by it; 16-bit ones, which that would round twice, are computed again (`Upstream`).
+// Gradients leave with the loss, for an upstream gradient of one.  Where it turns out to be another, fp32 gradients are
+// multiplied by it; 16-bit ones, which that would round twice, are computed again (`Upstream`).
+//
+// Bounds: instructions and their latencies; a token costs two exponentials, a series and five sums.  512 x 16384 tokens with a KL
+// term, half of them masked: 10 us to count and 36 for the rest (168 MB without the masked tokens' would be 26 at the memory's
+// rate); reading a masked token's inputs cost 42.  160 pairs of 16384 tokens 18 us (84 MB: 13), 600 of them 65 (255 MB: 39); a
+// block's worth of fp64 exponentials instead of one thread's cost 3 us there.  Small calls are one or two launches of 5 to 9 us,
+// behind 110 us of Python, 60 of which are an empty autograd function's.
 #include <cooperative_groups.h>
 
 #include "common.cuh"
@@ -68,15 +74,16 @@ __device__ __forceinline__ void put(T* p, const float* f) {
   *reinterpret_cast<Few<T, N>*>(p) = v;
 }
 
-// N values of a mask.  They are loaded as they are and become fp32 when they are needed: a branch on their type that waited for them
-// would keep the other loads waiting too.
+// N values of a mask.  They are loaded as they are and become fp32 when they are needed: a branch on their type that waited for
+// them would keep the other loads waiting too.
 template <int N>
 struct MaskBits {
   uint32_t w[2 * N];
 };
 template <typename T, int N>
 __device__ __forceinline__ float mask_value(const MaskBits<N>& b, int i) {
-  if constexpr (sizeof(T) == 8) return static_cast<float>(static_cast<long long>(b.w[2 * i] | static_cast<unsigned long long>(b.w[2 * i + 1]) << 32));
+  if constexpr (sizeof(T) == 8)
+    return static_cast<float>(static_cast<long long>(b.w[2 * i] | static_cast<unsigned long long>(b.w[2 * i + 1]) << 32));
   constexpr int in_word = 4 / sizeof(T) > 0 ? 4 / sizeof(T) : 1;
   const uint32_t word = b.w[i / in_word] >> (i % in_word * (32 / in_word));
   if constexpr (sizeof(T) == 1) return static_cast<float>(word & 0xff);
@@ -179,7 +186,9 @@ __device__ __forceinline__ void block_sums(double* v, double (*scratch)[N]) {
 constexpr int POLICY_PER_SM = 4;         // blocks of an SM
 constexpr int POLICY_SUMS = 5;           // loss, kl m, clipped m, ratio m, m
 constexpr int POLICY_SPLIT = 8;          // most blocks that count a row
-constexpr int POLICY_ALONE = 8192;       // tokens that one block takes by itself, in one launch
+// Tokens that one block takes by itself, in one launch (8 x 64: 5.4 us, in two launches 7.8; 8 x 1024: 8.9 and 9.0; 16 x 1024:
+// 13.1 and 8.1).
+constexpr int POLICY_ALONE = 8192;
 constexpr int POLICY_ALONE_THREADS = 1024, POLICY_ALONE_ROWS = 4096;
 
 struct Policy {
@@ -358,8 +367,8 @@ __device__ __forceinline__ void policy_results(const double* sums, float* loss, 
     for (int k = 1; k < 4; ++k) stats[k - 1] = static_cast<float>(sums[k] / fmax(sums[4], 1.0));
 }
 
-// What the tokens weigh: weights [rows] (reduction 0, a block or a cluster per row), sums of the mask by block (reduction 1); and the
-// counter that tells the next kernel's last block.
+// What the tokens weigh: weights [rows] (reduction 0, a block or a cluster per row), sums of the mask by block (reduction 1); and
+// the counter that tells the next kernel's last block.
 template <int VEC>
 __global__ void __launch_bounds__(PT_THREADS) policy_count_kernel(Policy a, float* __restrict__ weights, double* __restrict__ counts,
                                                                   unsigned* __restrict__ ticket, Upstream up) {
@@ -394,10 +403,9 @@ __global__ void __launch_bounds__(PT_THREADS) policy_count_kernel(Policy a, floa
 }
 
 template <typename T, int VEC, bool FLAT>
-__global__ void __launch_bounds__(PT_THREADS, POLICY_PER_SM) policy_kernel(Policy a, const float* __restrict__ weights, const double* __restrict__ counts,
-                                                            double* __restrict__ partial, unsigned* __restrict__ ticket,
-                                                            T* __restrict__ grad, float* __restrict__ loss, float* __restrict__ stats,
-                                                            Upstream up) {
+__global__ void __launch_bounds__(PT_THREADS, POLICY_PER_SM)
+    policy_kernel(Policy a, const float* __restrict__ weights, const double* __restrict__ counts, double* __restrict__ partial,
+                  unsigned* __restrict__ ticket, T* __restrict__ grad, float* __restrict__ loss, float* __restrict__ stats, Upstream up) {
   __shared__ double scratch[32][POLICY_SUMS];
   __shared__ bool last;
   if (up.done()) return;
@@ -470,7 +478,8 @@ __global__ void __launch_bounds__(POLICY_ALONE_THREADS) policy_alone_kernel(Poli
 __global__ void __launch_bounds__(PT_THREADS) scale_kernel(float* __restrict__ grad, const float* __restrict__ factor, long long n) {
   const float f = *factor;
   if (f == 1.f) return;
-  const long long step = gridDim.x * static_cast<long long>(PT_THREADS), first = blockIdx.x * static_cast<long long>(PT_THREADS) + threadIdx.x;
+  const long long step = gridDim.x * static_cast<long long>(PT_THREADS);
+  const long long first = blockIdx.x * static_cast<long long>(PT_THREADS) + threadIdx.x;
   float4* fours = reinterpret_cast<float4*>(grad);
   for (long long i = first; i < n / 4; i += step) {
     const float4 v = fours[i];
@@ -515,12 +524,13 @@ __device__ __forceinline__ double pair_loss(const Pairs& a, double x, double* sl
   return d * d;
 }
 
-// Calls f(t, N) over [begin, end) of a row whose token 0 is `phase` tokens behind a vector's boundary: single tokens up to the first
-// boundary and behind the last, VEC at a time between them.
+// Calls f(t, N) over [begin, end) of a row whose token 0 is `phase` tokens behind a vector's boundary: single tokens up to the
+// first boundary and behind the last, VEC at a time between them.
 template <int VEC, typename F>
 __device__ __forceinline__ void over_row(long long begin, long long end, int phase, F&& f) {
   const long long first = min(end, begin + (VEC - (begin + phase) % VEC) % VEC), past = first + (end - first) / VEC * VEC;
-  for (long long t = first + static_cast<long long>(threadIdx.x) * VEC; t < past; t += PT_THREADS * VEC) f(t, std::integral_constant<int, VEC>());
+  for (long long t = first + static_cast<long long>(threadIdx.x) * VEC; t < past; t += PT_THREADS * VEC)
+    f(t, std::integral_constant<int, VEC>());
   const int before = static_cast<int>(first - begin), singles = before + static_cast<int>(end - past), i = threadIdx.x;
   if (i < singles) f(i < before ? begin + i : past + (i - before), std::integral_constant<int, 1>());
 }
@@ -639,9 +649,9 @@ using namespace ts;
 
 TS_DEFINE_ERROR_API(ts_posttrain)
 
-// The arguments of a call, eight bytes each (ops/policy.py packs them).  dtype (of logp, old, ref and grad): 0 bf16, 1 fp16, 2 fp32.
-// ref, grad and stats may be null; loss too where only the gradient is wanted, times *factor (and where that is one, with `redo`
-// alone).  stats: mean kl, share of clipped tokens, mean ratio.
+// The arguments of a call, eight bytes each (ops/policy.py packs them).  dtype (of logp, old, ref and grad): 0 bf16, 1 fp16, 2
+// fp32. ref, grad and stats may be null; loss too where only the gradient is wanted, times *factor (and where that is one, with
+// `redo` alone).  stats: mean kl, share of clipped tokens, mean ratio.
 struct PolicyCall {
   long long dtype;
   const void* logp;
@@ -684,13 +694,15 @@ extern "C" int ts_policy_loss(const PolicyCall* c, void* stream) {
   a.mask = mask_of(c->mask, c->s_mask, c->mask_kind);
   a.rows = c->rows, a.T = c->T, a.tokens = n;
   a.constant = c->constant, a.reduction = static_cast<int>(c->reduction);
-  a.bound_low[0] = static_cast<float>(c->log_low), a.bound_low[1] = c->log_low < -1e30 ? 0.f : static_cast<float>(c->log_low - high_part(c->log_low));
+  a.bound_low[0] = static_cast<float>(c->log_low);
+  a.bound_low[1] = c->log_low < -1e30 ? 0.f : static_cast<float>(c->log_low - high_part(c->log_low));
   a.bound_high[0] = static_cast<float>(c->log_high), a.bound_high[1] = static_cast<float>(c->log_high - high_part(c->log_high));
   a.low = static_cast<float>(c->low), a.high = static_cast<float>(c->high), a.beta = static_cast<float>(c->beta);
   // four tokens at a time where they lie together and on a boundary in every tensor: rows without gaps, or rows of whole fours
   const int e = type_bytes(static_cast<int>(c->dtype)), m = 1 << a.mask.shift;
   a.flat = a.s_logp == a.T && a.s_old == a.T && (!a.ref || a.s_ref == a.T) && a.mask.stride == a.T;
-  const bool fours = (a.flat || ((a.T | a.s_logp | a.s_old | (a.ref ? a.s_ref : 0) | a.mask.stride) & 3) == 0) && on_boundary(a.logp, 4 * e) &&
+  const bool fours = (a.flat || ((a.T | a.s_logp | a.s_old | (a.ref ? a.s_ref : 0) | a.mask.stride) & 3) == 0) &&
+                     on_boundary(a.logp, 4 * e) &&
                      on_boundary(a.old, 4 * e) && on_boundary(a.ref, 4 * e) && on_boundary(a.mask.p, m == 8 ? 16 : 4 * m) &&
                      on_boundary(c->grad, 4 * e) && (!a.per_token || on_boundary(a.advantages, 16)) && n % 4 == 0;
   const int vec = fours ? 4 : 1;
@@ -716,9 +728,11 @@ extern "C" int ts_policy_loss(const PolicyCall* c, void* stream) {
       if (a.reduction == 0)
         while (parts < POLICY_SPLIT && a.rows * parts < 2 * sm_count() && a.T / parts >= 8 * PT_THREADS * VEC) parts *= 2;
       const unsigned counters = a.reduction == 0 ? static_cast<unsigned>(a.rows * parts) : a.reduction == 1 ? used : 1;
-      const int rc = launch_chained(policy_count_kernel<VEC>, dim3(counters), dim3(PT_THREADS), 0, st, parts, false, a, weights, counts, ticket, up);
+      const int rc = launch_chained(policy_count_kernel<VEC>, dim3(counters), dim3(PT_THREADS), 0, st, parts, false, a, weights, counts,
+                                    ticket, up);
       if (rc) return rc;
-      policy_kernel<E, VEC, FLAT><<<used, PT_THREADS, 0, st>>>(a, weights, counts, partial, ticket, static_cast<E*>(c->grad), c->loss, c->stats, up);
+      policy_kernel<E, VEC, FLAT><<<used, PT_THREADS, 0, st>>>(a, weights, counts, partial, ticket, static_cast<E*>(c->grad), c->loss,
+                                                               c->stats, up);
       return static_cast<int>(cudaGetLastError());
     };
     using four = std::integral_constant<int, 4>;
@@ -762,12 +776,14 @@ extern "C" int ts_preference_loss(const PairsCall* c, void* stream) {
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const Pairs a{c->logp, c->ref, c->s_logp, c->s_ref, mask_of(c->mask, c->s_mask, c->mask_kind), c->pairs, c->T,
                 c->beta, c->gamma, c->smoothing, c->nll, static_cast<int>(c->kind), static_cast<int>(c->normalized)};
-  // four tokens at a time where all tensors start on a boundary and their rows are as far behind one (the gradient's rows are T long)
+  // four tokens at a time where all tensors start on a boundary and their rows are as far behind one (the gradient's rows are T
+  // long)
   const int e = type_bytes(static_cast<int>(c->dtype)), m = 1 << a.mask.shift;
   const bool fours = ((a.s_logp ^ a.T) & 3) == 0 && (!a.ref || ((a.s_ref ^ a.T) & 3) == 0) && ((a.mask.stride ^ a.T) & 3) == 0 &&
                      on_boundary(a.logp, 4 * e) && on_boundary(a.ref, 4 * e) && on_boundary(a.mask.p, m == 8 ? 16 : 4 * m) &&
                      on_boundary(c->grad, 4 * e);
-  // a pair is split while blocks are fewer than four to an SM and its parts are worth one
+  // a pair is split while blocks are fewer than four to an SM and its parts are worth one (in one block and split: one pair of
+  // 16384 24.3 and 10.6 us, 160 of them 31.9 and 18.9; one of 1024 7.2 and 8.9, 160 of 4096 in eight blocks each 12.5 and 23.4)
   int parts = 1;
   while (parts < PAIR_SPLIT && a.pairs * parts < 4 * sm_count() && a.T / parts >= 2 * PAIR_TOKENS) parts *= 2;
   return pt_by_type(static_cast<int>(c->dtype), [&](auto* t) {

@@ -238,7 +238,8 @@ def grpo_loss(logp: torch.Tensor = None, old_logp: torch.Tensor = None, ref_logp
     if policy_log_probs is not None:
         return _reference_rl_loss("grpo", policy_log_probs, ref_log_probs, advantages, mask, beta)
     if _takes_policy_kernel(logp, old_logp, ref_logp, advantages, mask) and 0 <= clip and 0 <= beta:
-        return clipped_policy_loss(logp, old_logp, advantages, mask, ref_logp if beta else None, clip=clip, beta=beta if ref_logp is not None else 0.0)
+        beta = beta if ref_logp is not None else 0.0
+        return clipped_policy_loss(logp, old_logp, advantages, mask, ref_logp if beta else None, clip=clip, beta=beta)
     ratio = torch.exp(logp - old_logp)
     a = advantages.unsqueeze(-1)
     obj = torch.minimum(ratio * a, ratio.clamp(1 - clip, 1 + clip) * a)
