@@ -190,7 +190,7 @@ __device__ __forceinline__ Pair capped2(float z, float w, float inv_cap) {
   const float2 x = v.get();
   const float2 series = (v * fma2(q, fma2(q, fma2(q, Pair(-17.f / 315.f, -17.f / 315.f), Pair(2.f / 15.f, 2.f / 15.f)),
                                           Pair(-1.f / 3.f, -1.f / 3.f)), one)).get();
-  const Pair e(fast_ex2(fabsf(x.x) * (-2.f * LOG2E)), fast_ex2(fabsf(x.y) * (-2.f * LOG2E))), d = (e + one) * minus;
+  const Pair e(fast_ex2(fabsf(x.x) * (-2.f * LOG2E)), fast_ex2(fabsf(x.y) * (-2.f * LOG2E))), d = fma2(e, minus, minus);
   Pair r = fma2(e, fma2(e, Pair(1.f / 3.f, 1.f / 3.f), Pair(-5.f / 6.f, -5.f / 6.f)), one);
   r = r * fma2(d, r, two);
   r = r * fma2(d, r, two);

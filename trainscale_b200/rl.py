@@ -226,7 +226,7 @@ def preference_loss(policy_logps: torch.Tensor, ref_logps: torch.Tensor | None, 
     P = policy_logps.shape[0] // 2
     loss, rewards = policy_ops.preference_loss(policy_logps, ref_logps, mask, float(beta), loss_type, float(label_smoothing), float(gamma),
                                                bool(length_normalized), float(nll_weight))
-    return loss, rewards[:P], rewards[P:]
+    return (loss, *rewards.view(2, P).unbind())
 
 
 def grpo_loss(logp: torch.Tensor = None, old_logp: torch.Tensor = None, ref_logp: torch.Tensor | None = None,
