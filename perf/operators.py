@@ -340,7 +340,7 @@ def _run_clip(s, case):
     if own:
         from trainscale_b200.optim import clip_grad_norm_
         norm = clip_grad_norm_(s["parameters"], limit, kind)
-        return [norm, *s["buffers"]]
+        return [norm.float(), *s["buffers"]]        # (the largest value of gradients of one type comes in that type)
     grads = [p.grad for p in s["parameters"]]
     if case["norm"] == "inf":
         norm = torch.stack([g.float().abs().max() for g in grads]).max()
