@@ -566,6 +566,9 @@ static int row_parts(long long rows, long long V, int dtype) {
   return parts <= 1 ? 1 : rows < 4 * sm_count() ? 0 : static_cast<int>(parts);
 }
 
+// Fewer rows than these need no workspace.
+extern "C" int ts_logprob_few_rows() { return 4 * sm_count(); }
+
 // Bytes of workspace that ts_logprob_fwd needs.
 extern "C" long long ts_logprob_workspace(long long rows, long long V, int dtype) {
   const int parts = row_parts(rows, V, dtype);
@@ -612,6 +615,7 @@ extern "C" int ts_logprob_fwd(const LogprobCall* c, void* stream) {
     const T* z = static_cast<const T*>(c->logits);
     if (units) {
       Softmax* partial = static_cast<Softmax*>(c->workspace);
+      if (units > 1 && !partial) return -1;
       logprob_part_kernel<T, CAP, ENT><<<static_cast<unsigned>((a.rows * units + warps - 1) / warps), LP_PART_THREADS, 0, st>>>(
           z, c->labels, partial, c->logp, c->entropy, c->kept, a, units);
       if (units == 1) return static_cast<int>(cudaGetLastError());

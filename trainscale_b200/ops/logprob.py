@@ -65,6 +65,7 @@ def _library():
     lib = _lib.load("logprob")
     lib.ts_logprob_fwd.argtypes = lib.ts_logprob_bwd.argtypes = [c_char_p, c_void_p]
     lib.ts_logprob_workspace.argtypes, lib.ts_logprob_workspace.restype = [c_longlong, c_longlong, c_int], c_longlong
+    lib.few_rows = lib.ts_logprob_few_rows()         # fewer never need a workspace
     return lib
 
 
@@ -76,10 +77,15 @@ def _stream() -> int:
     return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
 
 
+def fp32(x: torch.Tensor, *shape: int) -> torch.Tensor:
+    """A new fp32 tensor where `x` is (spelling the type out costs a microsecond)."""
+    return x.new_empty(shape) if x.dtype is torch.float32 else x.new_empty(shape, dtype=torch.float32)
+
+
 def _run_forward(x, rows, labels, logp, H, kept, factor=1.0, cap=0.0, ignore_index=None, lenient=False) -> None:
     lib, V, kind = _library(), x.shape[-1], _DTYPES[x.dtype]
-    need = lib.ts_logprob_workspace(rows[0], V, kind)
-    work = x.new_empty(need, dtype=torch.uint8) if need else None
+    need = lib.ts_logprob_workspace(rows[0], V, kind) if rows[0] >= lib.few_rows else 0
+    work = fp32(x, need // 4) if need else None
     call = _CALL.pack(x.data_ptr(), kind, labels.data_ptr(), logp.data_ptr(), _address(H), _address(kept), _address(work), 0, 0, *rows, V,
                       factor, cap, _NEVER if ignore_index is None else ignore_index, lenient)
     _lib.check(lib.ts_logprob_fwd(call, _stream()), "ts_logprob_fwd")
@@ -93,9 +99,9 @@ def _run_backward(x, rows, labels, kept, g, h, grad, pitch, factor=1.0, cap=0.0,
 
 def _forward(logits, labels, how, entropy: bool, keep: bool):
     x, rows = _rows(logits)
-    logp = x.new_empty(labels.shape, dtype=torch.float32)
-    H = x.new_empty(labels.shape, dtype=torch.float32) if entropy else None
-    kept = x.new_empty((rows[0], 4), dtype=torch.float32) if keep else None
+    logp = fp32(x, *labels.shape)
+    H = fp32(x, *labels.shape) if entropy else None
+    kept = fp32(x, rows[0], 4) if keep else None
     _run_forward(x, rows, labels, logp, H, kept, *how)
     return logp, H, kept
 
@@ -142,19 +148,21 @@ class _TokenLogProbs(torch.autograd.Function):
 def token_log_probs(logits: torch.Tensor, labels: torch.Tensor, factor: float = 1.0, cap: float = 0.0,
                     ignore_index: int | None = -100, entropy: bool = False):
     """log softmax(factor * cap tanh(logits / cap))[labels] in fp32 (and the distribution's entropy)."""
-    if labels.shape != logits.shape[:-1]:
-        raise ValueError(f"labels of shape {tuple(labels.shape)} for logits of shape {tuple(logits.shape)}")
-    if labels.dtype != torch.int64 and labels.dtype != torch.int32:
-        raise TypeError(f"labels are int64 or int32, not {labels.dtype}")
+    shape, kind = logits.shape, labels.dtype
+    if labels.shape != shape[:-1]:
+        raise ValueError(f"labels of shape {tuple(labels.shape)} for logits of shape {tuple(shape)}")
+    if kind is not torch.int64 and kind is not torch.int32:
+        raise TypeError(f"labels are int64 or int32, not {kind}")
     if not logits.is_floating_point():
         raise TypeError(f"logits are floating point, not {logits.dtype}")
-    if logits.shape[-1] == 0:
+    if shape[-1] == 0:
         raise ValueError("logits of an empty vocabulary")
     how = (factor, cap, ignore_index)
     if not native(logits, labels):
         return plain(logits, labels, *how, entropy)
-    labels = labels.to(torch.int64).contiguous()
-    if torch.is_grad_enabled() and logits.requires_grad:
+    if kind is not torch.int64 or not labels.is_contiguous():
+        labels = labels.to(torch.int64).contiguous()
+    if logits.requires_grad and torch.is_grad_enabled():
         labels = labels.clone() if labels.is_inference() else labels      # (such tensors cannot be kept for a backward pass)
         return _TokenLogProbs.apply(logits, labels, how, entropy)
     logp, H, _ = _forward(logits, labels, how, entropy, False)

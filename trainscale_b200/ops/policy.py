@@ -16,7 +16,7 @@ import torch
 import torch.nn.functional as F
 
 from . import _lib
-from .logprob import _DTYPES, _address, _stream, on_this_gpu
+from .logprob import _DTYPES, _address, _stream, fp32, on_this_gpu
 
 _MASKS = {torch.bool: 0, torch.uint8: 0, torch.int32: 1, torch.int64: 2, torch.float32: 3, torch.bfloat16: 4, torch.float16: 5}
 REDUCTIONS = {"sequence": 0, "token": 1, "constant": 2}
@@ -141,18 +141,20 @@ class PolicyLoss:
 
     def __call__(self, logp, old, advantages, mask, ref, grad=None, factor=None):
         p, old, ref = _one_type(logp, old, ref)
-        mask, advantages = _mask_of(mask), advantages.float().contiguous()
+        mask = _mask_of(mask)
+        if advantages.dtype is not torch.float32 or not advantages.is_contiguous():
+            advantages = advantages.float().contiguous()
         B, T = p.shape
         lib, low, high = _library(), self.low, self.high
         loss = stats = work = None
         if factor is None:
-            loss = p.new_empty((), dtype=torch.float32)
+            loss = fp32(p)
             if self.stats:
-                stats = p.new_empty(3, dtype=torch.float32)
+                stats = fp32(p, 3)
         out = _gradient(p) if grad is True else grad
         need = lib.ts_policy_workspace(B, T)
         if need:
-            work = p.new_empty(need, dtype=torch.float64)
+            work = fp32(p, 2 * need)
         call = _POLICY_CALL.pack(
             _DTYPES[p.dtype], *_place(p), *_place(old), *_place(ref), advantages.data_ptr(), advantages.dim() == 2, *_place(mask),
             _MASKS[mask.dtype], B, T, math.log1p(-low) if low < 1 else -math.inf, math.log1p(high), 1 - low, 1 + high, self.beta,
@@ -208,9 +210,9 @@ class PairLoss:
         R, T = p.shape
         loss = rewards = None
         if factor is None:
-            loss, rewards = p.new_empty((), dtype=torch.float32), p.new_empty(R, dtype=torch.float32)
+            loss, rewards = fp32(p), fp32(p, R)
         out = _gradient(p) if grad is True else grad
-        work = p.new_empty(R // 2, dtype=torch.float64)
+        work = fp32(p, R)                             # R / 2 fp64 values
         call = _PAIRS_CALL.pack(
             _DTYPES[p.dtype], *_place(p), *_place(ref), *_place(mask), _MASKS[mask.dtype], R // 2, T, self.beta, self.gamma,
             self.smoothing, self.nll, KINDS[self.kind], self.normalized, _address(out), _address(loss), _address(rewards),
