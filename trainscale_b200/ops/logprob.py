@@ -28,7 +28,8 @@ def on_this_gpu(*tensors) -> bool:
 
 
 def native(logits: torch.Tensor, labels: torch.Tensor) -> bool:
-    return logits.dtype in _DTYPES and on_this_gpu(logits, labels) and logits.numel() > 0 and logits.shape[-1] < 1 << 31
+    """Whether the kernels take these: 16- or 32-bit logits on the current device, some of them, and no more rows than a launch counts."""
+    return (logits.dtype in _DTYPES and on_this_gpu(logits, labels) and 0 < labels.numel() < 1 << 28 and 0 < logits.shape[-1] < 1 << 31)
 
 
 def plain(logits, labels, factor: float, cap: float, ignore_index: int | None, entropy: bool):

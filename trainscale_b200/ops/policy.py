@@ -114,8 +114,11 @@ class _Loss(torch.autograd.Function):
 
 
 def native(logp, *others) -> bool:
-    """Whether the kernels take these log-probabilities: [rows, T], on the current device, with some tokens."""
-    return logp.dim() == 2 and logp.dtype in _DTYPES and logp.numel() > 0 and on_this_gpu(logp, *others)
+    """Whether the kernels take these log-probabilities: [rows, T], on the current device, with some tokens and no more than a launch
+    counts."""
+    shape = logp.shape
+    return (len(shape) == 2 and logp.dtype in _DTYPES and 0 < shape[0] < 1 << 28 and 0 < shape[1] < 1 << 30
+            and on_this_gpu(logp, *others))
 
 
 def _run(op, logp, *constants):
