@@ -198,6 +198,65 @@ def test_constants_made_in_inference_mode():
         token_log_probs(w, y, return_entropy=True)
 
 
+def test_broadcast_inputs():
+    """A row that several sequences share gets the sum of their gradients."""
+    from trainscale_b200.rl import clipped_policy_loss, preference_loss, token_log_probs
+    logp, old, adv, mask, ref = _policy_case(6, 52, torch.float32, torch.bool, 3, spoil=False)
+    one = logp[:1].clone().requires_grad_()
+    clipped_policy_loss(one.expand(6, 52), old, adv, mask, ref, beta=0.1).backward()
+    _, grad, _ = policy_oracle(logp[:1].expand(6, 52), old, adv, mask, ref, 0.2, 0.2, 0.1, "sequence", 52)
+    torch.testing.assert_close(one.grad.double(), grad.sum(0, keepdim=True), rtol=1e-5, atol=1e-8)
+    one = logp[:1].clone().requires_grad_()
+    preference_loss(one.expand(6, 52), ref, mask, loss_type="ipo")[0].backward()
+    *_, grad = preference_oracle(logp[:1].expand(6, 52), ref, mask, 0.1, "ipo", 0.0, 0.0, False, 0.0)
+    torch.testing.assert_close(one.grad.double().cpu(), grad.sum(0, keepdim=True), rtol=1e-5, atol=1e-8)
+    z = torch.randn(1, 1, 99, device=DEV, requires_grad=True)
+    y = torch.arange(12, device=DEV).view(3, 4)
+    token_log_probs(z.expand(3, 4, 99), y).sum().backward()
+    p = torch.softmax(z.detach().double(), -1)
+    torch.testing.assert_close(z.grad.double(), (torch.arange(99, device=DEV) < 12).double() - 12 * p, rtol=1e-4, atol=1e-5)
+
+
+def test_transforms_take_the_pytorch_form():
+    """torch.func and forward-mode derivatives, which cannot see into a kernel."""
+    from trainscale_b200.rl import clipped_policy_loss, preference_loss, token_log_probs
+    logp, old, adv, mask, ref = _policy_case(6, 20, torch.float32, torch.bool, 3, spoil=False)
+    for f in (lambda p: clipped_policy_loss(p, old, adv, mask, ref, beta=0.1), lambda p: preference_loss(p, ref, mask)[0]):
+        x = logp.clone().requires_grad_()
+        f(x).backward()
+        torch.testing.assert_close(torch.func.grad(f)(logp), x.grad, rtol=1e-4, atol=1e-7)
+        _, tangent = torch.func.jvp(f, (logp,), (torch.ones_like(logp),))
+        torch.testing.assert_close(tangent, x.grad.sum(), rtol=1e-4, atol=1e-6)
+    z, y = torch.randn(5, 3, 33, device=DEV), torch.randint(0, 33, (5, 3), device=DEV)
+    torch.testing.assert_close(torch.func.vmap(token_log_probs)(z, y), token_log_probs(z, y), rtol=1e-5, atol=1e-5)
+
+
+def test_two_streams_at_once():
+    """Calls that run side by side have workspaces of their own."""
+    from trainscale_b200.rl import clipped_policy_loss, preference_loss, token_log_probs
+    cases = [(_policy_case(500, 700, torch.float32, torch.bool, i), _pair_case(200, 3000, torch.float32, torch.bool, i),
+              torch.randn(700, 9000, device=DEV, generator=_gen(i))) for i in range(2)]
+    y = torch.randint(0, 9000, (700,), device=DEV)
+
+    def run(case):
+        (logp, old, adv, mask, ref), (lp, rf, m), z = case
+        grads = [z.clone(), lp.nan_to_num(neginf=0.0)]
+        return [*clipped_policy_loss(logp, old, adv, mask, ref, beta=0.1, return_stats=True)[1], *preference_loss(lp, rf, m),
+                *token_log_probs(z, y, return_entropy=True), _clip(grads, 1.0), *grads]
+
+    want = [run(c) for c in cases]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in cases]
+    for _ in range(5):
+        got = []
+        for s, c in zip(streams, cases):
+            with torch.cuda.stream(s):
+                got.append(run(c))
+        torch.cuda.synchronize()
+        for a, b in zip(want, got):
+            assert all(torch.equal(u, v) for u, v in zip(a, b))
+
+
 def test_inputs_changed_before_their_gradient():
     from trainscale_b200.rl import clipped_policy_loss
     logp, old, adv, mask, ref = _policy_case(6, 50, torch.float32, torch.bool, 3, spoil=False)
