@@ -435,6 +435,13 @@ def test_policy_bounds_and_extremes():
     zero = clipped_policy_loss(logp, old, torch.zeros(1, device=DEV), torch.ones(1, 8, device=DEV))
     assert float(zero) == 0                                 # ratios that overflow have no say without an advantage
     assert float(clipped_policy_loss(logp, old, torch.ones(1, device=DEV), torch.zeros(1, 8, device=DEV))) == 0
+    for device in (DEV, "cpu"):                             # a reference that is only looked at, however far away
+        x = torch.zeros(1, 4, device=device, requires_grad=True)
+        far = torch.full((1, 4), 200.0, device=device)
+        loss, stats = clipped_policy_loss(x, torch.zeros(1, 4, device=device), torch.ones(1, device=device), torch.ones(1, 4, device=device),
+                                          far, return_stats=True)
+        loss.backward()
+        assert float(loss) == -1 and (x.grad == -0.25).all() and float(stats.kl) == math.inf
     bad = logp.clone()
     bad[0, 2] = math.nan
     assert clipped_policy_loss(bad, old, torch.zeros(1, device=DEV), torch.ones(1, 8, device=DEV)).isnan()
@@ -542,6 +549,12 @@ def test_preference_loss_of_inputs_that_lie_elsewhere():
 
 def test_far_pairs_do_not_overflow():
     from trainscale_b200.rl import preference_loss
+    for device in (DEV, "cpu"):                             # a rejected token of no probability: nothing is left to learn
+        lp = torch.tensor([[-1.0, -2.0], [-math.inf, -1.0]], device=device, requires_grad=True)
+        for kind in ("sigmoid", "robust", "hinge"):
+            loss, chosen, rejected = preference_loss(lp, None, torch.ones(2, 2, device=device), loss_type=kind)
+            (d,) = torch.autograd.grad(loss, lp)
+            assert float(loss) == 0 and (d == 0).all() and float(rejected) == -math.inf
     lp = torch.tensor([[-3e4, -3e4], [0.0, 0.0]], device=DEV, requires_grad=True)
     for kind in ("sigmoid", "robust", "hinge", "ipo"):
         for order in (lp, lp.flip(0)):

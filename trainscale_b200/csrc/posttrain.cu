@@ -344,8 +344,10 @@ __device__ __forceinline__ void policy_tokens(const Policy& a, long long begin, 
       if (a.ref) {
         float less;
         const float kl = exp_rest(used ? ref[e] - x : 0.f, &less);
-        token += a.beta * kl;
-        slope[e] -= a.beta * less;
+        if (a.beta != 0.f) {             // (0 * inf: a reference that is only looked at has no say)
+          token += a.beta * kl;
+          slope[e] -= a.beta * less;
+        }
         part[1] += m[e] * kl;
       }
       const float mw = m[e] * w[e];
@@ -513,7 +515,7 @@ __device__ __forceinline__ double pair_loss(const Pairs& a, double x, double* sl
   if (a.kind <= 1) {
     const double sign = a.kind == 0 ? 1.0 : -1.0, f = a.kind == 0 ? 1.0 : 1.0 / (1.0 - 2.0 * e);
     *slope = a.beta * f * (sign * e * sigmoid(q) - (1.0 - e) * sigmoid(-q));
-    return f * ((1.0 - e) * softplus(-q) + sign * e * softplus(q));
+    return f * ((1.0 - e) * softplus(-q) + (e != 0.0 ? sign * e * softplus(q) : 0.0));      // (0 * inf: a token of no probability)
   }
   if (a.kind == 2) {
     *slope = q < 1.0 ? -a.beta : (q == q ? 0.0 : q);

@@ -181,7 +181,8 @@ class PolicyLoss:
         if ref_logp is not None:
             d = _masked(ref_logp, used).to(m.dtype) - logp
             kl = torch.expm1(d) - d
-            token = token + self.beta * kl
+            if self.beta:                             # (0 * inf: a reference that is only looked at has no say)
+                token = token + self.beta * kl
         total = m.sum().clamp(min=1)
         if self.reduction == "sequence":
             loss = ((token * m).sum(1) / m.sum(1).clamp(min=1)).sum() / max(1, m.shape[0])
@@ -235,7 +236,8 @@ class PairLoss:
             score = score / count
         x = score[:P] - score[P:]
         q = self.beta * x - self.gamma
-        eps, up, down = self.smoothing, F.softplus(-q, threshold=1e3), F.softplus(q, threshold=1e3)
+        eps, up = self.smoothing, F.softplus(-q, threshold=1e3)
+        down = F.softplus(q, threshold=1e3) if eps else 0.0       # (0 * inf: a token of no probability)
         if self.kind == "sigmoid":
             loss = (1 - eps) * up + eps * down
         elif self.kind == "robust":
