@@ -481,9 +481,17 @@ def test_group_relative_losses_keep_their_results():
     y = logp.clone().requires_grad_()
     (e,) = torch.autograd.grad(pytorch("grpo", y), y, create_graph=True)
     torch.testing.assert_close(dd, torch.autograd.grad(e.sum(), y)[0], rtol=1e-4, atol=1e-8)
-    g = rl.GRPOCompute(group_size=4, beta=0.01)
-    loss, stats = g.compute_grpo_loss(logp.clone().requires_grad_(), ref, torch.randn(16, device=DEV), mask, old)
-    assert set(stats) == {"reward_mean", "reward_std", "advantage_abs_mean", "kl"} and type(loss.grad_fn).__name__ == "_LossBackward"
+    rewards = torch.randn(16, device=DEV, generator=_gen(8))
+    d = ref - logp
+    kl = float(((torch.exp(d) - d - 1) * mask).sum() / mask.sum())
+    for variant in ("grpo", "drgrpo", "dapo"):
+        g = rl.GRPOCompute(group_size=4, beta=0.01, variant=variant)
+        x = logp.clone().requires_grad_()
+        loss, stats = g.compute_grpo_loss(x, ref, rewards, mask, old)
+        assert set(stats) == {"reward_mean", "reward_std", "advantage_abs_mean", "kl"} and type(loss.grad_fn).__name__ == "_LossBackward"
+        assert stats["kl"] == pytest.approx(kl, rel=1e-4)
+        torch.testing.assert_close(loss, g(x, old, ref, rewards, mask), rtol=1e-6, atol=1e-8)
+        assert "kl" not in g.compute_grpo_loss(x, None, rewards, mask, old)[1]
 
 
 # ------------------------------------------------------------------------------------------------ pairs

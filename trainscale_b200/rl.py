@@ -339,13 +339,20 @@ class GRPOCompute:
         if self.reward_clip:
             rewards = rewards.clamp(-self.reward_clip, self.reward_clip)
         old = policy_log_probs.detach() if old_log_probs is None else old_log_probs
-        loss = self(policy_log_probs, old, ref_log_probs, rewards, mask)
         adv = compute_advantages(rewards, self.group_size, scale=self.variant != "drgrpo")
+        kl = None
+        if _takes_policy_kernel(policy_log_probs, old, ref_log_probs, adv, mask) and self.clip >= 0 and self.beta >= 0:
+            kw = {"drgrpo": dict(reduction="constant"), "dapo": dict(reduction="token", clip_high=0.28)}.get(
+                self.variant, dict(beta=self.beta if ref_log_probs is not None else 0.0))
+            loss, seen = clipped_policy_loss(policy_log_probs, old, adv, mask, ref_log_probs, clip=self.clip, return_stats=True, **kw)
+            kl = seen.kl                              # (out of the pass that made the loss)
+        else:
+            loss = self(policy_log_probs, old, ref_log_probs, rewards, mask)
         stats = {"reward_mean": float(rewards.float().mean()), "reward_std": float(rewards.float().std()),
                  "advantage_abs_mean": float(adv.abs().mean())}
         if ref_log_probs is not None:
-            d = (ref_log_probs - policy_log_probs).detach()
-            stats["kl"] = float(_masked_mean(torch.exp(d) - d - 1, mask))
+            d = (ref_log_probs - policy_log_probs).detach() if kl is None else None
+            stats["kl"] = float(_masked_mean(torch.exp(d) - d - 1, mask) if kl is None else kl)
         return loss, stats
 
     def __call__(self, logp, old_logp, ref_logp, rewards, mask):
