@@ -186,6 +186,8 @@ __device__ __forceinline__ void block_sums(double* v, double (*scratch)[N]) {
 constexpr int POLICY_PER_SM = 4;         // blocks of an SM
 constexpr int POLICY_SUMS = 5;           // loss, kl m, clipped m, ratio m, m
 constexpr int POLICY_SPLIT = 8;          // most blocks that count a row
+// Tokens of a row that a warp counts (by warps and by blocks: 4096 x 128 12.6 and 18.3 us a call, 512 x 1024 12.1 and 12.9).
+constexpr int POLICY_SHORT = 1024;
 // Tokens that one block takes by itself, in one launch (8 x 64: 5.4 us, in two launches 7.8; 8 x 1024: 8.9 and 9.0; 16 x 1024:
 // 13.1 and 8.1).
 constexpr int POLICY_ALONE = 8192;
@@ -228,12 +230,12 @@ struct Place {
   __device__ __forceinline__ long long in(long long stride) const { return row * stride + t; }
 };
 
-// Sum of the mask's values [begin, end) by a block, four vectors of a thread in flight.
+// A thread's part of the sum of the mask's values [begin, end), one of `threads`; four vectors in flight.
 template <typename M, int VEC>
-__device__ __forceinline__ double sum_values(const M* p, long long begin, long long end) {
-  const long long width = static_cast<long long>(blockDim.x) * VEC;
+__device__ __forceinline__ double sum_values(const M* p, long long begin, long long end, int thread, int threads) {
+  const long long width = static_cast<long long>(threads) * VEC;
   double n = 0.0;
-  for (long long i = begin + static_cast<long long>(threadIdx.x) * VEC; i < end; i += 4 * width) {
+  for (long long i = begin + static_cast<long long>(thread) * VEC; i < end; i += 4 * width) {
     float m[4][VEC], s = 0.f;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -252,22 +254,22 @@ __device__ __forceinline__ double sum_values(const M* p, long long begin, long l
 
 // Sum of the mask over tokens [begin, end), which lie in one row or are `flat`.
 template <int VEC>
-__device__ __forceinline__ double mask_run(const Policy& a, long long begin, long long end) {
+__device__ __forceinline__ double mask_run(const Policy& a, long long begin, long long end, int thread, int threads) {
   const long long at = a.flat ? 0 : begin / a.T * (a.mask.stride - a.T);
   switch (a.mask.kind) {
-    case 0: return sum_values<unsigned char, VEC>(static_cast<const unsigned char*>(a.mask.p) + at, begin, end);
-    case 1: return sum_values<int, VEC>(static_cast<const int*>(a.mask.p) + at, begin, end);
-    case 2: return sum_values<long long, VEC>(static_cast<const long long*>(a.mask.p) + at, begin, end);
-    case 3: return sum_values<float, VEC>(static_cast<const float*>(a.mask.p) + at, begin, end);
-    case 4: return sum_values<__nv_bfloat16, VEC>(static_cast<const __nv_bfloat16*>(a.mask.p) + at, begin, end);
-    default: return sum_values<__half, VEC>(static_cast<const __half*>(a.mask.p) + at, begin, end);
+    case 0: return sum_values<unsigned char, VEC>(static_cast<const unsigned char*>(a.mask.p) + at, begin, end, thread, threads);
+    case 1: return sum_values<int, VEC>(static_cast<const int*>(a.mask.p) + at, begin, end, thread, threads);
+    case 2: return sum_values<long long, VEC>(static_cast<const long long*>(a.mask.p) + at, begin, end, thread, threads);
+    case 3: return sum_values<float, VEC>(static_cast<const float*>(a.mask.p) + at, begin, end, thread, threads);
+    case 4: return sum_values<__nv_bfloat16, VEC>(static_cast<const __nv_bfloat16*>(a.mask.p) + at, begin, end, thread, threads);
+    default: return sum_values<__half, VEC>(static_cast<const __half*>(a.mask.p) + at, begin, end, thread, threads);
   }
 }
 
 // The same of any tokens.
 template <int VEC>
 __device__ __forceinline__ double mask_sum(const Policy& a, long long begin, long long end) {
-  if (a.flat) return mask_run<VEC>(a, begin, end);
+  if (a.flat) return mask_run<VEC>(a, begin, end, threadIdx.x, blockDim.x);
   const int width = static_cast<int>(blockDim.x) * VEC;
   long long i = begin + static_cast<long long>(threadIdx.x) * VEC;
   double n = 0.0;
@@ -369,7 +371,7 @@ __device__ __forceinline__ void policy_results(const double* sums, float* loss, 
     for (int k = 1; k < 4; ++k) stats[k - 1] = static_cast<float>(sums[k] / fmax(sums[4], 1.0));
 }
 
-// What the tokens weigh: weights [rows] (reduction 0, a block or a cluster per row), sums of the mask by block (reduction 1); and
+// What the tokens weigh: weights [rows] (reduction 0, a warp, a block or a cluster per row), sums of the mask by block (reduction 1); and
 // the counter that tells the next kernel's last block.
 template <int VEC>
 __global__ void __launch_bounds__(PT_THREADS) policy_count_kernel(Policy a, float* __restrict__ weights, double* __restrict__ counts,
@@ -387,11 +389,23 @@ __global__ void __launch_bounds__(PT_THREADS) policy_count_kernel(Policy a, floa
     if (threadIdx.x == 0) counts[blockIdx.x] = n[0];
     return;
   }
+  // (a row that starts between vectors is counted token by token)
+  const bool vectors = a.T % VEC == 0;
+  auto weight = [&](double n) { return static_cast<float>(1.0 / (fmax(n, 1.0) * static_cast<double>(a.rows))); };
+  if (a.T <= POLICY_SHORT) {
+    const long long row = blockIdx.x * static_cast<long long>(PT_THREADS / 32) + (threadIdx.x >> 5);
+    if (row >= a.rows) return;
+    const int lane = threadIdx.x & 31;
+    double n = vectors ? mask_run<VEC>(a, row * a.T, (row + 1) * a.T, lane, 32) : mask_run<1>(a, row * a.T, (row + 1) * a.T, lane, 32);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
+    if (lane == 0) weights[row] = weight(n);
+    return;
+  }
   if (parts > 1) cluster.barrier_arrive();      // (no block writes to another's shared memory before that one has begun)
   const long long row = blockIdx.x / parts, part = (a.T / VEC + parts - 1) / parts * VEC;
   const long long begin = row * a.T + rank * part, end = rank == parts - 1 ? (row + 1) * a.T : min((row + 1) * a.T, begin + part);
-  // (a row that starts between vectors is counted token by token)
-  double n[1] = {(row * a.T | a.T) % VEC == 0 ? mask_run<VEC>(a, begin, end) : mask_run<1>(a, begin, end)};
+  double n[1] = {vectors ? mask_run<VEC>(a, begin, end, threadIdx.x, PT_THREADS) : mask_run<1>(a, begin, end, threadIdx.x, PT_THREADS)};
   block_sums<1>(n, scratch);
   if (parts > 1) {
     cluster.barrier_wait();
@@ -401,7 +415,7 @@ __global__ void __launch_bounds__(PT_THREADS) policy_count_kernel(Policy a, floa
     n[0] = 0.0;
     for (int i = 0; i < parts; ++i) n[0] += by_block[i];
   }
-  if (threadIdx.x == 0) weights[row] = static_cast<float>(1.0 / (fmax(n[0], 1.0) * static_cast<double>(a.rows)));
+  if (threadIdx.x == 0) weights[row] = weight(n[0]);
 }
 
 template <typename T, int VEC, bool FLAT>
@@ -729,7 +743,9 @@ extern "C" int ts_policy_loss(const PolicyCall* c, void* stream) {
       int parts = 1;
       if (a.reduction == 0)
         while (parts < POLICY_SPLIT && a.rows * parts < 2 * sm_count() && a.T / parts >= 8 * PT_THREADS * VEC) parts *= 2;
-      const unsigned counters = a.reduction == 0 ? static_cast<unsigned>(a.rows * parts) : a.reduction == 1 ? used : 1;
+      constexpr int warps = PT_THREADS / 32;
+      const unsigned by_row = static_cast<unsigned>(a.T <= POLICY_SHORT ? (a.rows + warps - 1) / warps : a.rows * parts);
+      const unsigned counters = a.reduction == 0 ? by_row : a.reduction == 1 ? used : 1;
       const int rc = launch_chained(policy_count_kernel<VEC>, dim3(counters), dim3(PT_THREADS), 0, st, parts, false, a, weights, counts,
                                     ticket, up);
       if (rc) return rc;
