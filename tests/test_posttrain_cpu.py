@@ -144,3 +144,18 @@ def test_clipping_on_the_cpu_is_as_before():
     assert float(clip_grad_norm_(ps, 1.0)) == pytest.approx(math.sqrt(28))
     assert float(ps[0].grad[0]) == pytest.approx(2 / math.sqrt(28), rel=1e-5)
     assert float(clip_grad_norm_([torch.nn.Parameter(torch.zeros(1))], 1.0)) == 0
+
+
+def test_labels_of_the_fused_head():
+    """What the row kernels read: dense int64 labels, one for every row at least, where the rows are."""
+    from trainscale_b200.ops.cross_entropy import _dense_labels
+    ids = torch.arange(8).view(4, 2)
+    cpu = torch.device("cpu")
+    for labels in (ids[:, 1:], ids[:, 1], ids[:, 1].int(), ids[:, 1:].unsqueeze(0)):
+        got = _dense_labels(labels, 4, cpu)
+        assert got.is_contiguous() and got.dtype == torch.int64 and got.tolist() == [1, 3, 5, 7]
+    same = torch.arange(4)
+    assert _dense_labels(same, 4, cpu).data_ptr() == same.data_ptr()
+    for labels, device in ((torch.arange(3), cpu), (torch.arange(4, device="meta"), cpu)):
+        with pytest.raises(ValueError, match="labels"):
+            _dense_labels(labels, 4, device)

@@ -317,6 +317,28 @@ def test_log_probs_of_the_fused_head(T, V, chunk):
         assert torch.equal(logp, fused_linear_token_logprobs(h, w, y, chunk_tokens=chunk))
 
 
+@pytest.mark.parametrize("case", ["every other", "column", "int32 column"])
+def test_fused_head_reads_labels_that_lie_apart(case):
+    """Labels of a tensor that can be viewed as one dimension and keeps a stride: log-probabilities, losses and their gradients."""
+    from trainscale_b200.ops import cross_entropy as ce
+    h = torch.randn(6, 128, device=DEV, generator=_gen(1)).bfloat16()
+    w = (torch.randn(40, 128, device=DEV, generator=_gen(2)) * 0.3).bfloat16()
+    ids = torch.randint(0, 40, (6, 2), device=DEV, generator=_gen(3))
+    y = {"every other": ids.view(-1)[::2], "column": ids[:, 1:], "int32 column": ids.int()[:, 1:]}[case]
+    assert not y.reshape(-1).is_contiguous()
+    z = torch.randn(6, 40, device=DEV, generator=_gen(4)).bfloat16()
+    calls = (lambda h, y: ce.fused_linear_token_logprobs(h, w, y).sum(), lambda h, y: ce.fused_linear_cross_entropy(h, w, y)[0],
+             lambda h, y: ce.cross_entropy_rows(z + 0 * h[:, :40], y).sum(),
+             lambda h, y: ce.focal_loss_rows(z + 0 * h[:, :40], y.reshape(-1)).sum(), lambda h, y: ce.cross_entropy_logits(z, y)[0].sum() + 0 * h.sum())
+    for call in calls:
+        out = []
+        for labels in (y, y.long().clone(memory_format=torch.contiguous_format)):
+            x = h.clone().requires_grad_()
+            loss = call(x, labels)
+            out.append((loss.detach(), *torch.autograd.grad(loss, x)))
+        assert all(torch.equal(u, v) for u, v in zip(*out))
+
+
 def test_selective_log_softmax_keeps_its_results():
     from trainscale_b200.rl import selective_log_softmax
     y = torch.randint(0, 999, (4, 5), device=DEV)

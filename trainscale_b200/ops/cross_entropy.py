@@ -22,6 +22,14 @@ from .gemm import matmul_nn, matmul_nt, matmul_tn
 DEFAULT_CHUNK_TOKENS = 4096
 
 
+def _dense_labels(labels: torch.Tensor, rows: int, device: torch.device) -> torch.Tensor:
+    """The labels of `rows` rows as the kernels read them: int64, one after the other (a column of a matrix can be viewed as one
+    dimension and keeps its stride), on the rows' device."""
+    if labels.device != device or labels.numel() < rows:
+        raise ValueError(f"{labels.numel()} labels on {labels.device} for {rows} rows on {device}")
+    return labels.reshape(-1).to(torch.int64).contiguous()
+
+
 def _ce_rows(logits, labels, loss, lse, ignore_index, label_smoothing, logit_scale, softcap, gscale_ptr, gscale_mul,
              row_gscale, write_grad):
     lib = _lib.load("elementwise")
@@ -40,6 +48,7 @@ def cross_entropy_logits(logits: torch.Tensor, labels: torch.Tensor, ignore_inde
     rows = logits.shape[0]
     loss = torch.empty(rows, dtype=torch.float32, device=logits.device)
     lse = torch.empty(rows, dtype=torch.float32, device=logits.device)
+    labels = _dense_labels(labels, rows, logits.device)
     _ce_rows(logits, labels, loss, lse, ignore_index, label_smoothing, logit_scale, softcap, None, 1.0, None, False)
     return loss, lse
 
@@ -59,6 +68,7 @@ class _FocalLossFn(torch.autograd.Function):
             pad = torch.zeros(rows, _pad_ld(lg.shape[1]), dtype=lg.dtype, device=lg.device)
             pad[:, :lg.shape[1]] = lg
             lg = pad[:, :logits.shape[1]]
+        labels = _dense_labels(labels, rows, logits.device)
         _ce_rows(lg, labels, loss, lse, ignore_index, 0.0, 1.0, 0.0, None, 1.0, None, False)
         p = torch.exp(-loss)
         valid = labels != ignore_index
@@ -94,7 +104,7 @@ class FusedCrossEntropyFunction(torch.autograd.Function):
             pad = torch.zeros(rows, _pad_ld(lg.shape[1]), dtype=lg.dtype, device=lg.device)
             pad[:, :lg.shape[1]] = lg
             lg = pad[:, :logits.shape[1]]
-        labels = labels.reshape(-1).to(torch.int64)
+        labels = _dense_labels(labels, rows, logits.device)
         loss = torch.empty(rows, dtype=torch.float32, device=lg.device)
         lse = torch.empty(rows, dtype=torch.float32, device=lg.device)
         _ce_rows(lg, labels, loss, lse, ignore_index, label_smoothing, 1.0, 0.0, None, 1.0, None, False)
@@ -143,7 +153,7 @@ class _FusedLinearCE(torch.autograd.Function):
         T, H = hidden.shape
         V = weight.shape[0]
         dev = hidden.device
-        labels = labels.reshape(-1).to(torch.int64)
+        labels = _dense_labels(labels, T, hidden.device)
         valid = (labels != ignore_index)
         count = valid.sum().clamp(min=1).to(torch.float32)
         if reduction == "mean":
@@ -245,7 +255,7 @@ class _FusedLinearLogProb(torch.autograd.Function):
     def forward(ctx, hidden, weight, labels, ignore_index, chunk_tokens):
         T, H = hidden.shape
         V = weight.shape[0]
-        labels = labels.reshape(-1).to(torch.int64)
+        labels = _dense_labels(labels, T, hidden.device)
         chunk = min(chunk_tokens, T)
         buf = torch.empty(chunk, _pad_ld(V), dtype=torch.bfloat16, device=hidden.device)
         logp = torch.empty(T, dtype=torch.float32, device=hidden.device)
