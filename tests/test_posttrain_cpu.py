@@ -159,3 +159,28 @@ def test_labels_of_the_fused_head():
     for labels, device in ((torch.arange(3), cpu), (torch.arange(4, device="meta"), cpu)):
         with pytest.raises(ValueError, match="labels"):
             _dense_labels(labels, 4, device)
+
+
+def test_operations_that_are_recorded_or_transformed():
+    """Where a kernel called by address would leave nothing behind: traces, modes, transforms, compiled functions."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    from torch.utils.flop_counter import FlopCounterMode
+    from trainscale_b200.ops import _lib
+    seen, x = [], torch.ones(3)
+
+    def f(x):
+        seen.append(_lib.eager())
+        return x + 1
+
+    assert f(x) is not None and seen.pop()
+    torch.jit.trace(f, x, check_trace=False)
+    make_fx(f)(x)
+    make_fx(f, tracing_mode="fake")(x)
+    torch.func.vmap(f)(x)
+    torch.func.grad(lambda x: f(x).sum())(x)
+    torch.func.jvp(f, (x,), (x,))
+    with FlopCounterMode(display=False):
+        f(x)
+    assert seen == [False] * 7
+    g = torch.compile(lambda x: x + (1 if _lib.eager() else 2), backend="eager", fullgraph=True)
+    assert torch.equal(g(x), x + 2) and _lib.eager()

@@ -231,6 +231,55 @@ def test_transforms_take_the_pytorch_form():
     torch.testing.assert_close(torch.func.vmap(token_log_probs)(z, y), token_log_probs(z, y), rtol=1e-5, atol=1e-5)
 
 
+def _recorded_calls():
+    """(name, function of one tensor, its argument) of everything that has PyTorch operations to record."""
+    from trainscale_b200 import rl
+    from trainscale_b200.optim import clip_grad_norm_
+    from trainscale_b200.parallel.dist_utils import fused_clip_grad_norm_
+    logp, old, adv, mask, ref = _policy_case(6, 52, torch.float32, torch.float32, 3, spoil=False)
+    y = torch.randint(0, 33, (5,), device=DEV, generator=_gen(1))
+    z = torch.randn(5, 33, device=DEV, generator=_gen(2))
+
+    def clipped(clip):
+        def f(g):
+            p = torch.nn.Parameter(torch.zeros_like(g))
+            p.grad = g.clone()
+            return clip([p], 0.5), p.grad
+        return f
+
+    return [("selective_log_softmax", lambda z: rl.selective_log_softmax(z, y), z), ("token_log_probs", lambda z: rl.token_log_probs(z, y), z),
+            ("grpo", lambda x: rl.grpo_loss(x, old, ref, adv, mask), logp), ("drgrpo", lambda x: rl.drgrpo_loss(x, old, adv, mask), logp),
+            ("dapo", lambda x: rl.dapo_loss(x, old, adv, mask), logp), ("pairs", lambda x: rl.preference_loss(x, ref, mask)[0], logp),
+            ("clip", clipped(clip_grad_norm_), logp), ("fused clip", clipped(fused_clip_grad_norm_), logp)]
+
+
+@pytest.mark.parametrize("how", ["jit.trace", "make_fx", "compile"])
+def test_recorded_calls_replay(how):
+    """A recording holds the operations, not the memory that a kernel once filled."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    for name, f, x in _recorded_calls():
+        if how == "compile" and "clip" in name:
+            continue                                        # (a parameter made inside: not for fullgraph)
+        recorded = {"jit.trace": lambda: torch.jit.trace(f, x, check_trace=False), "make_fx": lambda: make_fx(f)(x),
+                    "compile": lambda: torch.compile(f, backend="eager", fullgraph=True)}[how]()
+        other = x * 0.5 + 0.1
+        for a, b in zip(*[(t if isinstance(t, tuple) else (t,)) for t in (recorded(other), f(other))]):
+            torch.testing.assert_close(a, b, rtol=1e-4, atol=1e-6, msg=lambda m: f"{name}: {m}")
+
+
+def test_recorded_gradients_replay():
+    """The gradient of a loss that a kernel has computed, recorded as a function of what flows into it."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    for name, f, x in _recorded_calls()[:6]:
+        x = x.clone().requires_grad_()
+        out = f(x)
+        assert type(out.grad_fn).__name__ in ("_LossBackward", "_TokenLogProbsBackward"), name
+        grad = lambda g: torch.autograd.grad(out, x, g, retain_graph=True)[0]       # noqa: E731, B023
+        recorded = make_fx(grad)(torch.ones_like(out))
+        g = torch.rand_like(out)
+        torch.testing.assert_close(recorded(g), grad(g), rtol=1e-4, atol=1e-7, msg=lambda m: f"{name}: {m}")
+
+
 def test_two_streams_at_once():
     """Calls that run side by side have workspaces of their own."""
     from trainscale_b200.rl import clipped_policy_loss, preference_loss, token_log_probs

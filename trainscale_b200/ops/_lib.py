@@ -62,6 +62,14 @@ def ptr(t: torch.Tensor | None) -> ctypes.c_void_p:
     return ctypes.c_void_p(t.data_ptr())
 
 
+def eager() -> bool:
+    """Whether operations only run now.  Kernels called by address are invisible to whatever records operations (torch.jit.trace,
+    make_fx, torch.compile), handles them itself (dispatch modes) or derives others from them (functorch transforms, forward-mode
+    differentiation): those get PyTorch operations."""
+    return not (torch.compiler.is_compiling() or torch._C._is_tracing() or torch._C._len_torch_dispatch_stack()
+                or torch._C._are_functorch_transforms_active() or torch.autograd.forward_ad._current_level >= 0)
+
+
 def check(rc: int, what: str) -> None:
     if rc != 0:
         raise KernelError(f"{what} failed with code {rc}")

@@ -20,11 +20,13 @@ _NEVER = -(1 << 63)                              # no label: nothing is ignored
 
 
 def on_this_gpu(*tensors) -> bool:
-    """Plain CUDA tensors of the current device (or None), outside functorch transforms and forward-mode differentiation."""
+    """Plain CUDA tensors of the current device (or None), while operations only run (`_lib.eager`)."""
+    if not _lib.eager():
+        return False
     for t in tensors:
         if t is not None and (type(t) not in _PLAIN or not t.is_cuda or t.get_device() != torch._C._cuda_getDevice()):
             return False
-    return not torch._C._are_functorch_transforms_active() and torch.autograd.forward_ad._current_level < 0
+    return True
 
 
 def native(logits: torch.Tensor, labels: torch.Tensor) -> bool:
@@ -120,6 +122,17 @@ def rows_backward_(logits: torch.Tensor, labels: torch.Tensor, kept: torch.Tenso
     _run_backward(logits, (n, n, 0, pitch), labels, kept, g, None, logits, pitch, ignore_index=ignore_index, lenient=True)
 
 
+def gradient(form, x: torch.Tensor, upstream) -> torch.Tensor:
+    """The gradient in `x` of results of PyTorch operations, form(x), where some of `upstream` flows into them: for a backward pass
+    that is recorded or transformed, or that will be differentiated itself."""
+    again = torch.is_grad_enabled()
+    with torch.enable_grad():
+        x = x if again else x.detach().requires_grad_()
+        out = form(x)
+        pairs = [(o, d) for o, d in zip(out if isinstance(out, tuple) else (out,), upstream) if d is not None]
+        return torch.autograd.grad([o for o, _ in pairs], x, [d for _, d in pairs], create_graph=again)[0]
+
+
 class _TokenLogProbs(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, labels, how, entropy):
@@ -134,11 +147,8 @@ class _TokenLogProbs(torch.autograd.Function):
         logits, labels, kept = ctx.saved_tensors
         if g is None and h is None:
             return None, None, None, None
-        if torch.is_grad_enabled():                      # this gradient will be differentiated itself
-            out = plain(logits, labels, *ctx.how, ctx.entropy)
-            pairs = [(o, d) for o, d in zip(out if ctx.entropy else (out,), (g, h)) if d is not None]
-            (grad,) = torch.autograd.grad([o for o, _ in pairs], logits, [d for _, d in pairs], create_graph=True)
-            return grad, None, None, None
+        if torch.is_grad_enabled() or not _lib.eager():
+            return gradient(lambda x: plain(x, labels, *ctx.how, ctx.entropy), logits, (g, h)), None, None, None
         x, rows = _rows(logits)
         grad = torch.empty_like(logits, memory_format=torch.contiguous_format)
         g, h = (None if d is None else d.float().contiguous() for d in (g, h))

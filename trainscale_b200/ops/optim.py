@@ -114,7 +114,7 @@ def _gradnorm():
 
 class GradList:
     """Gradients as the kernels take them.  `GradList.of` gives None where they do not: other types or devices, gradients that are
-    not dense in memory, norms other than 1, 2 and inf."""
+    not dense in memory, norms other than 1, 2 and inf, operations that are recorded or transformed (`_lib.eager`)."""
 
     def __init__(self, grads: list, codes: bytes):
         self.grads, self.codes = grads, codes
@@ -125,7 +125,7 @@ class GradList:
     @staticmethod
     def of(grads: list, norm_type) -> "GradList | None":
         # (each check is one C-level pass over the list: a loop in Python costs more than the kernels of a short list)
-        if norm_type not in _NORMS or set(map(type, grads)) != {torch.Tensor}:
+        if not _lib.eager() or norm_type not in _NORMS or set(map(type, grads)) != {torch.Tensor}:
             return None
         if not grads[0].is_cuda or set(map(torch.Tensor.get_device, grads)) != {torch._C._cuda_getDevice()}:
             return None

@@ -16,7 +16,7 @@ import torch
 import torch.nn.functional as F
 
 from . import _lib
-from .logprob import _DTYPES, _address, _stream, fp32, on_this_gpu
+from .logprob import _DTYPES, _address, _stream, fp32, gradient, on_this_gpu
 
 _MASKS = {torch.bool: 0, torch.uint8: 0, torch.int32: 1, torch.int64: 2, torch.float32: 3, torch.bfloat16: 4, torch.float16: 5}
 REDUCTIONS = {"sequence": 0, "token": 1, "constant": 2}
@@ -98,17 +98,17 @@ class _Loss(torch.autograd.Function):
         none = (None,) * (1 + len(constants))
         if g is None:
             return None, *none
-        again = torch.is_grad_enabled()               # this gradient will be differentiated itself
+        kernel = not torch.is_grad_enabled() and _lib.eager()       # (else this gradient is differentiated or recorded itself)
         grad, ctx.grad = ctx.grad, None
         if ctx.captured != torch._C._cuda_isCurrentStreamCapturing():
             grad = None
-        if grad is not None and grad.dtype is torch.float32 and not again:
+        if grad is not None and grad.dtype is torch.float32 and kernel:
             _lib.check(_library().ts_scale_by(grad.data_ptr(), g.data_ptr(), grad.numel(), _stream()), "ts_scale_by")
         else:
             if _changed(constants) != ctx.versions:
                 raise RuntimeError("an input of a policy or preference loss was changed in place before its gradient was computed")
-            if again:
-                return torch.autograd.grad(ctx.op.plain(logp, *constants)[0], logp, g, create_graph=True)[0], *none
+            if not kernel:
+                return gradient(lambda x: ctx.op.plain(x, *constants)[0], logp, (g,)), *none
             grad = ctx.op(logp, *constants, grad=True if grad is None else grad, factor=g)[2]
         return grad if grad.dtype is logp.dtype else grad.to(logp.dtype), *none
 
