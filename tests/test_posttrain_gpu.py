@@ -280,6 +280,26 @@ def test_recorded_gradients_replay():
         torch.testing.assert_close(recorded(g), grad(g), rtol=1e-4, atol=1e-7, msg=lambda m: f"{name}: {m}")
 
 
+def test_batched_gradients():
+    """Several upstream gradients in one backward pass, and Jacobians made of them."""
+    from trainscale_b200 import rl
+    for name, f, x in _recorded_calls()[:6]:
+        x = x.clone().requires_grad_()
+        out = f(x)
+        many = torch.randn(4, *out.shape, device=DEV, generator=_gen(9))
+        (got,) = torch.autograd.grad(out, x, many, is_grads_batched=True, retain_graph=True)
+        want = torch.stack([torch.autograd.grad(out, x, g, retain_graph=True)[0] for g in many])
+        torch.testing.assert_close(got, want, rtol=1e-4, atol=1e-7, msg=lambda m: f"{name}: {m}")
+        torch.testing.assert_close(torch.autograd.functional.jacobian(f, x, vectorize=True), torch.autograd.functional.jacobian(f, x),
+                                   rtol=1e-4, atol=1e-7, msg=lambda m: f"{name}: {m}")
+    z, y = torch.randn(4, 9, device=DEV, requires_grad=True), torch.arange(4, device=DEV)
+    _, H = rl.token_log_probs(z, y, return_entropy=True)
+    many = torch.randn(3, 4, device=DEV)
+    (got,) = torch.autograd.grad(H, z, many, is_grads_batched=True, retain_graph=True)
+    for g, d in zip(many, got):
+        torch.testing.assert_close(d, torch.autograd.grad(H, z, g, retain_graph=True)[0], rtol=1e-4, atol=1e-6)
+
+
 def test_two_streams_at_once():
     """Calls that run side by side have workspaces of their own."""
     from trainscale_b200.rl import clipped_policy_loss, preference_loss, token_log_probs

@@ -122,9 +122,15 @@ def rows_backward_(logits: torch.Tensor, labels: torch.Tensor, kept: torch.Tenso
     _run_backward(logits, (n, n, 0, pitch), labels, kept, g, None, logits, pitch, ignore_index=ignore_index, lenient=True)
 
 
+def batched(*grads) -> bool:
+    """Whether autograd runs one backward pass for several upstream gradients (is_grads_batched, jacobian(vectorize=True))."""
+    f = torch._C._functorch
+    return any(d is not None and (f.is_legacy_batchedtensor(d) or f.is_batchedtensor(d)) for d in grads)
+
+
 def gradient(form, x: torch.Tensor, upstream) -> torch.Tensor:
     """The gradient in `x` of results of PyTorch operations, form(x), where some of `upstream` flows into them: for a backward pass
-    that is recorded or transformed, or that will be differentiated itself."""
+    that is recorded or transformed, runs for several gradients at once, or will be differentiated itself."""
     again = torch.is_grad_enabled()
     with torch.enable_grad():
         x = x if again else x.detach().requires_grad_()
@@ -147,7 +153,7 @@ class _TokenLogProbs(torch.autograd.Function):
         logits, labels, kept = ctx.saved_tensors
         if g is None and h is None:
             return None, None, None, None
-        if torch.is_grad_enabled() or not _lib.eager():
+        if torch.is_grad_enabled() or not _lib.eager() or batched(g, h):
             return gradient(lambda x: plain(x, labels, *ctx.how, ctx.entropy), logits, (g, h)), None, None, None
         x, rows = _rows(logits)
         grad = torch.empty_like(logits, memory_format=torch.contiguous_format)
