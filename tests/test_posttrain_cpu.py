@@ -184,3 +184,41 @@ def test_operations_that_are_recorded_or_transformed():
     assert seen == [False] * 7
     g = torch.compile(lambda x: x + (1 if _lib.eager() else 2), backend="eager", fullgraph=True)
     assert torch.equal(g(x), x + 2) and _lib.eager()
+
+
+def test_preference_trainer_asks_the_loss_that_it_holds():
+    """The pair kernel stands for the losses that the trainer makes itself, and for nothing that a user put in their place."""
+    from trainscale_b200 import rl
+    from trainscale_b200.losses import CPOLoss, DPOLoss, SimPOLoss
+
+    def trainer(kind, **kw):
+        return rl.PreferenceTrainer(None, None, None, kind, **kw)
+
+    assert trainer("dpo")._pair_kernel() == dict(loss_type="sigmoid", label_smoothing=0.0, beta=0.1)
+    assert trainer("simpo", gamma=0.4)._pair_kernel() == dict(label_smoothing=0.0, gamma=0.4, length_normalized=True, beta=0.1)
+    assert trainer("cpo", alpha=0.5)._pair_kernel() == dict(label_smoothing=0.0, nll_weight=0.5, beta=0.1)
+    for kind, base in (("dpo", DPOLoss), ("simpo", SimPOLoss), ("cpo", CPOLoss)):
+        class Own(base):
+            def forward(self, *args):
+                return super().forward(*args)
+
+        for change in (lambda t: setattr(t, "loss_fn", Own()), lambda t: setattr(t, "loss_fn", torch.nn.MSELoss()),
+                       lambda t: t.loss_fn.register_forward_hook(lambda *a: None),
+                       lambda t: t.loss_fn.register_forward_pre_hook(lambda *a: None),
+                       lambda t: t.loss_fn.register_full_backward_hook(lambda *a: None),
+                       lambda t: setattr(t.loss_fn, "forward", lambda *a: None),
+                       lambda t: setattr(t.loss_fn, "beta", torch.nn.Parameter(torch.tensor(0.1))),
+                       lambda t: setattr(t.loss_fn, "beta", math.inf)):
+            t = trainer(kind)
+            assert t._pair_kernel() is not None
+            change(t)
+            assert t._pair_kernel() is None
+        t = trainer(kind)
+        handle = torch.nn.modules.module.register_module_forward_hook(lambda *a: None)
+        try:
+            assert t._pair_kernel() is None
+        finally:
+            handle.remove()
+    t = trainer("dpo")
+    t.loss_fn = lambda *a: None                             # no module at all
+    assert t._pair_kernel() is None

@@ -702,6 +702,30 @@ def test_preference_trainer_goes_through_the_kernel(kind, kw, monkeypatch):
         assert float((u - v).norm()) <= 2e-2 * float(v.norm()) + 1e-6       # bf16 weight gradients of two fp32 roundings apart
 
 
+def test_preference_trainer_calls_a_loss_of_its_users_own():
+    from trainscale_b200.data.synthetic import synthetic_preference_dataloader
+    from trainscale_b200.losses import DPOLoss
+    from trainscale_b200.models.llama import build_model
+    from trainscale_b200.rl import PreferenceTrainer
+    torch.manual_seed(0)
+    model = build_model("tiny", dtype=torch.bfloat16, device=DEV)
+    t = PreferenceTrainer(model, None, PreferenceTrainer.make_reference(model), "dpo", 0.3)
+    batch = {k: v.to(DEV) for k, v in next(iter(synthetic_preference_dataloader(32000, 20, 40, 4))).items()}
+    plain = float(t.compute_loss(batch)[0].detach())
+
+    class Twice(DPOLoss):
+        def forward(self, *args):
+            loss, *rest = super().forward(*args)
+            return 2 * loss, *rest
+
+    t.loss_fn = Twice(0.3)
+    assert float(t.compute_loss(batch)[0].detach()) == pytest.approx(2 * plain, rel=1e-4)
+    t.loss_fn, seen = DPOLoss(0.3), []
+    t.loss_fn.register_forward_hook(lambda *a: seen.append(1))
+    t.compute_loss(batch)
+    assert seen == [1]
+
+
 # ------------------------------------------------------------------------------------------------ gradient clipping
 def _clip(grads, limit, kind=2.0, **kw):
     from trainscale_b200.optim import clip_grad_norm_

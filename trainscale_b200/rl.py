@@ -20,6 +20,7 @@ from typing import Any, Dict
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
+from torch.nn.modules.module import _has_any_global_hook
 
 from .losses import CPOLoss, DPOLoss, KTOLoss, ORPOLoss, SimPOLoss
 from .ops import cross_entropy as ce_ops
@@ -437,8 +438,13 @@ class PreferenceTrainer:
         return lp.sum(-1), valid.sum(-1)
 
     def _pair_kernel(self) -> dict | None:
-        """The loss as arguments of `preference_loss`; None for those that are not a function of one pair's scores."""
+        """The loss as arguments of `preference_loss`; None for those that are not a function of one pair's scores, and for a loss module
+        that is not just what the constructor makes: a subclass, another module, one with hooks, a replaced forward or a learned beta."""
         f, kind = self.loss_fn, self.kind
+        if type(f) is not {"dpo": DPOLoss, "simpo": SimPOLoss, "cpo": CPOLoss}.get(kind) or (
+                "forward" in f.__dict__ or f._forward_hooks or f._forward_pre_hooks or f._backward_hooks or f._backward_pre_hooks
+                or _has_any_global_hook()):
+            return None
         if kind == "dpo" and f.loss_type in policy_ops.KINDS and (f.loss_type != "robust" or f.label_smoothing < 0.5):
             kw = dict(loss_type=f.loss_type, label_smoothing=f.label_smoothing if f.loss_type in ("sigmoid", "robust") else 0.0)
         elif kind == "simpo":
@@ -447,7 +453,11 @@ class PreferenceTrainer:
             kw = dict(label_smoothing=f.eps, nll_weight=f.alpha)
         else:
             return None
-        return dict(kw, beta=f.beta) if f.beta > 0 and 0 <= kw["label_smoothing"] <= 1 else None
+        kw["beta"] = f.beta
+        numbers = [v for k, v in kw.items() if k not in ("loss_type", "length_normalized")]
+        if not all(isinstance(v, (int, float)) and math.isfinite(v) for v in numbers):
+            return None
+        return kw if f.beta > 0 and 0 <= kw["label_smoothing"] <= 1 else None
 
     def compute_loss(self, batch: Dict[str, torch.Tensor]):
         B = batch["chosen_input_ids"].shape[0]
