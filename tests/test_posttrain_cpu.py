@@ -222,3 +222,23 @@ def test_preference_trainer_asks_the_loss_that_it_holds():
     t = trainer("dpo")
     t.loss_fn = lambda *a: None                             # no module at all
     assert t._pair_kernel() is None
+
+
+def test_preference_trainer_keeps_an_overridden_sum():
+    """A trainer that makes its sequences' log-probabilities in its own way is asked for them, of the policy too."""
+    from trainscale_b200 import rl
+    asked = []
+
+    class Own(rl.PreferenceTrainer):
+        def _seq_logps(self, model, ids, mask, labels, grad):
+            asked.append(model)
+            return torch.full((4,), -1.0, requires_grad=grad), torch.full((4,), 3)
+
+    batch = {f"{side}_{k}": torch.ones(2, 3, dtype=torch.long) for side in ("chosen", "rejected")
+             for k in ("input_ids", "attention_mask", "labels")}
+    for kind in ("dpo", "simpo", "cpo", "orpo"):
+        t = Own(torch.nn.Linear(1, 1), None, None, kind)
+        assert not t._sums_plainly() and t.compute_loss(batch)[0].isfinite()
+        assert asked.pop() is t.policy and not asked
+    t = rl.PreferenceTrainer(None, None, None, "dpo")
+    assert t._sums_plainly()

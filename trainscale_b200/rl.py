@@ -437,6 +437,9 @@ class PreferenceTrainer:
         lp, valid = self._token_logps(model, ids, mask, labels, grad)
         return lp.sum(-1), valid.sum(-1)
 
+    def _sums_plainly(self) -> bool:
+        return type(self)._seq_logps is PreferenceTrainer._seq_logps and "_seq_logps" not in self.__dict__
+
     def _pair_kernel(self) -> dict | None:
         """The loss as arguments of `preference_loss`; None for those that are not a function of one pair's scores, and for a loss module
         that is not just what the constructor makes: a subclass, another module, one with hooks, a replaced forward or a learned beta."""
@@ -464,10 +467,16 @@ class PreferenceTrainer:
         ids = torch.cat((batch["chosen_input_ids"], batch["rejected_input_ids"]))
         mask = torch.cat((batch["chosen_attention_mask"], batch["rejected_attention_mask"]))
         labels = torch.cat((batch["chosen_labels"], batch["rejected_labels"]))
-        tokens, valid = self._token_logps(self.policy, ids, mask, labels, True)
         metrics = {}
-        kernel = self._pair_kernel()
-        if kernel is not None and policy_ops.native(tokens, valid):
+        # (a trainer that sums in its own way has no token log-probabilities to give)
+        kernel = self._pair_kernel() if self._sums_plainly() else None
+        if kernel is not None:
+            tokens, valid = self._token_logps(self.policy, ids, mask, labels, True)
+            if not policy_ops.native(tokens, valid):
+                kernel, lp, n = None, tokens.sum(-1), valid.sum(-1)
+        else:
+            lp, n = self._seq_logps(self.policy, ids, mask, labels, True)
+        if kernel is not None:
             ref = None
             if self.kind == "dpo" and self.ref is not None and not self.loss_fn.reference_free:
                 ref, _ = self._token_logps(self.ref, ids, mask, labels, False)
@@ -477,7 +486,6 @@ class PreferenceTrainer:
             if self.kind == "dpo":
                 metrics["reward_margin"] = (cr - rjr).mean()
             return loss, metrics
-        lp, n = tokens.sum(-1), valid.sum(-1)
         pc, pr, nc, nr = lp[:B], lp[B:], n[:B], n[B:]
         if self.kind == "dpo":
             rc = rr = None
