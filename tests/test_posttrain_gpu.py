@@ -585,6 +585,22 @@ def test_group_relative_losses_keep_their_results():
         assert "kl" not in g.compute_grpo_loss(x, None, rewards, mask, old)[1]
 
 
+def test_an_overridden_policy_loss_is_called():
+    from trainscale_b200.rl import GRPOCompute
+    logp, old, _, mask, ref = _policy_case(8, 20, torch.float32, torch.float32, 5, spoil=False)
+
+    class Own(GRPOCompute):
+        def __call__(self, *args):
+            return 3 * super().__call__(*args)
+
+    rewards = torch.randn(8, device=DEV, generator=_gen(1))
+    for variant in ("grpo", "drgrpo", "dapo"):
+        loss, stats = GRPOCompute(4, variant=variant).compute_grpo_loss(logp, ref, rewards, mask, old)
+        own, same = Own(4, variant=variant).compute_grpo_loss(logp, ref, rewards, mask, old)
+        assert float(own) == pytest.approx(3 * float(loss), rel=1e-5)
+        assert {k: pytest.approx(v, rel=1e-4) for k, v in stats.items()} == same
+
+
 # ------------------------------------------------------------------------------------------------ pairs
 def _pair_case(P, T, dtype, mask_type, seed, spoil=True):
     g = _gen(seed)

@@ -342,7 +342,8 @@ class GRPOCompute:
         old = policy_log_probs.detach() if old_log_probs is None else old_log_probs
         adv = compute_advantages(rewards, self.group_size, scale=self.variant != "drgrpo")
         kl = None
-        if _takes_policy_kernel(policy_log_probs, old, ref_log_probs, adv, mask) and self.clip >= 0 and self.beta >= 0:
+        if (_takes_policy_kernel(policy_log_probs, old, ref_log_probs, adv, mask) and self.clip >= 0 and self.beta >= 0
+                and type(self).__call__ is GRPOCompute.__call__):
             kw = {"drgrpo": dict(reduction="constant"), "dapo": dict(reduction="token", clip_high=0.28)}.get(
                 self.variant, dict(beta=self.beta if ref_log_probs is not None else 0.0))
             loss, seen = clipped_policy_loss(policy_log_probs, old, adv, mask, ref_log_probs, clip=self.clip, return_stats=True, **kw)
