@@ -242,3 +242,40 @@ def test_preference_trainer_keeps_an_overridden_sum():
         assert asked.pop() is t.policy and not asked
     t = rl.PreferenceTrainer(None, None, None, "dpo")
     assert t._sums_plainly()
+
+
+def test_calls_that_the_kernels_entries_would_refuse_keep_the_pytorch_form(monkeypatch):
+    """No bound on a ratio, an infinite temperature, numbers that are tensors: the dispatch leaves them where they were."""
+    from trainscale_b200 import rl
+    g = _gen(6)
+    logp = torch.randn(4, 5, generator=g)
+    old, ref, adv, mask = logp + 0.5 * torch.randn(4, 5, generator=g), logp + 0.1, torch.randn(4, generator=g), torch.ones(4, 5)
+    z, y = torch.randn(4, 9, generator=g), torch.arange(4)
+    inf, nan, one = math.inf, math.nan, torch.tensor(0.2)
+    rewards = torch.randn(4, generator=g)
+
+    def group(**kw):
+        return rl.GRPOCompute(2, **kw).compute_grpo_loss(logp, ref, rewards, mask, old)[0]
+
+    calls = [lambda: rl.grpo_loss(logp, old, ref, adv, mask, clip=inf), lambda: rl.grpo_loss(logp, old, ref, adv, mask, beta=inf),
+             lambda: rl.grpo_loss(logp, old, ref, adv, mask, clip=one), lambda: rl.drgrpo_loss(logp, old, adv, mask, clip=inf),
+             lambda: rl.drgrpo_loss(logp, old, adv, mask, max_len=torch.tensor(7.0)), lambda: rl.dapo_loss(logp, old, adv, mask, clip_high=inf),
+             lambda: rl.dapo_loss(logp, old, adv, mask, clip_low=inf), lambda: group(clip=inf), lambda: group(clip=nan),
+             lambda: group(clip=inf, variant="dapo"), lambda: rl.selective_log_softmax(z, y, inf),
+             lambda: rl.selective_log_softmax(z, y, 1e-35), lambda: rl.selective_log_softmax(z, y, 1.0, inf),
+             lambda: rl.selective_log_softmax(z, y, 1.0, 30.0, 1e35), lambda: rl.selective_log_softmax(z, y, torch.tensor(0.7)),
+             lambda: rl.selective_log_softmax(z, y, 1.0, torch.tensor(5.0))]
+    want = [call() for call in calls]
+    asked = []
+    monkeypatch.setattr(rl.policy_ops, "native", lambda *t: True)
+    monkeypatch.setattr(rl.lp_ops, "native", lambda *t: True)
+    monkeypatch.setattr(rl, "clipped_policy_loss", lambda *a, **k: asked.append(1))
+    monkeypatch.setattr(rl, "token_log_probs", lambda *a, **k: asked.append(1))
+    for call, w in zip(calls, want):
+        torch.testing.assert_close(call(), w, rtol=0, atol=0, equal_nan=True)
+    assert not asked
+    rl.grpo_loss(logp, old, ref, adv, mask)
+    rl.drgrpo_loss(logp, old, adv, mask, max_len=7)
+    rl.dapo_loss(logp, old, adv, mask)
+    rl.selective_log_softmax(z, y, 0.7, None, 1.5)
+    assert len(asked) == 4

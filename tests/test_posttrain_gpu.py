@@ -585,6 +585,16 @@ def test_group_relative_losses_keep_their_results():
         assert "kl" not in g.compute_grpo_loss(x, None, rewards, mask, old)[1]
 
 
+def test_policies_without_a_bound():
+    """Infinite clip ranges and temperatures, which the kernels' own entries refuse, as on the CPU."""
+    from trainscale_b200 import rl
+    logp, old, adv, mask, ref = _policy_case(8, 20, torch.float32, torch.float32, 5, spoil=False)
+    z, y = torch.randn(8, 50, device=DEV, generator=_gen(2)), torch.arange(8, device=DEV)
+    for f, args, kw in ((rl.grpo_loss, (logp, old, ref, adv, mask), dict(clip=math.inf)), (rl.drgrpo_loss, (logp, old, adv, mask), dict(clip=math.inf)),
+                        (rl.dapo_loss, (logp, old, adv, mask), dict(clip_high=math.inf)), (rl.selective_log_softmax, (z, y), dict(temperature=math.inf))):
+        torch.testing.assert_close(f(*args, **kw).cpu(), f(*[t.cpu() for t in args], **kw), rtol=1e-5, atol=1e-6)
+
+
 def test_an_overridden_policy_loss_is_called():
     from trainscale_b200.rl import GRPOCompute
     logp, old, _, mask, ref = _policy_case(8, 20, torch.float32, torch.float32, 5, spoil=False)

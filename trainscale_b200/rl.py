@@ -30,6 +30,14 @@ from .ops.policy import PolicyStats
 from .utils.refargs import ANY, reference_kwargs
 
 
+def _takes_transforms(temperature, cap, scale) -> bool:
+    """Whether `token_log_probs` takes these: finite, and their product within the range of fp32."""
+    if not (0 < temperature < math.inf and 0 <= cap < math.inf and 0 <= scale < math.inf):
+        return False
+    factor = (scale or 1.0) / temperature
+    return 1e-30 < factor < 1e30 and factor * (cap or 1.0) < 1e30
+
+
 def token_log_probs(logits: torch.Tensor, labels: torch.Tensor, *, temperature: float = 1.0, logit_softcapping: float = 0.0,
                     logit_scale: float = 0.0, ignore_index: int | None = -100, return_entropy: bool = False):
     """log p(labels) under `logits` [..., V] in fp32, shape of `labels` [...]; differentiable in the logits.
@@ -42,10 +50,10 @@ def token_log_probs(logits: torch.Tensor, labels: torch.Tensor, *, temperature: 
     if not (0 < temperature < math.inf and 0 <= logit_softcapping < math.inf and 0 <= logit_scale < math.inf):
         raise ValueError(f"the temperature is finite and positive, the cap and the scale are finite and not negative; not {temperature}, "
                          f"{logit_softcapping} and {logit_scale}")
-    factor = (logit_scale or 1.0) / temperature
-    if not 1e-30 < factor < 1e30 or not factor * (logit_softcapping or 1.0) < 1e30:
+    if not _takes_transforms(temperature, logit_softcapping, logit_scale):
         raise ValueError(f"a logit scale of {logit_scale}, a cap of {logit_softcapping} and a temperature of {temperature} leave the range "
                          "of fp32")
+    factor = (logit_scale or 1.0) / temperature
     return lp_ops.token_log_probs(logits, labels, factor, float(logit_softcapping), ignore_index, return_entropy)
 
 
@@ -55,11 +63,10 @@ def selective_log_softmax(logits: torch.Tensor, index: torch.Tensor, temperature
     """log_softmax(logits)[..., index] without keeping the full log-softmax.  Optional transforms of the logits, in
     this order: soft-cap c tanh(z / c), scale, divide by the temperature.  The transforms happen in the type of the logits;
     `token_log_probs` makes them in fp32 whatever that is, and is what computes this on the GPU where the two agree."""
-    plain = not (logit_softcapping or logit_scale) and temperature == 1.0
-    if ((plain or logits.dtype == torch.float32) and index.dtype == torch.int64 and index.shape == logits.shape[:-1] and temperature > 0
-            and logit_softcapping >= 0 and logit_scale >= 0 and lp_ops.native(logits, index)):
-        return token_log_probs(logits, index, temperature=temperature, logit_softcapping=logit_softcapping, logit_scale=logit_scale,
-                               ignore_index=None)
+    how = (temperature, logit_softcapping or 0.0, logit_scale or 0.0)
+    if (_numbers(*how) and (logits.dtype == torch.float32 or how == (1.0, 0.0, 0.0)) and index.dtype == torch.int64
+            and index.shape == logits.shape[:-1] and _takes_transforms(*how) and lp_ops.native(logits, index)):
+        return token_log_probs(logits, index, temperature=how[0], logit_softcapping=how[1], logit_scale=how[2], ignore_index=None)
     if logit_softcapping:
         logits = logit_softcapping * torch.tanh(logits / logit_softcapping)
     if logit_scale:
@@ -188,11 +195,17 @@ def clipped_policy_loss(logp: torch.Tensor, old_logp: torch.Tensor, advantages: 
     return (loss, PolicyStats(*stats.unbind())) if return_stats else loss
 
 
-def _takes_policy_kernel(logp, old_logp, ref_logp, advantages, mask) -> bool:
+def _numbers(*values) -> bool:
+    """Plain numbers: a tensor of one may want a gradient, or be filled in by a captured graph."""
+    return all(isinstance(v, (int, float)) for v in values)
+
+
+def _takes_policy_kernel(logp, old_logp, ref_logp, advantages, mask, *numbers) -> bool:
     """Whether `clipped_policy_loss` stands for the PyTorch form of a group-relative loss: fp32 on the GPU, a gradient for the
-    policy's log-probabilities alone."""
+    policy's log-probabilities alone, clip ranges and a weight of the KL term (`numbers`) that are finite and not negative."""
     others = [t for t in (old_logp, ref_logp, advantages, mask) if t is not None]
-    return (all(torch.is_tensor(t) for t in (logp, *others)) and policy_ops.native(logp, *others)
+    return (_numbers(*numbers) and all(0 <= v < math.inf for v in numbers)
+            and all(torch.is_tensor(t) for t in (logp, *others)) and policy_ops.native(logp, *others)
             and all(t.dtype == torch.float32 for t in (logp, old_logp, advantages) if t is not None)
             and (ref_logp is None or ref_logp.dtype == torch.float32) and advantages.shape == logp.shape[:1]
             and old_logp.shape == mask.shape == logp.shape and (ref_logp is None or ref_logp.shape == logp.shape)
@@ -238,7 +251,7 @@ def grpo_loss(logp: torch.Tensor = None, old_logp: torch.Tensor = None, ref_logp
     the reference's sequence-level loss instead and returns (loss, metrics): see `_reference_rl_loss`."""
     if policy_log_probs is not None:
         return _reference_rl_loss("grpo", policy_log_probs, ref_log_probs, advantages, mask, beta)
-    if _takes_policy_kernel(logp, old_logp, ref_logp, advantages, mask) and 0 <= clip and 0 <= beta:
+    if _takes_policy_kernel(logp, old_logp, ref_logp, advantages, mask, clip, beta):
         beta = beta if ref_logp is not None else 0.0
         return clipped_policy_loss(logp, old_logp, advantages, mask, ref_logp if beta else None, clip=clip, beta=beta)
     ratio = torch.exp(logp - old_logp)
@@ -258,7 +271,7 @@ def drgrpo_loss(logp=None, old_logp=None, advantages=None, mask=None, clip: floa
     returning (loss, metrics)."""
     if policy_log_probs is not None:
         return _reference_rl_loss("drgrpo", policy_log_probs, ref_log_probs, advantages, mask, beta, epsilon)
-    if _takes_policy_kernel(logp, old_logp, None, advantages, mask) and 0 <= clip and (max_len is None or max_len > 0):
+    if _takes_policy_kernel(logp, old_logp, None, advantages, mask, clip) and (max_len is None or _numbers(max_len) and max_len > 0):
         return clipped_policy_loss(logp, old_logp, advantages, mask, clip=clip, reduction="constant", max_len=max_len)
     ratio = torch.exp(logp - old_logp)
     a = advantages.unsqueeze(-1)
@@ -274,7 +287,7 @@ def dapo_loss(logp=None, old_logp=None, advantages=None, mask=None, clip_low: fl
     returning (loss, metrics)."""
     if policy_log_probs is not None:
         return _reference_rl_loss("dapo", policy_log_probs, ref_log_probs, rewards, mask, beta, temperature=temperature)
-    if _takes_policy_kernel(logp, old_logp, None, advantages, mask) and 0 <= clip_low and 0 <= clip_high:
+    if _takes_policy_kernel(logp, old_logp, None, advantages, mask, clip_low, clip_high):
         return clipped_policy_loss(logp, old_logp, advantages, mask, clip=clip_low, clip_high=clip_high, reduction="token")
     ratio = torch.exp(logp - old_logp)
     a = advantages.unsqueeze(-1)
@@ -342,7 +355,7 @@ class GRPOCompute:
         old = policy_log_probs.detach() if old_log_probs is None else old_log_probs
         adv = compute_advantages(rewards, self.group_size, scale=self.variant != "drgrpo")
         kl = None
-        if (_takes_policy_kernel(policy_log_probs, old, ref_log_probs, adv, mask) and self.clip >= 0 and self.beta >= 0
+        if (_takes_policy_kernel(policy_log_probs, old, ref_log_probs, adv, mask, self.clip, self.beta)
                 and type(self).__call__ is GRPOCompute.__call__):
             kw = {"drgrpo": dict(reduction="constant"), "dapo": dict(reduction="token", clip_high=0.28)}.get(
                 self.variant, dict(beta=self.beta if ref_log_probs is not None else 0.0))
