@@ -595,6 +595,15 @@ def test_policies_without_a_bound():
         torch.testing.assert_close(f(*args, **kw).cpu(), f(*[t.cpu() for t in args], **kw), rtol=1e-5, atol=1e-6)
 
 
+def test_masks_in_fp64_give_losses_in_fp64():
+    from trainscale_b200 import rl
+    logp, old, adv, mask, ref = _policy_case(8, 20, torch.float32, torch.float64, 5, spoil=False)
+    for f, args in ((rl.grpo_loss, (logp, old, ref, adv, mask)), (rl.drgrpo_loss, (logp, old, adv, mask)), (rl.dapo_loss, (logp, old, adv, mask))):
+        got, want = f(*args), f(*[t.cpu() for t in args])
+        assert got.dtype == want.dtype == torch.float64
+        torch.testing.assert_close(got.cpu(), want, rtol=1e-6, atol=1e-8)
+
+
 def test_an_overridden_policy_loss_is_called():
     from trainscale_b200.rl import GRPOCompute
     logp, old, _, mask, ref = _policy_case(8, 20, torch.float32, torch.float32, 5, spoil=False)

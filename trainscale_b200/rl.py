@@ -206,7 +206,7 @@ def _takes_policy_kernel(logp, old_logp, ref_logp, advantages, mask, *numbers) -
     others = [t for t in (old_logp, ref_logp, advantages, mask) if t is not None]
     return (_numbers(*numbers) and all(0 <= v < math.inf for v in numbers)
             and all(torch.is_tensor(t) for t in (logp, *others)) and policy_ops.native(logp, *others)
-            and all(t.dtype == torch.float32 for t in (logp, old_logp, advantages) if t is not None)
+            and all(t.dtype == torch.float32 for t in (logp, old_logp, advantages) if t is not None) and mask.dtype != torch.float64
             and (ref_logp is None or ref_logp.dtype == torch.float32) and advantages.shape == logp.shape[:1]
             and old_logp.shape == mask.shape == logp.shape and (ref_logp is None or ref_logp.shape == logp.shape)
             and not (torch.is_grad_enabled() and any(t.requires_grad for t in others)))
