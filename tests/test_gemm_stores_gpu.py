@@ -97,3 +97,25 @@ def test_grouped_reductions_stay_in_their_slabs(M, N, first):
     ref = torch.cat([a[s:t].double().t() @ b[s:t].double() for s, t in zip(at, at[1:])])
     _check(wide, out, ref)
     assert (out[M:2 * M] == 0).all()
+
+
+def _single_rows(K):
+    """One row of K values (a multiple of 8) with pitches that a tensor map takes and that it does not."""
+    for pitch in (K, K + 8, K + 1, K + 5):
+        yield _rand(1, pitch)[:, :K]
+    yield _rand(K).as_strided((1, K), (0, 1))
+    yield _rand(K).as_strided((1, K), (8, 1))
+    yield _rand(K, 1).t()
+
+
+@pytest.mark.parametrize("K", [64, 136])
+def test_a_single_row_may_have_any_pitch(K):
+    from trainscale_b200.ops import gemm
+    torch.manual_seed(0)
+    b = _rand(72, K)
+    for a in _single_rows(K):
+        assert a.dim() == 2 and a.data_ptr() % 16 == 0
+        for got, want in ((gemm.matmul_nt(a, b), a.double() @ b.double().t()), (gemm.matmul_nt(b, a), b.double() @ a.double().t()),
+                          (gemm.matmul_nn(a, b.t().contiguous()), a.double() @ b.double().t()),
+                          (gemm.matmul_tn(a, _rand(1, 72).fill_(1.0)), a.double().t().expand(K, 72))):
+            assert got.shape == want.shape and ((got.double() - want).abs() <= 2.0 ** -8 * want.abs() + 1e-3).all()

@@ -148,3 +148,17 @@ def test_optimizer_shards_reslice_exactly_between_world_sizes(old, new, used):
     assert whole.numel() == n_new
     torch.testing.assert_close(whole[:used], full)
     assert float(whole[used:].abs().sum()) == 0.0
+
+
+def test_rows_of_a_product_keep_a_pitch_that_a_tensor_map_takes():
+    """Rows as the products' kernels read them: dense within themselves, on 16-byte pitches; a single row's pitch says nothing."""
+    import torch
+    from trainscale_b200.ops.gemm import _rows2d
+    base = torch.arange(4 * 160, dtype=torch.float32).bfloat16()
+    for t in (base[:144].view(1, 144)[:, :136], base[:137].view(1, 137)[:, :136], base.as_strided((1, 136), (0, 1)),
+              base.as_strided((1, 136), (8, 1)), base[:136].view(136, 1).t(), base[:141].view(1, 1, 141)[..., :136]):
+        r = _rows2d(t)
+        assert torch.equal(r, t.reshape(-1, 136)) and r.stride(1) == 1 and r.stride(0) >= 136 and r.stride(0) % 8 == 0
+    assert _rows2d(base[:144].view(1, 144)[:, :136]).stride(0) == 144
+    assert _rows2d(base[:4 * 144].view(4, 144)[:, :136]).stride(0) == 144
+    assert _rows2d(base[:4 * 137].view(4, 137)[:, :136]).stride(0) == 136

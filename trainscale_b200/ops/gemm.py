@@ -31,7 +31,10 @@ def gemm_raw(a: torch.Tensor, b: torch.Tensor, out: torch.Tensor, M: int, N: int
 
 
 def _rows2d(t: torch.Tensor) -> torch.Tensor:
-    t = t if t.dim() == 2 else t.reshape(-1, t.shape[-1])       # (reshape would forget the pitch of a single row)
+    # reshape gives a single row a pitch of its length.  Only one that a tensor map refuses goes that way: the pitch of a padded row
+    # may be right where its length is not.
+    if t.dim() != 2 or (t.shape[0] == 1 and (t.stride(0) < t.shape[1] or (t.stride(0) * t.element_size()) % 16 != 0)):
+        t = t.reshape(-1, t.shape[-1])
     if t.stride(-1) != 1 or (t.stride(0) * t.element_size()) % 16 != 0 or t.data_ptr() % 16 != 0:
         t = t.contiguous()
     return t
