@@ -279,3 +279,40 @@ def test_calls_that_the_kernels_entries_would_refuse_keep_the_pytorch_form(monke
     rl.dapo_loss(logp, old, adv, mask)
     rl.selective_log_softmax(z, y, 0.7, None, 1.5)
     assert len(asked) == 4
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float64])
+def test_ratios_that_overflow(dtype):
+    """A clipped ratio, and one without an advantage, have no say: neither in the loss nor in its derivatives, however large."""
+    far = 100.0 if dtype == torch.float32 else 800.0
+    old, mask = torch.zeros(1, 3, dtype=dtype), torch.ones(1, 3)
+    for adv, want, slope in ((1.0, -(1.2 + 1.0 + 0.5) / 3, [0.0, -1 / 3, -0.5 / 3]), (0.0, 0.0, [0.0, 0.0, 0.0])):
+        x = torch.tensor([[far, 0.0, math.log(0.5)]], dtype=dtype, requires_grad=True)
+        loss, stats = clipped_policy_loss(x, old, torch.tensor([adv]), mask, return_stats=True)
+        (d,) = torch.autograd.grad(loss, x, create_graph=True)
+        (dd,) = torch.autograd.grad(d.sum(), x)
+        assert float(loss) == pytest.approx(want, rel=1e-6) and d[0].tolist() == pytest.approx(slope, rel=1e-6) and dd.isfinite().all()
+        assert float(stats.ratio) == math.inf and float(stats.clip_fraction) == pytest.approx(1 / 3 if adv else 0.0)
+    x = torch.tensor([[-far, 0.0, 0.0]], dtype=dtype, requires_grad=True)
+    loss = clipped_policy_loss(x, old, torch.tensor([-1.0]), mask)
+    assert float(loss) == pytest.approx((0.8 + 2) / 3, rel=1e-6)
+    assert torch.autograd.grad(loss, x)[0][0].tolist() == pytest.approx([0.0, 1 / 3, 1 / 3], rel=1e-6)
+    x = torch.tensor([[far, 0.0, 0.0]], dtype=dtype, requires_grad=True)      # one that counts does overflow
+    loss = clipped_policy_loss(x, old, torch.tensor([-1.0]), mask)
+    assert float(loss) == math.inf and float(torch.autograd.grad(loss, x)[0][0, 0]) == math.inf
+    assert clipped_policy_loss(torch.full((1, 3), math.nan, dtype=dtype), old, torch.zeros(1), mask).isnan()
+
+
+def test_tokens_at_a_clip_bound():
+    """A difference that fp32 rounds onto the bound, or past it, is on the side where it lies."""
+    from fractions import Fraction
+    x = torch.tensor([[-1.0, -1.0, -1.0, -1.0]])
+    up, down = math.log1p(0.2), math.log1p(-0.2)
+    f32 = lambda v: torch.tensor(v, dtype=torch.float32)                               # noqa: E731
+    old = torch.stack([f32(-1.0 - up), torch.nextafter(f32(-1.0 - up), f32(0.0)), f32(-1.0 - down), torch.nextafter(f32(-1.0 - down), f32(-2.0))])
+    moved = [Fraction(-1) - Fraction(float(o)) for o in old]
+    above, below = [v > Fraction(up) for v in moved], [v < Fraction(down) for v in moved]
+    for sign, want in ((1.0, above), (-1.0, below)):
+        p = x.clone().requires_grad_()
+        clipped_policy_loss(p, old.unsqueeze(0), torch.tensor([sign]), torch.ones(1, 4)).backward()
+        assert [float(d) == 0 for d in p.grad[0]] == want

@@ -604,6 +604,21 @@ def test_masks_in_fp64_give_losses_in_fp64():
         torch.testing.assert_close(got.cpu(), want, rtol=1e-6, atol=1e-8)
 
 
+def test_overflowing_ratios_whose_gradient_is_differentiated():
+    """The PyTorch form behind a kernel's gradient keeps the kernel's zeros."""
+    from trainscale_b200.rl import clipped_policy_loss
+    old, mask = torch.zeros(2, 3, device=DEV), torch.ones(2, 3, device=DEV)
+    x = torch.tensor([[100.0, 0.0, -0.5], [100.0, 0.0, -0.5]], device=DEV, requires_grad=True)
+    adv = torch.tensor([1.0, 0.0], device=DEV)
+    loss = clipped_policy_loss(x, old, adv, mask)
+    (d,) = torch.autograd.grad(loss, x, retain_graph=True)
+    (e,) = torch.autograd.grad(loss, x, create_graph=True)
+    torch.testing.assert_close(d, e.detach(), rtol=1e-6, atol=1e-9)
+    assert d.isfinite().all() and (d[1] == 0).all() and float(d[0, 0]) == 0
+    (dd,) = torch.autograd.grad(e.sum(), x)
+    torch.testing.assert_close(dd, e.detach(), rtol=1e-6, atol=1e-9)        # (the derivative of -a r / n is itself)
+
+
 def test_an_overridden_policy_loss_is_called():
     from trainscale_b200.rl import GRPOCompute
     logp, old, _, mask, ref = _policy_case(8, 20, torch.float32, torch.float32, 5, spoil=False)

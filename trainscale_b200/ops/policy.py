@@ -175,10 +175,14 @@ class PolicyLoss:
         logp, old = _masked(logp, used).to(m.dtype), _masked(old_logp, used).to(m.dtype)
         a = advantages if advantages.dim() == 2 else advantages.unsqueeze(1)
         a = _masked(a.to(m.dtype).expand(logp.shape), used)
-        ratio = torch.exp(logp - old)
-        gain = torch.minimum(ratio * a, ratio.clamp(1 - self.low, 1 + self.high) * a)
-        clipped = ((a > 0) & (ratio > 1 + self.high)) | ((a < 0) & (ratio < 1 - self.low))
-        token, kl = -gain, torch.zeros_like(gain)
+        with torch.no_grad():
+            moved = logp.double() - old.double()      # (fp32 could round it to the other side of a bound)
+            clipped = ((a > 0) & (moved > math.log1p(self.high))) | ((a < 0) & (moved < (math.log1p(-self.low) if self.low < 1 else -math.inf)))
+            idle = clipped | ((a == 0) & ~moved.isnan())
+        # (0 * inf: a ratio that has no say may overflow, and so would its derivative: it is not taken)
+        ratio = torch.exp((logp - old).where(~idle, 0.0))
+        bound = torch.full_like(a, 1 - self.low).masked_fill(a > 0, 1 + self.high)
+        token, kl = -a * bound.where(clipped, ratio), torch.zeros_like(logp)
         if ref_logp is not None:
             d = _masked(ref_logp, used).to(m.dtype) - logp
             kl = torch.expm1(d) - d
@@ -192,7 +196,7 @@ class PolicyLoss:
         else:
             loss = (token * m).sum() / max(1, m.shape[0] * (self.length or m.shape[1]))
         with torch.no_grad():
-            stats = torch.stack([(x.detach() * m).sum() / total for x in (kl, clipped.to(m.dtype), ratio)])
+            stats = torch.stack([(x.detach() * m).sum() / total for x in (kl, clipped.to(m.dtype), torch.exp(logp - old))])
         return loss, stats
 
 
