@@ -316,3 +316,16 @@ def test_tokens_at_a_clip_bound():
         p = x.clone().requires_grad_()
         clipped_policy_loss(p, old.unsqueeze(0), torch.tensor([sign]), torch.ones(1, 4)).backward()
         assert [float(d) == 0 for d in p.grad[0]] == want
+
+
+@pytest.mark.parametrize("listed,port", [("", 29781), ("0,1", 29782), ("1", 29783)])
+def test_a_norm_over_ranks(listed, port):
+    """Two ranks, tensor by tensor, through the kernels' list (a stand-in), and one of each."""
+    import subprocess
+    import sys
+    from pathlib import Path
+    case = Path(__file__).parent / "dist_cases" / "clip_norm.py"
+    r = subprocess.run([sys.executable, "-m", "torch.distributed.run", "--nnodes=1", "--nproc-per-node=2", "--master-addr", "127.0.0.1",
+                        "--master-port", str(port), str(case), f"--listed={listed}"], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stdout[-2000:] + r.stderr[-2000:]
+    assert r.stdout.count("ok=True") == 2

@@ -890,6 +890,33 @@ def test_fused_clip_grad_norm():
         assert float(after) == pytest.approx(float(norm) / 3, rel=1e-5)
 
 
+@pytest.mark.parametrize("scale", [1.0, 1e25, 1e-25])
+def test_fused_clip_grad_norm_over_a_group(scale, monkeypatch):
+    """The kernels' norm between two ranks that hold the same (the collective is a stand-in): powers of it stay in range."""
+    import torch.distributed as dist
+    from trainscale_b200.parallel.dist_utils import fused_clip_grad_norm_
+    group, seen = object(), []
+
+    def all_reduce(t, op=dist.ReduceOp.SUM, group=None):
+        seen.append((t.dtype, group))
+        if op == dist.ReduceOp.SUM:
+            t.mul_(2)
+
+    monkeypatch.setattr(dist, "is_initialized", lambda: True)
+    monkeypatch.setattr(dist, "get_world_size", lambda group=None: 2)
+    monkeypatch.setattr(dist, "all_reduce", all_reduce)
+    for kind in (2.0, 1.0, math.inf):
+        p = torch.nn.Parameter(torch.zeros(1000, device=DEV))
+        p.grad = torch.randn(1000, device=DEV, generator=_gen(2)) * scale
+        before = p.grad.double()
+        norm = torch.linalg.vector_norm(torch.cat((before, before)), kind)
+        got = fused_clip_grad_norm_([p], float(norm) / 3, group=group, norm_type=kind)
+        _near(got, norm, F32 * 4 * norm)
+        want = before * min(1.0, float(norm) / 3 / (float(norm) + 1e-6))
+        _near(p.grad, want, 8 * F32 * want.abs() + 1e-38)
+    assert seen == [(torch.float64, group)] * 3
+
+
 def test_clip_marks_gradients_as_changed():
     x = torch.randn(50, device=DEV, requires_grad=True)
     p = torch.nn.Parameter(torch.zeros(50, device=DEV))

@@ -323,6 +323,17 @@ class TensorPool:
         return dict(self._stats, pooled_bytes=self._held, hit_rate=self._stats["hits"] / a if a else 0.0)
 
 
+def _norm_over_ranks(total: torch.Tensor, norm_type: float, group) -> torch.Tensor:
+    """The norm, in fp32, of what the ranks of `group` hold together, out of each one's sum of powers (norm inf: its largest value).
+    Sums of powers are fp64 between ranks: squares of 1e20 and of 1e-23 leave the range of fp32."""
+    total = total.double()
+    if norm_type == float("inf"):
+        dist.all_reduce(total, op=dist.ReduceOp.MAX, group=group)
+        return total.float()
+    dist.all_reduce(total, group=group)
+    return total.pow(1.0 / norm_type).float()
+
+
 @torch.no_grad()
 @reference_kwargs({"foreach": ANY}, model_or_params="parameters", process_group="group")
 def fused_clip_grad_norm_(parameters, max_norm: float, group=None, norm_type: float = 2.0,
@@ -339,12 +350,8 @@ def fused_clip_grad_norm_(parameters, max_norm: float, group=None, norm_type: fl
     norm = listed.norm(norm_type) if listed is not None else None
     if norm is not None:
         if sharded:
-            if norm_type == float("inf"):
-                dist.all_reduce(norm, op=dist.ReduceOp.MAX, group=group)
-            else:
-                norm = norm.pow(norm_type)
-                dist.all_reduce(norm, group=group)
-                norm = norm.pow(1.0 / norm_type)
+            own = norm.double()
+            norm = _norm_over_ranks(own if norm_type == float("inf") else own.pow(norm_type), norm_type, group)
         if error_if_nonfinite and not bool(torch.isfinite(norm)):
             raise RuntimeError(f"the total gradient norm is {float(norm)}")
         listed.clip_(norm, max_norm)
@@ -352,12 +359,10 @@ def fused_clip_grad_norm_(parameters, max_norm: float, group=None, norm_type: fl
     if norm_type == float("inf"):
         norm = torch.stack([g.float().abs().max() for g in grads]).max()
         if sharded:
-            dist.all_reduce(norm, op=dist.ReduceOp.MAX, group=group)
+            norm = _norm_over_ranks(norm, norm_type, group)
     else:
         sq = torch.stack([g.float().abs().pow(norm_type).sum() for g in grads]).sum()
-        if sharded:
-            dist.all_reduce(sq, group=group)
-        norm = sq.pow(1.0 / norm_type)
+        norm = _norm_over_ranks(sq, norm_type, group) if sharded else sq.pow(1.0 / norm_type)
     if error_if_nonfinite and not bool(torch.isfinite(norm)):
         raise RuntimeError(f"the total gradient norm is {float(norm)}")
     coef = (max_norm / (norm + 1e-6)).clamp(max=1.0)
