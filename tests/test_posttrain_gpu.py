@@ -94,6 +94,53 @@ def test_token_log_probs_of_few_and_many_rows(rows, V, dtype, cap, entropy):
     _check_tokens(z, y, 0.6, cap, entropy)
 
 
+def _gradient64(z, y, temperature, cap, g, h):
+    """The gradient, and what fp32 may be off by in each of its elements.  A probability p_j is off by what its logarithm is: the
+    roundings of its exponent (4 of F32 times the largest |logit| and the distance between logits), of an exponential (two units in the
+    last place) and of the sum it is divided by (as many additions as a thread makes, at most V / 256 + 32).  With a cap, tanh and its
+    slope add 2^-21 each.  ln p + H is off by as much, against 1 + |ln p| + H; the chosen token's g by three roundings.  Exponentials
+    below 2^-126 are zero."""
+    V = z.shape[-1]
+    x = z.double()
+    t = torch.tanh(x / cap) if cap else None
+    v = (cap * t if cap else x) / temperature
+    slope = (1 - t * t if cap else torch.ones_like(x)) / temperature
+    lp = torch.log_softmax(v, -1)
+    p, used = lp.exp(), (y != -100).unsqueeze(-1)
+    H = -(p * lp).sum(-1, keepdim=True)
+    one = torch.zeros_like(x).scatter_(-1, y.clamp(min=0).unsqueeze(-1), 1.0)
+    g, h = (torch.zeros_like(H) if d is None else d.double().unsqueeze(-1) for d in (g, h))
+    grad = slope * (one * g - p * (g + h * (lp + H)))
+    big = v.abs().amax(-1, keepdim=True) + (v - v.amax(-1, keepdim=True)).abs()
+    rel = F32 * (4 * big + V / 256 + 40) + (2.0 ** -21 * (2 + big) if cap else 0.0)
+    tol = slope * (p * rel * (g.abs() + 2 * h.abs() * (1 + lp.abs() + H)) + one * g.abs() * (3 * F32 + (2.0 ** -21 if cap else 0.0)))
+    tol = tol + 2.0 ** -126 * (g.abs() + h.abs() * 200) + HALF[z.dtype] * grad.abs() * 1.01 + (2.0 ** -25 if z.dtype == torch.float16 else 2.0 ** -133)
+    return grad.where(used, 0.0), tol.where(used, 0.0)
+
+
+@pytest.mark.parametrize("entropy", [False, True])
+@pytest.mark.parametrize("cap", [0.0, 20.0])
+@pytest.mark.parametrize("dtype", list(HALF))
+@pytest.mark.parametrize("rows,V,first", [(19, 4099, 0), (19, 4099, 3), (19, 4104, 8), (3, 50001, 0), (620, 9001, 5)])
+def test_gradients_of_every_logit(rows, V, first, dtype, cap, entropy):
+    """Each element against its own size: a vector left out, a wrong tail or a missing term would show in any column."""
+    from trainscale_b200.rl import token_log_probs
+    z = (torch.randn(rows, first + V, device=DEV, generator=_gen(V)) * 3).to(dtype)[:, first:]
+    y = torch.randint(0, V, (rows,), device=DEV, generator=_gen(V + 1))
+    y[1] = -100
+    scale = 4096.0 if dtype == torch.float16 else 1.0       # (a loss scale, as training in fp16 has it)
+    g, h = (torch.randn(rows, device=DEV, generator=_gen(i)) * scale for i in (1, 2))
+    h = h if entropy else None
+    x = z.detach().requires_grad_()
+    out = token_log_probs(x, y, temperature=0.8, logit_softcapping=cap, return_entropy=entropy)
+    (d,) = torch.autograd.grad(out, x, (g, h) if entropy else (g,))
+    grad, tol = _gradient64(z, y, 0.8, cap, g, h)
+    used = y != -100
+    # the test looks at nearly every element: few are as small as what they may be off by
+    assert float((grad[used].abs() > 4 * tol[used]).double().mean()) > (0.85 if dtype == torch.float16 else 0.99)
+    _near(d, grad, tol)
+
+
 @pytest.mark.parametrize("V", [515, 520])
 def test_rows_that_lie_elsewhere(V):
     """Slices, pitched rows, unaligned starts, transposed storage, one row, four dimensions."""
