@@ -167,35 +167,54 @@ struct LogitRows {
   }
 };
 
-// tanh(x), x = z / c, out of E = e^(-2 |x|) <= 1, so that the slope 1 - tanh^2 = 4 E / (1 + E)^2 keeps its bits where tanh is
-// close to one; below 0.15, where 1 - E would lose them, a power series (x^9 is the first term left out: 6e-9).  Off by 2^-21 of
-// its value.
-__device__ __forceinline__ float tanh_series(float x) {
-  const float q = x * x;
-  return x * fmaf(q, fmaf(q, fmaf(q, -17.f / 315.f, 2.f / 15.f), -1.f / 3.f), 1.f);
-}
-template <bool CAP>
-__device__ __forceinline__ float capped(float z, float inv_cap, float* slope = nullptr) {
-  if (!CAP) return z;
-  const float x = z * inv_cap, e = fast_ex2(fabsf(x) * (-2.f * LOG2E)), r = fast_rcp(1.f + e);
-  if (slope) *slope = 4.f * e * r * r;
-  return fabsf(x) < 0.15f ? tanh_series(x) : copysignf((1.f - e) * r, x);
-}
-// Two at once, 1 / (1 + E) by Newton's iteration from a parabola through it at E = 0, 1/2 and 1 (off by 0.016, then by 3e-4 and
-// 7e-8): two calls of the special-function unit for an element instead of three, which is what bounds the forward pass.
-template <bool CAP>
-__device__ __forceinline__ Pair capped2(float z, float w, float inv_cap) {
+// tanh(x), x = z / c, of two values: below a seam the odd polynomial x + x q P(q), q = x^2, above it 1 - E 2 / (1 + E), E = e^(-2 |x|).
+// P is a minimax fit (Remez' exchange) to (tanh(x) / x - 1) / q, off by 2^-25.9 of tanh.  Rounding included, tanh is off by 2^-22.8 of its
+// value at most and 2^-25 in the mean, as far as the library's is: at the seam an error of E counts a third of itself, and where E is
+// closer to one and counts in full the polynomial has taken over.  (A seam at 0.15 took as long and was off by up to 2^-20.9.)
+// Without a slope the quotient is a fit as well (2^-26, for E <= e^-1.8), which leaves one call of the special-function unit for an
+// element; the forward pass asks for most of them.  With one it is a reciprocal, which also gives a quarter of the slope 1 - tanh^2,
+// E / (1 + E)^2.  FINE: below the seam, where that is off by 2^-21.7, the slope is the difference, which cancels only above; results of 16
+// bits do not show it (2103 x 32001 bf16 gradients take 74 us without and 85 with it, fp32 ones 92 and 92).
+constexpr float TANH_SEAM = 0.9f;
+enum Slope { NONE, COARSE, FINE };
+template <bool CAP, Slope SLOPE>
+__device__ __forceinline__ Pair capped2(float z, float w, float inv_cap, Pair* quarter = nullptr) {
   if (!CAP) return Pair(z, w);
-  const Pair v = Pair(z, w) * Pair(inv_cap, inv_cap), q = v * v, one(1.f, 1.f), two(2.f, 2.f), minus(-1.f, -1.f);
+  auto both = [](float v) { return Pair(v, v); };
+  const Pair v = Pair(z, w) * both(inv_cap), q = v * v;
   const float2 x = v.get();
-  const float2 series = (v * fma2(q, fma2(q, fma2(q, Pair(-17.f / 315.f, -17.f / 315.f), Pair(2.f / 15.f, 2.f / 15.f)),
-                                          Pair(-1.f / 3.f, -1.f / 3.f)), one)).get();
-  const Pair e(fast_ex2(fabsf(x.x) * (-2.f * LOG2E)), fast_ex2(fabsf(x.y) * (-2.f * LOG2E))), d = fma2(e, minus, minus);
-  Pair r = fma2(e, fma2(e, Pair(1.f / 3.f, 1.f / 3.f), Pair(-5.f / 6.f, -5.f / 6.f)), one);
-  r = r * fma2(d, r, two);
-  r = r * fma2(d, r, two);
-  const float2 t = (fma2(e, minus, one) * r).get();
-  return Pair(fabsf(x.x) < 0.15f ? series.x : copysignf(t.x, x.x), fabsf(x.y) < 0.15f ? series.y : copysignf(t.y, x.y));
+  const float2 e2 = make_float2(fast_ex2(fabsf(x.x) * (-2.f * LOG2E)), fast_ex2(fabsf(x.y) * (-2.f * LOG2E)));
+  const Pair e(e2.x, e2.y);
+  Pair p = fma2(q, both(1.30395975e-3f), both(-6.86005596e-3f));
+  p = fma2(q, p, both(2.09041275e-2f));
+  p = fma2(q, p, both(-5.37214912e-2f));
+  p = fma2(q, p, both(1.33303598e-1f));
+  p = fma2(q, p, both(-3.33332121e-1f));
+  const Pair odd = fma2(v, q * p, v);
+  const float2 low = odd.get();
+  const bool poly_x = fabsf(x.x) < TANH_SEAM, poly_y = fabsf(x.y) < TANH_SEAM;
+  float2 high;
+  if (SLOPE != NONE) {
+    const Pair r(fast_rcp(1.f + e2.x), fast_rcp(1.f + e2.y)), er = e * r;
+    high = fma2(er, both(-2.f), both(1.f)).get();
+    *quarter = er * r;
+    if (SLOPE == FINE) {
+      const float2 above = quarter->get(), below = fma2(odd * both(-0.25f), odd, both(0.25f)).get();
+      *quarter = Pair(poly_x ? below.x : above.x, poly_y ? below.y : above.y);
+    }
+  } else {
+    Pair r = fma2(e, both(-1.25909388f), both(1.87718737f));
+    r = fma2(e, r, both(-1.99024522f));
+    r = fma2(e, r, both(1.99965322f));
+    r = fma2(e, r, both(-1.99999595f));
+    high = fma2(e, r, both(1.f)).get();
+  }
+  return Pair(poly_x ? low.x : copysignf(high.x, x.x), poly_y ? low.y : copysignf(high.y, x.y));
+}
+// One value, with the bits of two.
+template <bool CAP>
+__device__ __forceinline__ float capped(float z, float inv_cap) {
+  return CAP ? capped2<CAP, NONE>(z, z, inv_cap).get().x : z;
 }
 
 struct Softmax {
@@ -250,7 +269,7 @@ __device__ __forceinline__ void add_vectors(Softmax& acc, const uint4* r, int n,
     W::unpack(r[j], f);
 #pragma unroll
     for (int e = 0; e < W::N; e += 2) {
-      const Pair t = (capped2<CAP>(f[e], f[e + 1], inv_cap) + minus) * k;
+      const Pair t = (capped2<CAP, NONE>(f[e], f[e + 1], inv_cap) + minus) * k;
       const float2 x = t.get();
       const Pair p(fast_ex2(x.x), fast_ex2(x.y));
       s = s + p;
@@ -485,26 +504,26 @@ __global__ void __launch_bounds__(LP_BACK_THREADS) logprob_bwd_kernel(const T* l
     }
   }
   const float4 k = kept[row];
-  const float m = k.x, f = a.k * (CAP ? a.inv_cap : 1.f);
+  const float m = k.x, f = a.k * (CAP ? 4.f * a.inv_cap : 1.f);     // (four quarters of a cap's slope)
   // f p (g + h (ln p + H)) = 2^u (flat + tilt u)
   const float tilt = ENT ? f * h * LN2 / k.y : 0.f, flat = f * (g + (ENT ? h * (k.z - logf(k.y)) : 0.f)) / k.y, fg = f * g;
+  constexpr Slope SLOPE = sizeof(T) == 4 ? FINE : COARSE;
   auto slope_of = [&](float value, bool chosen) {
-    float slope = 1.f;
-    const float u = exponent(capped<CAP>(value, a.inv_cap, &slope), m, a.k2);
+    Pair quarter(1.f, 1.f);
+    const float u = exponent(capped2<CAP, SLOPE>(value, value, a.inv_cap, &quarter).get().x, m, a.k2);
     const float r = (chosen ? fg : 0.f) - fast_ex2(u) * (ENT ? flat + tilt * u : flat);
-    return CAP ? slope * r : r;
+    return CAP ? quarter.get().x * r : r;
   };
   const Pair minus(-m, -m), k2(a.k2, a.k2), flat2(-flat, -flat), tilt2(-tilt, -tilt);
   auto slope_of_two = [&](float x, float y) {
-    float sx = 1.f, sy = 1.f;
-    Pair t = (Pair(capped<CAP>(x, a.inv_cap, &sx), capped<CAP>(y, a.inv_cap, &sy)) + minus) * k2;
+    Pair quarter(1.f, 1.f), t = (capped2<CAP, SLOPE>(x, y, a.inv_cap, &quarter) + minus) * k2;
     float2 u = t.get();
     if (ENT) {
       u.x = max_nan(u.x, LP_LOWEST), u.y = max_nan(u.y, LP_LOWEST);
       t = Pair(u.x, u.y);
     }
     const Pair r = Pair(fast_ex2(u.x), fast_ex2(u.y)) * (ENT ? fma2(tilt2, t, flat2) : flat2);
-    return (CAP ? r * Pair(sx, sy) : r).get();
+    return (CAP ? r * quarter : r).get();
   };
 #pragma unroll
   for (int j = 0; j < LP_BACK_FLIGHT; ++j) {
