@@ -329,3 +329,14 @@ def test_a_norm_over_ranks(listed, port):
                         "--master-port", str(port), str(case), f"--listed={listed}"], capture_output=True, text=True, timeout=300)
     assert r.returncode == 0, r.stdout[-2000:] + r.stderr[-2000:]
     assert r.stdout.count("ok=True") == 2
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float64, torch.bfloat16])
+def test_rows_without_a_distribution(dtype):
+    """What a logit of +inf, a row of -inf and a NaN leave, as the kernel has it."""
+    z = torch.zeros(5, 7, dtype=dtype)
+    z[0], z[1, 6], z[2, 3], z[3, 3] = -math.inf, math.nan, math.inf, math.inf
+    lp, H = token_log_probs(z, torch.tensor([0, 0, 0, 3, 0]), return_entropy=True)
+    assert lp[:2].isnan().all() and float(lp[2]) == -math.inf and lp[3].isnan() and lp[4].isfinite() and H[:4].isnan().all()
+    lp = token_log_probs(z, torch.tensor([-100, -100, 7, -1, 5]))
+    assert (lp[:2] == 0).all() and lp[2:4].isnan().all()

@@ -39,9 +39,13 @@ def plain(logits, labels, factor: float, cap: float, ignore_index: int | None, e
     z = logits if logits.dtype == torch.float64 else logits.float()
     if cap:
         z = cap * torch.tanh(z / cap)
-    log_p = torch.log_softmax(z * factor, dim=-1)
+    z = z * factor
+    log_p = torch.log_softmax(z, dim=-1)
     known = (labels >= 0) & (labels < logits.shape[-1])
-    logp = log_p.gather(-1, labels.where(known, 0).long().unsqueeze(-1)).squeeze(-1).where(known, math.nan)
+    chosen, top = labels.where(known, 0).long().unsqueeze(-1), z.detach().amax(-1)
+    logp = log_p.gather(-1, chosen).squeeze(-1)
+    # (beside a logit of +inf the others have no probability, as in the kernel; log_softmax says NaN)
+    logp = logp.where(top != math.inf, z.gather(-1, chosen).squeeze(-1) - top).where(known, math.nan)
     used = torch.ones_like(known) if ignore_index is None else labels != ignore_index
     logp = logp.where(used, 0.0)
     if not entropy:
