@@ -514,6 +514,7 @@ __global__ void __launch_bounds__(LP_BACK_THREADS) logprob_bwd_kernel(const T* l
     const float r = (chosen ? fg : 0.f) - fast_ex2(u) * (ENT ? flat + tilt * u : flat);
     return CAP ? quarter.get().x * r : r;
   };
+  const int chosen = label >= head && label < a.V ? (static_cast<int>(label) - head) / W::N : -1;      // the label's vector
   const Pair minus(-m, -m), k2(a.k2, a.k2), flat2(-flat, -flat), tilt2(-tilt, -tilt);
   auto slope_of_two = [&](float x, float y) {
     Pair quarter(1.f, 1.f), t = (capped2<CAP, SLOPE>(x, y, a.inv_cap, &quarter) + minus) * k2;
@@ -542,8 +543,8 @@ __global__ void __launch_bounds__(LP_BACK_THREADS) logprob_bwd_kernel(const T* l
       o[e] = t.x;
       o[e + 1] = t.y;
     }
-    const long long at = label - head - static_cast<long long>(i) * W::N;
-    if (at >= 0 && at < W::N) {
+    if (i == chosen) {
+      const long long at = label - head - static_cast<long long>(i) * W::N;
 #pragma unroll
       for (int e = 0; e < W::N; ++e)
         if (e == at) o[e] = slope_of(v[e], true);

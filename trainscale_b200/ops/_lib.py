@@ -9,6 +9,9 @@ import ctypes
 import functools
 
 import torch
+from torch._C import _are_functorch_transforms_active, _is_tracing, _len_torch_dispatch_stack
+from torch.autograd import forward_ad
+from torch.compiler import is_compiling
 
 from .build import build_libraries, lib_path
 
@@ -66,8 +69,8 @@ def eager() -> bool:
     """Whether operations only run now.  Kernels called by address are invisible to whatever records operations (torch.jit.trace,
     make_fx, torch.compile), handles them itself (dispatch modes) or derives others from them (functorch transforms, forward-mode
     differentiation): those get PyTorch operations."""
-    return not (torch.compiler.is_compiling() or torch._C._is_tracing() or torch._C._len_torch_dispatch_stack()
-                or torch._C._are_functorch_transforms_active() or torch.autograd.forward_ad._current_level >= 0)
+    return not (is_compiling() or _is_tracing() or _len_torch_dispatch_stack() or _are_functorch_transforms_active()
+                or forward_ad._current_level >= 0)
 
 
 def check(rc: int, what: str) -> None:

@@ -126,10 +126,9 @@ def rows_backward_(logits: torch.Tensor, labels: torch.Tensor, kept: torch.Tenso
     _run_backward(logits, (n, n, 0, pitch), labels, kept, g, None, logits, pitch, ignore_index=ignore_index, lenient=True)
 
 
-def batched(*grads) -> bool:
+def batched(grad: torch.Tensor | None) -> bool:
     """Whether autograd runs one backward pass for several upstream gradients (is_grads_batched, jacobian(vectorize=True))."""
-    f = torch._C._functorch
-    return any(d is not None and (f.is_legacy_batchedtensor(d) or f.is_batchedtensor(d)) for d in grads)
+    return grad is not None and torch._C._functorch.is_legacy_batchedtensor(grad)
 
 
 def gradient(form, x: torch.Tensor, upstream) -> torch.Tensor:
@@ -157,7 +156,7 @@ class _TokenLogProbs(torch.autograd.Function):
         logits, labels, kept = ctx.saved_tensors
         if g is None and h is None:
             return None, None, None, None
-        if torch.is_grad_enabled() or not _lib.eager() or batched(g, h):
+        if torch.is_grad_enabled() or not _lib.eager() or batched(g) or batched(h):
             return gradient(lambda x: plain(x, labels, *ctx.how, ctx.entropy), logits, (g, h)), None, None, None
         x, rows = _rows(logits)
         grad = torch.empty_like(logits, memory_format=torch.contiguous_format)
