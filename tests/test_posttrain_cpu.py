@@ -85,6 +85,13 @@ def test_preference_loss(kind, normalized):
     torch.testing.assert_close(x.grad, want[3], rtol=1e-10, atol=1e-12)
 
 
+def test_label_smoothing_counts_where_there_is_a_smoothed_form():
+    lp, mask = torch.randn(6, 4, generator=_gen(7)), torch.ones(6, 4)
+    for kind, counts in (("sigmoid", True), ("robust", True), ("hinge", False), ("ipo", False)):
+        a, b = (preference_loss(lp, None, mask, beta=0.5, loss_type=kind, label_smoothing=e)[0] for e in (0.0, 0.2))
+        assert bool(a != b) == counts
+
+
 def test_gradients_against_differences():
     g = _gen(4)
     z, y = torch.randn(3, 5, generator=g, dtype=torch.float64, requires_grad=True), torch.tensor([0, 4, -100])

@@ -523,6 +523,16 @@ def test_selective_log_softmax_keeps_its_results():
     torch.testing.assert_close(dd.double(), ee, rtol=1e-4, atol=1e-5)
 
 
+def test_an_index_outside_the_vocabulary():
+    from trainscale_b200.rl import selective_log_softmax
+    z = torch.randn(4, 9, device=DEV)
+    for dtype in HALF:
+        got = selective_log_softmax(z.to(dtype), torch.tensor([0, 9, -1, 8], device=DEV))
+        assert got.isnan().tolist() == [False, True, True, False]
+    with pytest.raises(RuntimeError):
+        selective_log_softmax(z.cpu(), torch.tensor([0, 9, -1, 8]))
+
+
 # ------------------------------------------------------------------------------------------------ policy loss
 MASKS = [torch.bool, torch.uint8, torch.int32, torch.int64, torch.float32, torch.bfloat16, torch.float16, torch.float64]
 

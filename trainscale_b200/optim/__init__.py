@@ -29,9 +29,10 @@ def clip_grad_norm_(parameters: Iterable[torch.Tensor], max_norm: float, norm_ty
     """Scale the gradients of `parameters` in place so that their global norm is at most `max_norm`; returns the norm before.
     Nothing is read back to the host unless `error_if_nonfinite` asks for it.
 
-    bf16, fp16 and fp32 gradients of the current GPU and norms 1, 2 and inf take two launches over the whole list: the
-    sums are fp64, the coefficient min(1, max_norm / (norm + 1e-6)) is fp32 and each product is rounded once.  Other gradients,
-    and lists in which some share memory, go tensor by tensor."""
+    bf16, fp16 and fp32 gradients of the current GPU and norms 1, 2 and inf take three launches for up to 1024 of them (two more for
+    each further 1024): the norm, its last sum, the scaling.  A thread sums 64 values at a time in fp32 - in fp64 where their squares
+    leave its range - and those sums in fp64; the coefficient min(1, max_norm / (norm + 1e-6)) is fp32 and each product is rounded once.
+    Other gradients, and lists in which some share memory, go tensor by tensor."""
     grads = [g for p in parameters if (g := p.grad) is not None]
     if not grads:
         return torch.zeros(())

@@ -62,7 +62,8 @@ def selective_log_softmax(logits: torch.Tensor, index: torch.Tensor, temperature
                           logit_softcapping: float = 0.0, logit_scale: float = 0.0) -> torch.Tensor:
     """log_softmax(logits)[..., index] without keeping the full log-softmax.  Optional transforms of the logits, in
     this order: soft-cap c tanh(z / c), scale, divide by the temperature.  The transforms happen in the type of the logits;
-    `token_log_probs` makes them in fp32 whatever that is, and is what computes this on the GPU where the two agree."""
+    `token_log_probs` makes them in fp32 whatever that is, and is what computes this on the GPU where the two agree.  There an index
+    outside the vocabulary gives NaN for its row; elsewhere it is an error."""
     how = (temperature, logit_softcapping or 0.0, logit_scale or 0.0)
     if (_numbers(*how) and (logits.dtype == torch.float32 or how == (1.0, 0.0, 0.0)) and index.dtype == torch.int64
             and index.shape == logits.shape[:-1] and _takes_transforms(*how) and lp_ops.native(logits, index)):
@@ -171,7 +172,8 @@ def clipped_policy_loss(logp: torch.Tensor, old_logp: torch.Tensor, advantages: 
     inf or NaN.  `reduction`: "sequence" (mean over the rows of the mean over their tokens), "token" (mean over all tokens) or
     "constant" (sum over B * max_len; max_len is T by default); a mask that leaves nothing counts as one token.
     `old_logp`, `advantages` and `ref_logp` are constants.  `return_stats`: (loss, `PolicyStats`), on the device.
-    On the GPU the loss and the gradient of fp32, bf16 or fp16 log-probabilities come out of one pass, summed in fp64."""
+    On the GPU the loss and the gradient of fp32, bf16 or fp16 log-probabilities leave one kernel together, behind one that counts the
+    mask where there are more than 8192 tokens; four tokens of a thread are summed in fp32, those sums in fp64."""
     shape = logp.shape
     if len(shape) != 2:
         raise ValueError(f"log-probabilities are [sequences, tokens], not {tuple(shape)}")
@@ -221,7 +223,8 @@ def preference_loss(policy_logps: torch.Tensor, ref_logps: torch.Tensor | None, 
     A sequence's score is the sum of mask * (policy - reference), divided by its tokens with `length_normalized`; the rewards are beta
     times the scores, and the loss is the mean over the pairs of a function of x, the difference of the two scores:
     "sigmoid" -log sigma(beta x - gamma) with `label_smoothing`, "robust" (its unbiased form under flipped labels), "hinge"
-    max(0, 1 - beta x + gamma) or "ipo" (x - 1 / (2 beta))^2.  `nll_weight` adds the chosen sequences' mean negative log-likelihood.
+    max(0, 1 - beta x + gamma) or "ipo" (x - 1 / (2 beta))^2; "hinge" and "ipo" have no smoothed form and are the same whatever
+    `label_smoothing` says.  `nll_weight` adds the chosen sequences' mean negative log-likelihood.
     Without `ref_logps` the loss is reference-free; reference log-probabilities are constants.  Tokens of mask zero are not read into
     the loss, not even inf or NaN.  Scores and what follows from them are fp64."""
     if policy_logps.dim() != 2 or policy_logps.shape[0] % 2:
