@@ -16,8 +16,8 @@
 // the time and the schedulers 60 %.  1644 rows of 128256 bf16 logits (421 MB) take 72 us, 79 with the entropy (5.8 and 5.3 TB/s,
 // joining included; a plain copy moves 6.5).  A block of 512 threads a row took 89: 1.4 to 1.7 rounds of blocks, and waits at
 // each row's end; clusters of two or four blocks 93 and 120; eight vectors in flight 105, parts of 512 vectors 89.  A quarter of
-// the exponentials as polynomials freed the special-function unit and cost as much in instructions.  A cap asks for 15
-// instructions an element: 2103 rows of 32001 fp32 logits (269 MB) take 67 us, 41 of them the memory's.
+// the exponentials as polynomials freed the special-function unit and cost as much in instructions.  A cap's tanh asks for
+// most of the instructions: 2103 rows of 32001 fp32 logits (269 MB) take 66 us, 41 of them the memory's; issue slots are 67 % busy.
 #include <cooperative_groups.h>
 
 #include "common.cuh"
