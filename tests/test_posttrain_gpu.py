@@ -435,6 +435,23 @@ def test_inputs_changed_before_their_gradient():
         loss.backward()
 
 
+def test_log_probabilities_changed_after_their_loss():
+    """Their gradient is known by then; a loss that has to compute it again refuses."""
+    from trainscale_b200 import rl
+    logp, old, adv, mask, ref = _policy_case(6, 50, torch.float32, torch.float32, 3, spoil=False)
+    for f in (lambda x: rl.grpo_loss(x, old, ref, adv, mask), lambda x: rl.drgrpo_loss(x, old, adv, mask),
+              lambda x: rl.dapo_loss(x, old, adv, mask), lambda x: rl.preference_loss(x, ref, mask)[0]):
+        leaf = logp.clone().requires_grad_()
+        (want,) = torch.autograd.grad(f(leaf * 1), leaf)
+        x = leaf * 1
+        loss = f(x)
+        x.zero_()
+        (got,) = torch.autograd.grad(loss, leaf, retain_graph=True)
+        assert torch.equal(got, want)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            torch.autograd.grad(loss, leaf)
+
+
 def test_rows_without_an_upstream_gradient_and_unused_results():
     from trainscale_b200.rl import token_log_probs
     z = torch.randn(6, 300, device=DEV, requires_grad=True)

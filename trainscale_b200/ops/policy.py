@@ -85,7 +85,7 @@ class _Loss(torch.autograd.Function):
     def forward(ctx, logp, op, *constants):
         loss, rest, ctx.grad = op(logp, *constants, grad=True)
         ctx.save_for_backward(logp)
-        ctx.op, ctx.constants, ctx.versions = op, constants, _changed(constants)
+        ctx.op, ctx.constants, ctx.versions, ctx.dtype = op, constants, _changed(constants), logp.dtype
         ctx.captured = torch._C._cuda_isCurrentStreamCapturing()
         if rest is not None:
             ctx.mark_non_differentiable(rest)
@@ -94,7 +94,7 @@ class _Loss(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, g, _):
-        (logp,), constants = ctx.saved_tensors, ctx.constants       # (refuses a freed graph, and log-probabilities changed since)
+        constants = ctx.constants
         none = (None,) * (1 + len(constants))
         if g is None:
             return None, *none
@@ -106,12 +106,13 @@ class _Loss(torch.autograd.Function):
         if grad is not None and grad.dtype is torch.float32 and kernel:
             _lib.check(_library().ts_scale_by(grad.data_ptr(), g.data_ptr(), grad.numel(), _stream()), "ts_scale_by")
         else:
+            (logp,) = ctx.saved_tensors               # (refuses a freed graph, and log-probabilities changed since)
             if _changed(constants) != ctx.versions:
                 raise RuntimeError("an input of a policy or preference loss was changed in place before its gradient was computed")
             if not kernel:
                 return gradient(lambda x: ctx.op.plain(x, *constants)[0], logp, (g,)), *none
             grad = ctx.op(logp, *constants, grad=True if grad is None else grad, factor=g)[2]
-        return grad if grad.dtype is logp.dtype else grad.to(logp.dtype), *none
+        return grad if grad.dtype is ctx.dtype else grad.to(ctx.dtype), *none
 
 
 def native(logp, *others) -> bool:
