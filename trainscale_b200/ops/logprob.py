@@ -10,6 +10,9 @@ import math
 import struct
 
 import torch
+from torch._C import _are_functorch_transforms_active, _len_torch_dispatch_stack
+from torch._C._functorch import is_legacy_batchedtensor
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -126,9 +129,12 @@ def rows_backward_(logits: torch.Tensor, labels: torch.Tensor, kept: torch.Tenso
     _run_backward(logits, (n, n, 0, pitch), labels, kept, g, None, logits, pitch, ignore_index=ignore_index, lenient=True)
 
 
-def batched(grad: torch.Tensor | None) -> bool:
-    """Whether autograd runs one backward pass for several upstream gradients (is_grads_batched, jacobian(vectorize=True))."""
-    return grad is not None and torch._C._functorch.is_legacy_batchedtensor(grad)
+def ordinary(grad: torch.Tensor | None) -> bool:
+    """Whether a backward pass only runs, once, for this gradient: not for several at once (is_grads_batched, jacobian(vectorize=True)),
+    recorded or transformed, nor differentiated itself.  (Traces and compiled functions have no kernel's node to run; one call here, for
+    it costs more in autograd's thread than elsewhere.)"""
+    return not (torch.is_grad_enabled() or _len_torch_dispatch_stack() or _are_functorch_transforms_active() or forward_ad._current_level >= 0
+                or (grad is not None and is_legacy_batchedtensor(grad)))
 
 
 def gradient(form, x: torch.Tensor, upstream) -> torch.Tensor:
@@ -156,7 +162,7 @@ class _TokenLogProbs(torch.autograd.Function):
         logits, labels, kept = ctx.saved_tensors
         if g is None and h is None:
             return None, None, None, None
-        if torch.is_grad_enabled() or not _lib.eager() or batched(g) or batched(h):
+        if not (ordinary(g) and ordinary(h)):
             return gradient(lambda x: plain(x, labels, *ctx.how, ctx.entropy), logits, (g, h)), None, None, None
         x, rows = _rows(logits)
         grad = torch.empty_like(logits, memory_format=torch.contiguous_format)

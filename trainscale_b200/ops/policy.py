@@ -16,7 +16,7 @@ import torch
 import torch.nn.functional as F
 
 from . import _lib
-from .logprob import _DTYPES, _address, _stream, batched, fp32, gradient, on_this_gpu
+from .logprob import _DTYPES, _address, _stream, fp32, gradient, on_this_gpu, ordinary
 
 _MASKS = {torch.bool: 0, torch.uint8: 0, torch.int32: 1, torch.int64: 2, torch.float32: 3, torch.bfloat16: 4, torch.float16: 5}
 REDUCTIONS = {"sequence": 0, "token": 1, "constant": 2}
@@ -98,8 +98,7 @@ class _Loss(torch.autograd.Function):
         none = (None,) * (1 + len(constants))
         if g is None:
             return None, *none
-        # (else this gradient is differentiated or recorded itself, or several are computed at once)
-        kernel = not torch.is_grad_enabled() and _lib.eager() and not batched(g)
+        kernel = ordinary(g)
         grad, ctx.grad = ctx.grad, None
         if ctx.captured != torch._C._cuda_isCurrentStreamCapturing():
             grad = None
